@@ -48,6 +48,9 @@ EXTRA = {
     "prefill_w4_f16.hip": _VGPR_FORM,
     "prefill_w4_bf16.hip": _VGPR_FORM,
     "prefill_w4_f32.hip": _VGPR_FORM,
+    # the same for prompt attention's 256 accumulators and 128 query registers per lane
+    "attn_prompt_bf16.hip": _VGPR_FORM,
+    "attn_prompt_f16.hip": _VGPR_FORM,
 }
 
 

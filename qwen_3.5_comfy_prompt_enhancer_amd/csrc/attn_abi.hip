@@ -1,0 +1,339 @@
+// extern "C" entry points of the attention operators (declared in include/qlin_attn.h): checks
+// of arguments and launch plans.
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <stdlib.h>
+
+#include <algorithm>
+
+#include "../../include/qlin_attn.h"
+#include "attn_internal.h"
+#include "qlin_dev.h"
+#include "qlin_internal.h"
+
+using namespace qlin;
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char msg[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  return set_error(code, msg);
+}
+
+int status(const char* fn, hipError_t e) {
+  if (e == hipSuccess) return QLIN_OK;
+  return fail(QLIN_ERR_HIP, "%s: HIP error %d (%s)", fn, (int)e, hipGetErrorString(e));
+}
+
+#define QA_TRY(expr)                \
+  do {                              \
+    const int rc_ = (expr);         \
+    if (rc_ != QLIN_OK) return rc_; \
+  } while (0)
+
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+constexpr int kMaxRows = 1 << 24;             // tokens of a call (rows of a key head stay below 2^31)
+constexpr int kMaxGroup = 64;                 // query heads of a key head
+constexpr long long kMaxKeys = 1LL << 30;     // keys of a sequence
+constexpr long long kMaxTokenStride = 1LL << 26;  // eight rows' offset stays in 32 bits
+
+// One 16-bit (es = 2) or int8 tensor: n of the outer strides.  `write`: rows must not overlap.
+int check_tensor(const char* fn, const char* name, const void* p, int es, int hd, long long n0, long long s0,
+                 long long n1, long long s1, bool write) {
+  const int mult = es == 1 ? 16 : 8;
+  if (!p) return fail(QLIN_ERR_INVALID, "%s: null %s", fn, name);
+  if (!aligned(p, 16) || s0 % mult || s1 % mult || s0 < 0 || s1 < 0)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: %s must be 16-byte aligned with strides that are multiples of %d", fn, name,
+                mult);
+  if (s0 > kMaxTokenStride || s1 > kMaxTokenStride)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: strides of %s above %lld", fn, name, kMaxTokenStride);
+  if (write && ((n0 > 1 && s0 < hd) || (n1 > 1 && s1 < hd)))
+    return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, name);
+  return QLIN_OK;
+}
+
+int check_heads(const char* fn, int hq, int hkv, int hd, int dtype) {
+  if (hq <= 0 || hkv <= 0 || hq % hkv != 0)
+    return fail(QLIN_ERR_INVALID, "%s: %d query heads must be a multiple of %d key heads", fn, hq, hkv);
+  if (hq / hkv > kMaxGroup)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d query heads to a key head", fn, kMaxGroup);
+  if (hd != 64 && hd != 128 && hd != 256)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: head size %d (need 64, 128 or 256)", fn, hd);
+  if (dtype != QLIN_BF16 && dtype != QLIN_F16)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: dtype %d (need bf16 or fp16)", fn, dtype);
+  return QLIN_OK;
+}
+
+int check_scale(const char* fn, float scale) {
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(QLIN_ERR_INVALID, "%s: scale must be positive", fn);
+  return QLIN_OK;
+}
+
+int check_cache(const char* fn, const qlin_paged_kv* c, int hkv, int hd, int dtype, bool write, PagedTensor& k,
+                PagedTensor& v) {
+  if (!c) return fail(QLIN_ERR_INVALID, "%s: null cache", fn);
+  if (c->dtype != QLIN_I8 && c->dtype != dtype)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: cache dtype %d (need int8 or the queries' type)", fn, c->dtype);
+  if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)))
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: page of %d tokens (need a power of two from 16 to 1024)", fn, c->page);
+  if (c->num_pages <= 0) return fail(QLIN_ERR_INVALID, "%s: a cache of no pages", fn);
+  const bool q8 = c->dtype == QLIN_I8;
+  const int es = q8 ? 1 : 2, mult = q8 ? 16 : 8;
+  QA_TRY(check_tensor(fn, "k_cache", c->k, es, hd, c->page, c->k_token, hkv, c->k_head, write));
+  QA_TRY(check_tensor(fn, "v_cache", c->v, es, hd, c->page, c->v_token, hkv, c->v_head, write));
+  if (c->k_page % mult || c->v_page % mult || c->k_page < 0 || c->v_page < 0)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides must be multiples of %d", fn, mult);
+  if (write && c->num_pages > 1 && (c->k_page < hd || c->v_page < hd))
+    return fail(QLIN_ERR_INVALID, "%s: pages of the cache overlap", fn);
+  if (q8) {
+    if (!c->k_s || !c->v_s) return fail(QLIN_ERR_INVALID, "%s: an int8 cache needs k_s and v_s", fn);
+    if (!aligned(c->k_s, 4) || !aligned(c->v_s, 4))
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: scales must be 4-byte aligned", fn);
+    const int64_t st[6] = {c->ks_page, c->ks_token, c->ks_head, c->vs_page, c->vs_token, c->vs_head};
+    const int n[3] = {c->num_pages, c->page, hkv};
+    for (int i = 0; i < 6; ++i) {
+      if (st[i] < 0) return fail(QLIN_ERR_UNSUPPORTED, "%s: negative stride of the scales", fn);
+      if (write && n[i % 3] > 1 && st[i] < 1) return fail(QLIN_ERR_INVALID, "%s: scales of the cache overlap", fn);
+    }
+  } else if (c->k_s || c->v_s) {
+    return fail(QLIN_ERR_INVALID, "%s: a 16-bit cache has no scales", fn);
+  }
+  k = PagedTensor{c->k, c->k_page, c->k_token, c->k_head, c->k_s, c->ks_page, c->ks_token, c->ks_head};
+  v = PagedTensor{c->v, c->v_page, c->v_token, c->v_head, c->v_s, c->vs_page, c->vs_token, c->vs_head};
+  return QLIN_OK;
+}
+
+int shift_of(int page) { return __builtin_ctz((unsigned)page); }
+
+int check_paged(const char* fn, const qlin_paged_kv* cache, const int* table, int64_t table_stride, int max_pages,
+                const int* kv_len, int hkv, int hd, int dtype, KvSrc& kv) {
+  QA_TRY(check_cache(fn, cache, hkv, hd, dtype, false, kv.k, kv.v));
+  if (!table || !kv_len) return fail(QLIN_ERR_INVALID, "%s: null page table or lengths", fn);
+  if (!aligned(table, 4) || !aligned(kv_len, 4))
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: table and kv_len must be 4-byte aligned", fn);
+  if (max_pages < 0 || table_stride < 0) return fail(QLIN_ERR_INVALID, "%s: negative page table size", fn);
+  if ((long long)max_pages * cache->page > kMaxKeys)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %lld keys a sequence", fn, kMaxKeys);
+  kv.table = table;
+  kv.table_stride = table_stride;
+  kv.num_pages = cache->num_pages;
+  kv.max_pages = max_pages;
+  kv.page_shift = shift_of(cache->page);
+  kv.len = kv_len;
+  kv.cu = nullptr;
+  kv.rows = 0;
+  return QLIN_OK;
+}
+
+// The partial sums' place in the workspace, behind its counters and exchange slots.
+int workspace_parts(const char* fn, void* ws, size_t bytes, char** part, size_t* avail) {
+  const size_t base = counter_bytes() + poll_bytes();
+  if (!ws || bytes < base) return fail(QLIN_ERR_WORKSPACE, "%s: workspace missing or too small", fn);
+  if (!aligned(ws, 256)) return fail(QLIN_ERR_INVALID, "%s: workspace must be 256-byte aligned", fn);
+  *part = (char*)ws + base;
+  *avail = bytes - base;
+  return QLIN_OK;
+}
+
+// Row tiles and key cuts of a prompt call.
+int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void* ws, size_t ws_bytes, int& rs) {
+  char* part;
+  size_t avail;
+  QA_TRY(workspace_parts(fn, ws, ws_bytes, &part, &avail));
+  const long long rows = (long long)a.T * a.G;
+  rs = rows > 128 ? 2 : 1;
+  long long target = 512;
+  if (const char* e = getenv("QLIN_PROMPT")) {  // "row sets,units" for tuning runs
+    int r = 0, t = -1;
+    if (sscanf(e, "%d,%d", &r, &t) == 2) {
+      if (r == 1 || r == 2) rs = r;
+      if (t >= 0) target = t;
+    }
+  }
+  const long long tiles = rows / prompt_rows(rs) + a.B;
+  const long long slot = prompt_slot_floats(rs, hd) * 4;
+  if (tiles * a.HKV >= 1024 || max_keys <= kPromptMinBlocks * kPromptBlock) target = 0;
+  // every unit of a key head has a slot: at most 2 target / HKV + tiles of them
+  target = std::min(target, ((long long)avail / slot / a.HKV - tiles - 1) * a.HKV / 2);
+  if (target <= a.HKV) target = 0;
+  a.target = (int)target;
+  a.tiles = (int)tiles;
+  a.units = (int)(tiles + (2 * target + a.HKV - 1) / a.HKV);
+  a.part = (float*)part;
+  return QLIN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qlin_qk_norm_rope(const qlin_rope* r, void* stream) {
+  const char* fn = "qlin_qk_norm_rope";
+  set_error(QLIN_OK, "");
+  if (!r) return fail(QLIN_ERR_INVALID, "%s: null arguments", fn);
+  if (r->T < 0) return fail(QLIN_ERR_INVALID, "%s: negative size", fn);
+  QA_TRY(check_heads(fn, r->q_heads, r->kv_heads, r->hd, r->dtype));
+  if (r->rot < 0 || r->rot > r->hd || r->rot % 16)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: %d rotated values (need a multiple of 16 up to the head size)", fn, r->rot);
+  if (r->axes < 1 || r->axes > 3) return fail(QLIN_ERR_UNSUPPORTED, "%s: %d position axes (need 1 to 3)", fn, r->axes);
+  int sum = 0;
+  for (int i = 0; i < r->axes; ++i) {
+    if (r->sections[i] < 0) return fail(QLIN_ERR_INVALID, "%s: negative section", fn);
+    sum += r->sections[i];
+    if (r->interleaved && i > 0 && r->sections[i] > 0 && r->axes * (r->sections[i] - 1) + i >= r->rot / 2)
+      return fail(QLIN_ERR_INVALID, "%s: axis %d has no %d turns among %d frequencies", fn, i, r->sections[i],
+                  r->rot / 2);
+  }
+  if (sum != r->rot / 2)
+    return fail(QLIN_ERR_INVALID, "%s: sections add up to %d, not %d frequencies", fn, sum, r->rot / 2);
+  if (r->T == 0) return QLIN_OK;
+  if (r->T > kMaxRows) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens", fn, kMaxRows);
+  QA_TRY(check_tensor(fn, "q", r->q, 2, r->hd, r->T, r->q_token, r->q_heads, r->q_head, false));
+  QA_TRY(check_tensor(fn, "k", r->k, 2, r->hd, r->T, r->k_token, r->kv_heads, r->k_head, false));
+  QA_TRY(check_tensor(fn, "q_out", r->q_out, 2, r->hd, r->T, r->qo_token, r->q_heads, r->qo_head, true));
+  if (r->k_out) QA_TRY(check_tensor(fn, "k_out", r->k_out, 2, r->hd, r->T, r->ko_token, r->kv_heads, r->ko_head, true));
+  if (!r->k_out && !r->cache) return fail(QLIN_ERR_INVALID, "%s: neither k_out nor a cache for the keys", fn);
+  if (r->rot > 0 && (!r->pos || !r->freqs)) return fail(QLIN_ERR_INVALID, "%s: null positions or frequencies", fn);
+  if (!aligned(r->pos, r->pos_64 ? 8 : 4) || !aligned(r->freqs, r->freqs_64 ? 8 : 4))
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: positions and frequencies must be aligned to their size", fn);
+  if (r->q_w || r->k_w) {
+    if (r->w_dtype != QLIN_BF16 && r->w_dtype != QLIN_F16 && r->w_dtype != QLIN_F32)
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: norm weight dtype %d", fn, r->w_dtype);
+    if (!aligned(r->q_w, 4) || !aligned(r->k_w, 4))
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: norm weights must be 4-byte aligned", fn);
+  }
+  RopeArgs a = {};
+  if (r->cache) {
+    if (!r->v || !r->slots) return fail(QLIN_ERR_INVALID, "%s: a cache needs values and slots", fn);
+    if (!aligned(r->slots, r->slots_64 ? 8 : 4))
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: slots must be aligned to their size", fn);
+    QA_TRY(check_tensor(fn, "v", r->v, 2, r->hd, r->T, r->v_token, r->kv_heads, r->v_head, false));
+    QA_TRY(check_cache(fn, r->cache, r->kv_heads, r->hd, r->dtype, true, a.kc, a.vc));
+    a.page_shift = shift_of(r->cache->page);
+    a.nslots = (long long)r->cache->num_pages * r->cache->page;
+  }
+  a.q = r->q, a.qt = r->q_token, a.qh = r->q_head;
+  a.k = r->k, a.kt = r->k_token, a.kh = r->k_head;
+  a.v = r->cache ? r->v : nullptr, a.vt = r->v_token, a.vh = r->v_head;
+  a.qo = r->q_out, a.qot = r->qo_token, a.qoh = r->qo_head;
+  a.ko = r->k_out, a.kot = r->ko_token, a.koh = r->ko_head;
+  a.slots = r->slots, a.slots64 = r->slots_64;
+  a.pos = r->pos, a.pos_a = r->pos_axis, a.pos_t = r->pos_token, a.pos64 = r->pos_64;
+  a.freqs = r->freqs, a.freqs64 = r->freqs_64;
+  a.qw = r->q_w, a.kw = r->k_w, a.wdt = r->w_dtype, a.one_plus = r->one_plus, a.eps = r->eps;
+  a.T = r->T, a.HQ = r->q_heads, a.HKV = r->kv_heads, a.hd = r->hd, a.rot = r->rot;
+  a.axes = r->axes, a.interleaved = r->interleaved, a.dt = r->dtype;
+  for (int i = 0; i < 3; ++i) a.sec[i] = i < r->axes ? r->sections[i] : 0;
+  return status(fn, launch_rope(a, (hipStream_t)stream));
+}
+
+int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                     const void* v, int64_t v_token, int64_t v_head, const int* cu_q, const int* cu_k, void* out,
+                     int64_t o_token, int64_t o_head, int T, int Tk, int B, int q_heads, int kv_heads, int hd,
+                     int dtype, float scale, int causal, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "qlin_attn_prompt";
+  set_error(QLIN_OK, "");
+  if (T < 0 || Tk < 0 || B < 0) return fail(QLIN_ERR_INVALID, "%s: negative size", fn);
+  QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
+  QA_TRY(check_scale(fn, scale));
+  if (T == 0 || B == 0) return QLIN_OK;
+  if (T > kMaxRows || Tk > kMaxRows || B > kMaxRows)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens or sequences", fn, kMaxRows);
+  if (!cu_q || !cu_k) return fail(QLIN_ERR_INVALID, "%s: null row bounds", fn);
+  if (!aligned(cu_q, 4) || !aligned(cu_k, 4))
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: row bounds must be 4-byte aligned", fn);
+  QA_TRY(check_tensor(fn, "q", q, 2, hd, T, q_token, q_heads, q_head, false));
+  QA_TRY(check_tensor(fn, "out", out, 2, hd, T, o_token, q_heads, o_head, true));
+  if (Tk > 0) {
+    QA_TRY(check_tensor(fn, "k", k, 2, hd, Tk, k_token, kv_heads, k_head, false));
+    QA_TRY(check_tensor(fn, "v", v, 2, hd, Tk, v_token, kv_heads, v_head, false));
+  }
+  PromptArgs a = {};
+  a.q = q, a.qt = q_token, a.qh = q_head;
+  a.o = out, a.ot = o_token, a.oh = o_head;
+  a.kv.k = PagedTensor{const_cast<void*>(k), 0, k_token, k_head, nullptr, 0, 0, 0};
+  a.kv.v = PagedTensor{const_cast<void*>(v), 0, v_token, v_head, nullptr, 0, 0, 0};
+  a.kv.cu = cu_k, a.kv.rows = Tk;
+  a.cu = cu_q, a.T = T, a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
+  a.causal = causal, a.c = scale * 1.44269504088896340736f;
+  int rs;
+  QA_TRY(plan_prompt(fn, a, hd, Tk, workspace, workspace_bytes, rs));
+  return status(fn, launch_prompt(a, dtype, hd, rs, (hipStream_t)stream));
+}
+
+int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const qlin_paged_kv* cache,
+                           const int* table, int64_t table_stride, int max_pages, const int* kv_len, const int* cu_q,
+                           void* out, int64_t o_token, int64_t o_head, int T, int B, int q_heads, int kv_heads,
+                           int hd, int dtype, float scale, int causal, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  const char* fn = "qlin_attn_prompt_paged";
+  set_error(QLIN_OK, "");
+  if (T < 0 || B < 0) return fail(QLIN_ERR_INVALID, "%s: negative size", fn);
+  QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
+  QA_TRY(check_scale(fn, scale));
+  if (T == 0 || B == 0) return QLIN_OK;
+  if (T > kMaxRows || B > kMaxRows)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens or sequences", fn, kMaxRows);
+  if (!cu_q) return fail(QLIN_ERR_INVALID, "%s: null row bounds", fn);
+  if (!aligned(cu_q, 4)) return fail(QLIN_ERR_UNSUPPORTED, "%s: row bounds must be 4-byte aligned", fn);
+  QA_TRY(check_tensor(fn, "q", q, 2, hd, T, q_token, q_heads, q_head, false));
+  QA_TRY(check_tensor(fn, "out", out, 2, hd, T, o_token, q_heads, o_head, true));
+  PromptArgs a = {};
+  QA_TRY(check_paged(fn, cache, table, table_stride, max_pages, kv_len, kv_heads, hd, dtype, a.kv));
+  a.q = q, a.qt = q_token, a.qh = q_head;
+  a.o = out, a.ot = o_token, a.oh = o_head;
+  a.cu = cu_q, a.T = T, a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
+  a.causal = causal, a.c = scale * 1.44269504088896340736f;
+  int rs;
+  QA_TRY(plan_prompt(fn, a, hd, (long long)max_pages * cache->page, workspace, workspace_bytes, rs));
+  return status(fn, launch_prompt(a, dtype, hd, rs, (hipStream_t)stream));
+}
+
+int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_paged_kv* cache, const int* table,
+                     int64_t table_stride, int max_pages, const int* kv_len, void* out, int64_t o_seq,
+                     int64_t o_head, int B, int q_heads, int kv_heads, int hd, int dtype, float scale,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "qlin_attn_decode";
+  set_error(QLIN_OK, "");
+  if (B < 0) return fail(QLIN_ERR_INVALID, "%s: negative size", fn);
+  QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
+  QA_TRY(check_scale(fn, scale));
+  if (B == 0) return QLIN_OK;
+  if (B > kMaxRows / kv_heads) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d rows", fn, kMaxRows);
+  QA_TRY(check_tensor(fn, "q", q, 2, hd, B, q_seq, q_heads, q_head, false));
+  QA_TRY(check_tensor(fn, "out", out, 2, hd, B, o_seq, q_heads, o_head, true));
+  DecodeArgs a = {};
+  QA_TRY(check_paged(fn, cache, table, table_stride, max_pages, kv_len, kv_heads, hd, dtype, a.kv));
+  char* part;
+  size_t avail;
+  QA_TRY(workspace_parts(fn, workspace, workspace_bytes, &part, &avail));
+  a.q = q, a.qb = q_seq, a.qh = q_head;
+  a.o = out, a.ob = o_seq, a.oh = o_head;
+  a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
+  a.gb = (a.G + 15) / 16;
+  a.c = scale * 1.44269504088896340736f;
+  const long long hg = (long long)kv_heads * a.gb;
+  const long long blocks = ((long long)max_pages * cache->page + kDecodeBlock - 1) / kDecodeBlock;
+  long long total = 512;
+  if (const char* e = getenv("QLIN_DECODE_UNITS")) {  // for tuning runs
+    if (atoi(e) > 0) total = atoi(e);
+  }
+  long long target = std::min(std::max(1LL, total / hg), std::max(1LL, B * ((blocks + kDecodeChunk - 1) / kDecodeChunk)));
+  const long long slot = (long long)decode_slot_floats(std::min(16, a.G), hd) * 4;
+  // without room for the parts (very many sequences) every sequence is one unit
+  if ((target + B) * hg * slot > (long long)avail || B * hg * kDecodeCounters * 4 > (long long)counter_bytes())
+    target = 0;
+  a.target = (int)target;
+  a.units = (int)(target + B);
+  a.part = (float*)part;
+  a.cnt = (unsigned*)workspace;
+  return status(fn, launch_decode(a, dtype, hd, (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,452 @@
+// Attention of one new token per sequence over a paged key-value cache.
+//
+//   o[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max),  j < len[b]
+//
+// Bound by the bytes of the cache: each key and value is read once for all query heads of its
+// key head (up to 16 a launch unit; more take further units).  The keys of all sequences are
+// cut into units of about the same number of 32-key blocks, so that a ragged batch fills the
+// chip evenly; every workgroup finds its unit from the sequences' lengths on the device.
+//
+// A workgroup's four waves take blocks in turn.  A block runs without LDS:
+//   * scores: S^T = K Q^T on 16x16x32 MFMAs, K rows straight from memory as the A operand
+//     (16 keys; a lane loads 16 bytes of one key), all query heads as the columns of B;
+//   * P^T leaves the score layout as the B operand of O^T = V^T P^T without crossing lanes: lane
+//     group g holds keys 4g .. 4g+3 and 16 + 4g .. 16 + 4g+3 of the block, and V's rows are
+//     loaded in that order;
+//   * V: a lane loads 8 keys' next hd/16 values; byte permutes pair the keys of a column, so
+//     that column c of all lanes is an A operand of 16 value columns;
+//   * int8: codes become 16-bit whole numbers (exact); a key's scale multiplies its scores in 32
+//     bits, a value's scale its probability.
+// The running maximum is a column's, hence a lane's own.  P is rounded to 16 bits for its
+// product (half a step of 2^-8 or 2^-11 of each term; the sum of P is of the unrounded); with
+// int8 values P times scale goes as bf16, whose range a small scale cannot leave.
+//
+// Waves join through LDS, units of a sequence through memory: the last of 16 units to arrive
+// adds their parts in unit order, the last of those groups adds the groups', so that the result
+// does not depend on the order of arrival and no workgroup reads more than 16 parts.
+#include "attn_dev.h"
+
+namespace qlin {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+
+// Unit -> (sequence, part): all units of a (key head, group) numbered by sequence.
+struct Unit {
+  int b, s;       // sequence, its part
+  int len;        // keys of the sequence
+  int chunk;      // blocks of a part
+  int parts;
+  int base;       // number of part 0
+};
+
+__device__ __forceinline__ long long wave_sum(long long v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+__device__ __forceinline__ int blocks_of(int len) { return (len + kDecodeBlock - 1) / kDecodeBlock; }
+
+__device__ __forceinline__ bool find_unit(const DecodeArgs& a, int u, Unit& r) {
+  const int lane = (int)threadIdx.x & 63;
+  long long total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) total += b0 + lane < a.B ? blocks_of(kv_length(a.kv, b0 + lane)) : 0;
+  total = wave_sum(total);
+  int chunk = 1 << 28;
+  if (a.target > 0) {
+    chunk = (int)((total + a.target - 1) / a.target);
+    chunk = (max(chunk, 1) + kDecodeChunk - 1) / kDecodeChunk * kDecodeChunk;
+  }
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int len = b0 + lane < a.B ? kv_length(a.kv, b0 + lane) : 0;
+    // an empty sequence has one part, which writes its zeros
+    const int parts = b0 + lane < a.B ? max(1, (blocks_of(len) + chunk - 1) / chunk) : 0;
+    int end = parts;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int o = __shfl_up(end, m);
+      if (lane >= m) end += o;
+    }
+    const int sum = __shfl(end, 63);
+    if (u < base + sum) {
+      const uint64_t past = __ballot(base + end > u);
+      const int at = __builtin_ctzll(past);
+      r.b = b0 + at;
+      r.len = (int)rfl32((uint32_t)__shfl(len, at));
+      r.parts = (int)rfl32((uint32_t)__shfl(parts, at));
+      r.base = (int)rfl32((uint32_t)(base + __shfl(end - parts, at)));
+      r.s = u - r.base;
+      r.chunk = chunk;
+      return true;
+    }
+    base += sum;
+  }
+  return false;
+}
+
+__device__ __forceinline__ float group_max(float v) {  // over the four lanes of a column
+  float x, y;
+  lane_pair<16>(v, x, y);
+  v = fmaxf(x, y);
+  lane_pair<32>(v, x, y);
+  return fmaxf(x, y);
+}
+
+__device__ __forceinline__ float group_sum(float v) {
+  float x, y;
+  lane_pair<16>(v, x, y);
+  v = x + y;
+  lane_pair<32>(v, x, y);
+  return x + y;
+}
+
+// Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
+  return T::pack_exact((float)(int8_t)(w0 >> (8 * c)), (float)(int8_t)(w1 >> (8 * c)));
+}
+
+// n values of a part, four at a time (float4 f of `rows * HD / 4`), and a row's maximum and sum
+// behind them: a part's layout in memory.
+template <int HD>
+__device__ __forceinline__ unsigned part_ml(int rows) {
+  return (unsigned)(rows * HD * 4);
+}
+
+template <typename T, int HD, bool Q8>
+__global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a) {
+  constexpr int STEPS = HD / 32;                 // score MFMAs of 16 keys
+  constexpr int VW = HD >= 128 && !Q8 ? 8 : HD / 16;  // adjacent value columns of a lane
+  constexpr int VC = HD / 16 / VW;               // runs of them, 16 VW columns apart
+  constexpr int KL = Q8 ? HD / 64 : HD / 32;     // 16-byte loads of a key
+  using TV = std::conditional_t<Q8, Bf16, T>;    // type of P and V in their product
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ int s_last;
+
+  const int hg = a.HKV * a.gb;
+  const int hh = (int)blockIdx.x % hg, unit = (int)blockIdx.x / hg;
+  Unit U;
+  if (!find_unit(a, unit, U)) return;
+  const int hk = hh % a.HKV, gi = hh / a.HKV;
+  const int rows = min(16, a.G - 16 * gi);
+  const int head0 = hk * a.G + 16 * gi;
+  const int tid = (int)threadIdx.x;
+  const int wave = (int)rfl32((uint32_t)tid >> 6), lane = tid & 63;
+  const int j = lane & 15, g = lane >> 4;
+  const uint16_t* q = (const uint16_t*)a.q + U.b * a.qb + head0 * a.qh;
+  uint16_t* out = (uint16_t*)a.o + U.b * a.ob + head0 * a.oh;
+
+  if (U.len == 0) {
+    for (int f = tid; f < rows * (HD / 8); f += kThreads)
+      *(u32x4*)(out + (f / (HD / 8)) * a.oh + (f % (HD / 8)) * 8) = u32x4{0, 0, 0, 0};
+    return;
+  }
+
+  // query operand: column j = head j, the same hd order as a key's loads
+  u32x4 qv[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int d = Q8 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
+    qv[s] = u32x4{0, 0, 0, 0};
+    if (j < rows) qv[s] = ld_global<u32x4>(q + j * a.qh + d);
+  }
+
+  f32x4 O[VC * VW];
+#pragma unroll
+  for (int c = 0; c < VC * VW; ++c) O[c] = f32x4{0, 0, 0, 0};
+  float m = kNegInf, l = 0.0f;
+  bool bad = false;
+
+  const int len = U.len;
+  const int nblk = blocks_of(len);
+  const int blk1 = (int)min((long long)nblk, (U.s + 1LL) * U.chunk);
+  const int* table = a.kv.table + U.b * a.kv.table_stride;
+  const long long pmask = (1LL << a.kv.page_shift) - 1;
+  constexpr int ES = Q8 ? 1 : 2;
+
+  for (int blk = U.s * U.chunk + wave; blk < blk1; blk += kWaves) {
+    const int key0 = blk * kDecodeBlock;
+    // the two halves of 16 keys lie in one page each; keys behind the last are the last again
+    const uint8_t *kp[2], *vp[2];
+    const float *ksp[2], *vsp[2];
+    int top[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int hs = min(key0 + 16 * h, (len - 1) & ~15);
+      top[h] = min(15, len - 1 - hs);
+      int pid = table[hs >> a.kv.page_shift];
+      if ((unsigned)pid >= (unsigned)a.kv.num_pages) {
+        bad = true;
+        pid = 0;
+      }
+      const long long off = hs & pmask;
+      kp[h] = (const uint8_t*)a.kv.k.p + (pid * a.kv.k.sp + off * a.kv.k.st + hk * a.kv.k.sh) * ES;
+      vp[h] = (const uint8_t*)a.kv.v.p + (pid * a.kv.v.sp + off * a.kv.v.st + hk * a.kv.v.sh) * ES;
+      if constexpr (Q8) {
+        ksp[h] = a.kv.k.s + pid * a.kv.k.ssp + off * a.kv.k.sst + hk * a.kv.k.ssh;
+        vsp[h] = a.kv.v.s + pid * a.kv.v.ssp + off * a.kv.v.sst + hk * a.kv.v.ssh;
+      }
+    }
+    u32x4 kr[2][KL];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < KL; ++i)
+        kr[h][i] = ld_global_nt<u32x4>(kp[h] + min(j, top[h]) * a.kv.k.st * ES + i * 64 + g * 16);
+    // value rows: slot s of lane group g is key 4g + s (s < 4) or 16 + 4g + s - 4
+    constexpr int VB = VW * ES;  // bytes of a run
+    typedef std::conditional_t<VB == 16, u32x4, std::conditional_t<VB == 8, u32x2, uint32_t>> VReg;
+    VReg vr[8][VC];
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int c = 0; c < VC; ++c)
+        vr[s][c] = ld_global_nt<VReg>(vp[s / 4] + min(4 * g + s % 4, top[s / 4]) * a.kv.v.st * ES + c * 16 * VB +
+                                      j * VB);
+    float ks[8], vs[8];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const int r = min(4 * g + s % 4, top[s / 4]);
+        ks[s] = ksp[s / 4][r * a.kv.k.sst];
+        vs[s] = vsp[s / 4][r * a.kv.v.sst];
+      }
+    }
+
+    float t[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 S = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        u32x4 kop;
+        if constexpr (Q8) {
+          const u32x4 r = kr[h][s / 2];
+          const uint32_t w0 = s % 2 ? r.z : r.x, w1 = s % 2 ? r.w : r.y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = e < 2 ? w0 : w1;
+            const int c = 2 * (e % 2);
+            kop[e] = T::pack_exact((float)(int8_t)(w >> (8 * c)), (float)(int8_t)(w >> (8 * c + 8)));
+          }
+        } else {
+          kop = kr[h][s];
+        }
+        S = T::mma16(kop, qv[s], S);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = Q8 ? S[i] * ks[4 * h + i] : S[i];
+        t[4 * h + i] = key0 + 16 * h + 4 * g + i < len ? x * a.c : kNegInf;
+      }
+    }
+    float mx = t[0];
+#pragma unroll
+    for (int s = 1; s < 8; ++s) mx = fmaxf(mx, t[s]);
+    const float mn = fmaxf(m, group_max(mx));
+    const float ms = mn == kNegInf ? 0.0f : mn;
+    const float al = exp2_(m - ms);
+    m = mn;
+    float p[8], ps = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      p[s] = exp2_(t[s] - ms);
+      ps += p[s];
+    }
+    l = l * al + ps;
+    u32x4 pop;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      pop[e] = Q8 ? TV::pack(p[2 * e] * vs[2 * e], p[2 * e + 1] * vs[2 * e + 1]) : TV::pack(p[2 * e], p[2 * e + 1]);
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int x = 0; x < VW; ++x) {
+        u32x4 vop;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w0, w1;
+          constexpr int PER = 4 / ES;  // columns of a dword
+          if constexpr (VB == 4) {
+            w0 = vr[2 * e][c];
+            w1 = vr[2 * e + 1][c];
+          } else {
+            w0 = vr[2 * e][c][x / PER];
+            w1 = vr[2 * e + 1][c][x / PER];
+          }
+          vop[e] = Q8 ? codes2<TV>(w0, w1, x % PER) : perm(w1, w0, x % 2 ? 0x07060302u : 0x05040100u);
+        }
+        f32x4& o = O[c * VW + x];
+        o = TV::mma16(vop, pop, f32x4{o[0] * al, o[1] * al, o[2] * al, o[3] * al});
+      }
+  }
+  if (bad) l = __builtin_nanf("");  // a page outside the cache: its sequence's output is NaN
+  l = group_sum(l);
+
+  // waves join in LDS: wave w's sums at w * rows * HD, maxima and sums of P behind all of them
+  float* mlw = lds + kWaves * rows * HD;
+  if (j < rows) {
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* dst = lds + (wave * rows + j) * HD + c * 16 * VW + VW * (4 * g + i);
+#pragma unroll
+        for (int x = 0; x < VW; x += 4)
+          *(f32x4*)(dst + x) = f32x4{O[c * VW + x][i], O[c * VW + x + 1][i], O[c * VW + x + 2][i], O[c * VW + x + 3][i]};
+      }
+    if (g == 0) {
+      mlw[(wave * 16 + j) * 2] = m;
+      mlw[(wave * 16 + j) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+
+  const int nf = rows * (HD / 4);
+  const unsigned slot_bytes = (unsigned)decode_slot_floats(min(16, a.G), HD) * 4u;
+  const long long upart = (long long)hh * a.units + U.base;  // number of the sequence's first part
+  const __amdgpu_buffer_rsrc_t rs = part_rsrc((const char*)a.part + upart * slot_bytes, (unsigned)U.parts * slot_bytes);
+  auto store_out = [&](int f, f32x4 o, float ls) {
+    const float inv = 1.0f / ls;
+    const uint32_t lo = T::pack(o[0] * inv, o[1] * inv), hi = T::pack(o[2] * inv, o[3] * inv);
+    *(u32x2*)(out + (f / (HD / 4)) * a.oh + (f % (HD / 4)) * 4) = u32x2{lo, hi};
+  };
+  auto store_part = [&](int part, int f, f32x4 o, float M, float ls) {
+    const unsigned at = (unsigned)part * slot_bytes;
+    st_coherent(o, rs, at + (unsigned)f * 16u);
+    if (f % (HD / 4) == 0)
+      st_coherent(f32x4{M, ls, 0, 0}, rs, at + part_ml<HD>(rows) + (unsigned)(f / (HD / 4)) * 16u);
+  };
+
+  for (int f = tid; f < nf; f += kThreads) {
+    const int r = f / (HD / 4);
+    float M = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, mlw[(w * 16 + r) * 2]);
+    const float Ms = M == kNegInf ? 0.0f : M;
+    f32x4 o = {0, 0, 0, 0};
+    float ls = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float e = exp2_(mlw[(w * 16 + r) * 2] - Ms);
+      const f32x4 x = *(const f32x4*)(lds + w * rows * HD + f * 4);
+      o += x * e;
+      ls += mlw[(w * 16 + r) * 2 + 1] * e;
+    }
+    if (U.parts == 1) store_out(f, o, ls);
+    else store_part(U.s, f, o, M, ls);
+  }
+  if (U.parts == 1) return;
+
+  // adds parts first, first + step, ... (n of them) in order
+  auto join = [&](int first, int step, int n, auto&& put) {
+    for (int f = tid; f < nf; f += kThreads) {
+      const unsigned ml = part_ml<HD>(rows) + (unsigned)(f / (HD / 4)) * 16u;
+      f32x4 o = {0, 0, 0, 0};
+      float M = kNegInf, ls = 0.0f;
+      for (int i0 = 0; i0 < n; i0 += 8) {
+        f32x4 x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const unsigned at = (unsigned)(first + min(i0 + i, n - 1) * step) * slot_bytes;
+          x[i] = ld_coherent(rs, at + (unsigned)f * 16u);
+          y[i] = ld_coherent(rs, at + ml);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i0 + i >= n) break;
+          const float mn = fmaxf(M, y[i][0]);
+          const float ms = mn == kNegInf ? 0.0f : mn;
+          const float e0 = exp2_(M - ms), e1 = exp2_(y[i][0] - ms);
+          o = o * e0 + x[i] * e1;
+          ls = ls * e0 + y[i][1] * e1;
+          M = mn;
+        }
+      }
+      put(f, o, M, ls);
+    }
+  };
+  // whether this workgroup is the last of n at counter c (its stores done), which it then clears
+  auto last_of = [&](unsigned* c, int n) {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (tid == 0) {
+      const unsigned prev = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int last = prev == (unsigned)(n - 1);
+      if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = last;
+    }
+    __syncthreads();
+    const bool r = s_last != 0;
+    __syncthreads();
+    return r;
+  };
+
+  unsigned* cnt = a.cnt + ((long long)U.b * hg + hh) * kDecodeCounters;
+  // groups of 16 parts, or more where there would be more of them than counters
+  const int per = max(kDecodeGroup, (U.parts + kDecodeCounters - 2) / (kDecodeCounters - 1));
+  const int groups = (U.parts + per - 1) / per;
+  const int gq = U.s / per;
+  const int first = gq * per, members = min(per, U.parts - first);
+  if (!last_of(cnt + 1 + gq, members)) return;
+  if (groups == 1) {
+    join(0, 1, members, [&](int f, f32x4 o, float, float ls) { store_out(f, o, ls); });
+    return;
+  }
+  // a group's sum takes the place of its first part (read before by the same thread alone: the
+  // maximum and sum behind a row's values are read by all of its threads, hence the barrier)
+  {
+    constexpr int MAXF = 16 * (HD / 4) / kThreads < 1 ? 1 : 16 * (HD / 4) / kThreads;
+    f32x4 keep[MAXF];
+    float km[MAXF], kl[MAXF];
+    int at = 0;
+    join(first, 1, members, [&](int, f32x4 o, float M, float ls) {
+#pragma unroll
+      for (int x = 0; x < MAXF; ++x)
+        if (x == at) keep[x] = o, km[x] = M, kl[x] = ls;
+      ++at;
+    });
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < MAXF; ++x) {
+      const int f = tid + x * kThreads;
+      if (f < nf) store_part(first, f, keep[x], km[x], kl[x]);
+    }
+  }
+  if (!last_of(cnt, groups)) return;
+  join(0, per, groups, [&](int f, f32x4 o, float, float ls) { store_out(f, o, ls); });
+}
+
+template <typename T, int HD>
+hipError_t launch(const DecodeArgs& a, hipStream_t st) {
+  const int rows = a.G < 16 ? a.G : 16;
+  const size_t lds = ((size_t)kWaves * rows * HD + kWaves * 32) * sizeof(float);
+  const dim3 grid((unsigned)(a.units * a.HKV * a.gb));
+  if (a.kv.k.s) hipLaunchKernelGGL((decode_kernel<T, HD, true>), grid, dim3(kThreads), lds, st, a);
+  else hipLaunchKernelGGL((decode_kernel<T, HD, false>), grid, dim3(kThreads), lds, st, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_hd(const DecodeArgs& a, int hd, hipStream_t st) {
+  if (hd == 256) return launch<T, 256>(a, st);
+  if (hd == 128) return launch<T, 128>(a, st);
+  return launch<T, 64>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_decode(const DecodeArgs& a, int dt, int hd, hipStream_t st) {
+  return dt == DT_BF16 ? launch_hd<Bf16>(a, hd, st) : launch_hd<F16>(a, hd, st);
+}
+
+}  // namespace qlin

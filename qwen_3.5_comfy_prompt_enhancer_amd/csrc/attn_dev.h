@@ -1,0 +1,66 @@
+// Device helpers of the attention kernels (gfx950): element types, MFMA products, and the
+// place of a sequence's keys in memory.
+#pragma once
+
+#include "attn_internal.h"
+#include "qlin_dev.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+namespace qlin {
+
+constexpr float kNegInf = -__builtin_inff();
+
+__device__ __forceinline__ uint32_t rfl32(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Element types: fp32 pairs to a dword of two values (round to nearest even; EXACT: the values
+// are whole numbers of at most 8 bits, which both types hold), and the MFMA products of 16-byte
+// operands held as dwords.
+struct Bf16 {
+  static constexpr int DT = DT_BF16;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    return bitcast<uint32_t>(v2{(__bf16)a, (__bf16)b});
+  }
+  static __device__ __forceinline__ uint32_t pack_exact(float a, float b) {
+    return perm(bitcast<uint32_t>(b), bitcast<uint32_t>(a), 0x07060302u);
+  }
+  static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float get(uint16_t h) { return bf16_to_f32(h); }
+};
+
+struct F16 {
+  static constexpr int DT = DT_F16;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return bitcast<uint32_t>(f16x2{(_Float16)a, (_Float16)b});
+  }
+  static __device__ __forceinline__ uint32_t pack_exact(float a, float b) {
+    return bitcast<uint32_t>(__builtin_amdgcn_cvt_pkrtz(a, b));
+  }
+  static __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float get(uint16_t h) { return (float)bitcast<_Float16>(h); }
+};
+
+// Keys of sequence b, clamped to what its row of the page table can hold.
+__device__ __forceinline__ int kv_length(const KvSrc& kv, int b) {
+  const long long most = (long long)kv.max_pages << kv.page_shift;
+  const int n = kv.len[b];
+  return n < 0 ? 0 : (long long)n > most ? (int)most : n;
+}
+
+// 2^x, and the factor between two running maxima (in powers of two) of which the first may be
+// -inf: nothing was seen yet, or scores of -inf alone.
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace qlin

@@ -1,0 +1,115 @@
+// Host/device shared definitions of the attention layer's middle (not part of the
+// public ABI): per-head norm with rotary positions into a paged cache, prompt and
+// decode attention.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace qlin {
+
+// One tensor of a paged cache: 16-bit or int8 values [pages][page][heads][hd] with any
+// strides (elements; the last axis is contiguous), and the fp32 scales of an int8 one
+// [pages][page][heads].
+struct PagedTensor {
+  void* p;
+  long long sp, st, sh;   // page, token and head strides
+  float* s;               // nullptr: 16-bit values
+  long long ssp, sst, ssh;
+};
+
+// Per-head norm, rotary positions, cache write (rope.hip).
+struct RopeArgs {
+  const void* q;
+  long long qt, qh;       // token and head strides (elements)
+  const void* k;
+  long long kt, kh;
+  const void* v;          // nullptr: no values
+  long long vt, vh;
+  void* qo;
+  long long qot, qoh;
+  void* ko;               // nullptr: rotated keys go to the cache only
+  long long kot, koh;
+  PagedTensor kc, vc;     // p == nullptr: no cache
+  long long nslots;       // pages * page
+  int page_shift;
+  const void* slots;      // [T]
+  int slots64;
+  const void* pos;        // [axes][T]
+  long long pos_a, pos_t;
+  int pos64;
+  const void* freqs;      // [rot / 2]
+  int freqs64;
+  const void* qw;         // norm weights [hd] or nullptr (no norm)
+  const void* kw;
+  int wdt;
+  int one_plus;
+  float eps;
+  int T, HQ, HKV, hd, rot;
+  int axes, sec[3], interleaved;
+  int dt;                 // DT_BF16 or DT_F16
+};
+hipError_t launch_rope(const RopeArgs& a, hipStream_t st);
+
+// Where attention finds keys and values: packed rows [rows][heads][hd] (table ==
+// nullptr; sequence b holds rows cu[b] .. cu[b + 1] - 1) or the pages table[b][...] of a
+// cache (sequence b holds len[b] keys).
+struct KvSrc {
+  PagedTensor k, v;
+  const int* table;
+  long long table_stride;
+  int num_pages, max_pages, page_shift;
+  const int* len;
+  const int* cu;
+  int rows;               // packed: rows of k and v
+};
+
+// Attention of one token per sequence (attn_decode.hip).
+struct DecodeArgs {
+  const void* q;
+  long long qb, qh;
+  void* o;
+  long long ob, oh;
+  KvSrc kv;
+  int B, HQ, HKV, G;      // G = HQ / HKV
+  int gb;                 // groups of 16 query heads of a key head
+  float c;                // scale * log2(e)
+  int target;             // work units a launch aims at
+  int units;              // units per (key head, group): the grid's bound
+  float* part;            // unit partials
+  unsigned* cnt;          // arrival counters, zero between calls
+};
+// A part: rows x hd sums of 32 bits, then (maximum, sum of P, 0, 0) of each row.
+__host__ __device__ constexpr int decode_slot_floats(int rows, int hd) { return rows * hd + rows * 4; }
+constexpr int kDecodeBlock = 32;     // keys a wave takes at a time
+constexpr int kDecodeChunk = 4;      // blocks of a unit come in multiples of this (one per wave)
+constexpr int kDecodeGroup = 16;     // units joined at a time
+constexpr int kDecodeCounters = 32;  // counters of a (sequence, key head, group)
+hipError_t launch_decode(const DecodeArgs& a, int dt, int hd, hipStream_t st);
+
+// Attention of packed prompts over packed keys or a paged cache (attn_prompt*.hip).
+struct PromptArgs {
+  const void* q;
+  long long qt, qh;       // token and head strides (elements)
+  void* o;
+  long long ot, oh;
+  KvSrc kv;               // table == nullptr: packed keys, sequence b's at kv.cu
+  const int* cu;          // [B + 1] rows of q of each sequence
+  int T, B, HQ, HKV, G;
+  int causal;
+  float c;                // scale * log2(e)
+  int target;             // work units to cut the keys into; 0: no cut
+  int units;              // units per key head: the grid's bound
+  int tiles;              // row tiles per key head: the join's bound
+  float* part;            // unit partials [key head][unit]
+};
+constexpr int kPromptBlock = 32;     // keys of a step
+constexpr int kPromptMinBlocks = 4;  // shortest cut
+// row sets of 32 per wave (tiles of 128 or 256 rows of tokens x the query heads of a key head)
+constexpr int prompt_rows(int rs) { return 128 * rs; }
+constexpr long long prompt_slot_floats(int rs, int hd) { return (long long)prompt_rows(rs) * (hd + 2); }
+hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, int rs, hipStream_t st);
+hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, int rs, hipStream_t st);
+hipError_t launch_prompt_f16(const PromptArgs& a, int hd, int rs, hipStream_t st);
+
+}  // namespace qlin
