@@ -142,23 +142,17 @@ int workspace_parts(const char* fn, void* ws, size_t bytes, char** part, size_t*
 }
 
 // Row tiles and key cuts of a prompt call.
-int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void* ws, size_t ws_bytes, int& rs) {
+int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void* ws, size_t ws_bytes) {
   char* part;
   size_t avail;
   QA_TRY(workspace_parts(fn, ws, ws_bytes, &part, &avail));
-  const long long rows = (long long)a.T * a.G;
-  rs = rows > 128 ? 2 : 1;
-  long long target = 512;
-  if (const char* e = getenv("QLIN_PROMPT")) {  // "row sets,units" for tuning runs
-    int r = 0, t = -1;
-    if (sscanf(e, "%d,%d", &r, &t) == 2) {
-      if (r == 1 || r == 2) rs = r;
-      if (t >= 0) target = t;
-    }
+  long long target = 1024;
+  if (const char* e = getenv("QLIN_PROMPT_UNITS")) {  // for tuning runs
+    if (atoi(e) >= 0) target = atoi(e);
   }
-  const long long tiles = rows / prompt_rows(rs) + a.B;
-  const long long slot = prompt_slot_floats(rs, hd) * 4;
-  if (tiles * a.HKV >= 1024 || max_keys <= kPromptMinBlocks * kPromptBlock) target = 0;
+  const long long tiles = (long long)a.T * a.G / kPromptRows + a.B;
+  const long long slot = prompt_slot_floats(hd) * 4;
+  if (tiles * a.HKV >= 2048 || max_keys <= kPromptMinBlocks * kPromptBlock) target = 0;
   // every unit of a key head has a slot: at most 2 target / HKV + tiles of them
   target = std::min(target, ((long long)avail / slot / a.HKV - tiles - 1) * a.HKV / 2);
   if (target <= a.HKV) target = 0;
@@ -262,9 +256,8 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void*
   a.kv.cu = cu_k, a.kv.rows = Tk;
   a.cu = cu_q, a.T = T, a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
-  int rs;
-  QA_TRY(plan_prompt(fn, a, hd, Tk, workspace, workspace_bytes, rs));
-  return status(fn, launch_prompt(a, dtype, hd, rs, (hipStream_t)stream));
+  QA_TRY(plan_prompt(fn, a, hd, Tk, workspace, workspace_bytes));
+  return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
 }
 
 int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const qlin_paged_kv* cache,
@@ -290,9 +283,8 @@ int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const
   a.o = out, a.ot = o_token, a.oh = o_head;
   a.cu = cu_q, a.T = T, a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
-  int rs;
-  QA_TRY(plan_prompt(fn, a, hd, (long long)max_pages * cache->page, workspace, workspace_bytes, rs));
-  return status(fn, launch_prompt(a, dtype, hd, rs, (hipStream_t)stream));
+  QA_TRY(plan_prompt(fn, a, hd, (long long)max_pages * cache->page, workspace, workspace_bytes));
+  return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
 }
 
 int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_paged_kv* cache, const int* table,

@@ -105,11 +105,11 @@ struct PromptArgs {
 };
 constexpr int kPromptBlock = 32;     // keys of a step
 constexpr int kPromptMinBlocks = 4;  // shortest cut
-// row sets of 32 per wave (tiles of 128 or 256 rows of tokens x the query heads of a key head)
-constexpr int prompt_rows(int rs) { return 128 * rs; }
-constexpr long long prompt_slot_floats(int rs, int hd) { return (long long)prompt_rows(rs) * (hd + 2); }
-hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, int rs, hipStream_t st);
-hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, int rs, hipStream_t st);
-hipError_t launch_prompt_f16(const PromptArgs& a, int hd, int rs, hipStream_t st);
+constexpr int kPromptRows = 128;     // rows of a tile: tokens x the query heads of a key head
+// a unit's partial: sums of its rows, then (maximum, sum of P) of each
+__host__ __device__ constexpr long long prompt_slot_floats(int hd) { return (long long)kPromptRows * (hd + 2); }
+hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, hipStream_t st);
+hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, hipStream_t st);
+hipError_t launch_prompt_f16(const PromptArgs& a, int hd, hipStream_t st);
 
 }  // namespace qlin

@@ -3,12 +3,12 @@
 
 namespace qlin {
 
-hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, int rs, hipStream_t st) {
-  return prompt_dispatch<Bf16>(a, hd, rs, st);
+hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, hipStream_t st) {
+  return prompt_dispatch<Bf16>(a, hd, st);
 }
 
-hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, int rs, hipStream_t st) {
-  return dt == DT_BF16 ? launch_prompt_bf16(a, hd, rs, st) : launch_prompt_f16(a, hd, rs, st);
+hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, hipStream_t st) {
+  return dt == DT_BF16 ? launch_prompt_bf16(a, hd, st) : launch_prompt_f16(a, hd, st);
 }
 
 }  // namespace qlin

@@ -3,8 +3,8 @@
 
 namespace qlin {
 
-hipError_t launch_prompt_f16(const PromptArgs& a, int hd, int rs, hipStream_t st) {
-  return prompt_dispatch<F16>(a, hd, rs, st);
+hipError_t launch_prompt_f16(const PromptArgs& a, int hd, hipStream_t st) {
+  return prompt_dispatch<F16>(a, hd, st);
 }
 
 }  // namespace qlin

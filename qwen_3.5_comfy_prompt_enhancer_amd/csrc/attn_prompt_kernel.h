@@ -49,6 +49,14 @@ __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 
+// 4-byte LDS DMA: lane i copies 4 bytes from its own address to LDS m0 + 4 i.
+__device__ __forceinline__ void dma4(const void* p, uint32_t m0) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(p), "{m0}"(m0) : "memory");
+}
+
+// LDS operands that are read ahead of their products.
+constexpr int kAhead = 3;
+
 template <typename P>
 __device__ __forceinline__ P* rfl_p(P* p) {
   const uint64_t v = (uint64_t)p;
@@ -96,8 +104,9 @@ struct Tile {
 
 // Work unit u (UNITS) or row tile u of a key head.  Tiles of a sequence are numbered from the
 // last, which sees most keys, so that long units start first.
-template <int ROWS, bool UNITS>
+template <bool UNITS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
+  constexpr int ROWS = kPromptRows;
   const int lane = (int)threadIdx.x & 63;
   int chunk = 1 << 30;
   if (a.target > 0) {
@@ -190,27 +199,44 @@ struct PGeo {
   static constexpr int NI = 8 / RPI;       // copies of a wave's 8 rows
   static constexpr int HALF = KB * ROWB;   // bytes of a K or V tile
   static constexpr int STAGE = 2 * HALF;
+  static constexpr int SCALES = 4 * 64;    // bytes of a block's scales: a wave's 8 of K and 8 of V
   static __device__ __forceinline__ int swk(int r) { return HD >= 128 ? r & 15 : (r >> 1) & 7; }
   static __device__ __forceinline__ int swv(int r) { return HD >= 128 ? r & 3 : (r >> 1) & 1; }
 };
 
-template <bool Q8>
-constexpr int prompt_stages() { return Q8 ? 2 : 4; }
+// LDS of a workgroup.  16-bit keys: a ring of two stages.  int8: one 16-bit tile, made from a
+// ring of two tiles of codes and their scales.
+template <int HD, bool Q8>
+constexpr int prompt_lds() {
+  return Q8 ? PGeo<HD>::STAGE + 2 * (PGeo<HD>::STAGE / 2 + PGeo<HD>::SCALES) : 2 * PGeo<HD>::STAGE;
+}
 
-// RS: row sets of 32 a wave holds.  Q8: int8 cache.
-template <typename T, int HD, int RS, bool Q8, bool PAGED>
-__global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptArgs a) {
+template <typename V>
+__device__ __forceinline__ V lds_ld(uint32_t at) {
+  return *(const __attribute__((address_space(3))) V*)at;
+}
+template <typename V>
+__device__ __forceinline__ void lds_st(uint32_t at, V v) {
+  *(__attribute__((address_space(3))) V*)at = v;
+}
+
+// Q8: int8 cache.
+template <typename T, int HD, bool Q8, bool PAGED>
+__global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void prompt_kernel(const PromptArgs a) {
   using G = PGeo<HD>;
-  constexpr int ROWS = prompt_rows(RS);
-  constexpr int NST = prompt_stages<Q8>();
+  using TV = std::conditional_t<Q8, Bf16, T>;  // type of P and V in their product
+  // fp16 queries over int8 values: P x scale as two bf16 numbers, so that neither range nor
+  // precision is lost
+  constexpr int PN = Q8 && T::DT == DT_F16 ? 2 : 1;
+  constexpr int ROWS = kPromptRows;
   constexpr int ES = Q8 ? 1 : 2;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
 
   int hk, unit;
   split_grid(a.HKV, a.units, hk, unit);
   Tile t;
-  if (hk >= a.HKV || unit >= a.units || !find_tile<ROWS, true>(a, unit, t)) return;
+  if (hk >= a.HKV || unit >= a.units || !find_tile<true>(a, unit, t)) return;
   t.uniform();
   const int tid = (int)threadIdx.x;
   const int wave = (int)rfl32((uint32_t)tid >> 6), lane = tid & 63;
@@ -218,37 +244,27 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
   const int per = (t.nblk + t.parts - 1) / t.parts;
   const int kb0 = t.part * per, kb1 = min(t.nblk, kb0 + per);
 
-  // rows: this lane's column of set rs is row R0 + 32 rs + col
-  const int R0 = t.tile * ROWS + wave * 32 * RS;
-  int tok[RS], head[RS], lim[RS];
-  u32x4 Q[RS][G::NS];
+  // this lane's row is R0 + col
+  const int R0 = t.tile * ROWS + wave * 32;
+  u32x4 Q[G::NS];
+  int lim;
+  {
+    const int i = (R0 + col) / a.G, ic = min(i, t.s.nq - 1);
+    lim = seen(a, t.s, ic);
+    const uint16_t* q = (const uint16_t*)a.q + (t.s.q0 + ic) * a.qt + (hk * a.G + (R0 + col - i * a.G)) * a.qh + 8 * h;
 #pragma unroll
-  for (int rs = 0; rs < RS; ++rs) {
-    const int R = R0 + 32 * rs + col;
-    const int i = R / a.G;
-    head[rs] = hk * a.G + (R - i * a.G);
-    tok[rs] = i < t.s.nq ? i : -1;
-    const int ic = min(i, t.s.nq - 1);
-    lim[rs] = seen(a, t.s, ic);
-    const uint16_t* q = (const uint16_t*)a.q + (t.s.q0 + ic) * a.qt + head[rs] * a.qh + 8 * h;
-#pragma unroll
-    for (int s = 0; s < G::NS; ++s) Q[rs][s] = ld_global<u32x4>(q + 16 * s);
+    for (int s = 0; s < G::NS; ++s) Q[s] = ld_global<u32x4>(q + 16 * s);
   }
   // what every row of the wave sees, and what some row sees
   const int wmin = seen(a, t.s, min(R0 / a.G, t.s.nq - 1));
-  const int wmax = R0 / a.G >= t.s.nq ? 0 : seen(a, t.s, min((R0 + 32 * RS - 1) / a.G, t.s.nq - 1));
+  const int wmax = R0 / a.G >= t.s.nq ? 0 : seen(a, t.s, min((R0 + 31) / a.G, t.s.nq - 1));
 
-  f32x16 O[RS][G::ND];
-  float m[RS], l[RS];
+  f32x16 O[G::ND];
+  float m = kNegInf, l = 0.0f;
 #pragma unroll
-  for (int rs = 0; rs < RS; ++rs) {
-    m[rs] = kNegInf;
-    l[rs] = 0.0f;
+  for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) O[rs][d][i] = 0.0f;
-  }
+    for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
 
   bool bad = false;
   const int* table = PAGED ? a.kv.table + t.b * a.kv.table_stride : nullptr;
@@ -264,6 +280,9 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
                                : (long long)(t.s.k0 + key8) * x.st;
     return (const uint8_t*)x.p + (at + hk * x.sh) * ES;
   };
+  auto scale_of = [&](const PagedTensor& x, int key8, int pid) {
+    return x.s + pid * x.ssp + (key8 & ((1 << a.kv.page_shift) - 1)) * x.sst + hk * x.ssh;
+  };
   auto checked = [&](int pid) {
     if (PAGED && (unsigned)pid >= (unsigned)a.kv.num_pages) {
       bad = true;
@@ -272,241 +291,305 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
     return pid;
   };
 
-  // 16-bit: this lane's copies
-  const int r_in = lane / G::LPR, p16 = lane % G::LPR;
-  auto issue = [&](int slot, int kb, int pid) __attribute__((always_inline)) {
+  // Copies of this wave's 8 keys of block kb.  16-bit: to their swizzled places in a stage.
+  auto issue = [&](uint32_t stage, int kb, int pid) __attribute__((always_inline)) {
+    // (from a value that the compiler takes for a new one each time: kept through the loop, the
+    // copies' offsets would push operands out of the registers)
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int r_in = lane / G::LPR, p16 = lane % G::LPR;
     const int key8 = key8_of(kb);
     pid = checked(pid);
     const int rmax = nk - 1 - key8;
     const uint8_t* kp = rfl_p(base_of(a.kv.k, key8, pid));
     const uint8_t* vp = rfl_p(base_of(a.kv.v, key8, pid));
-    const uint32_t at = lds0 + (uint32_t)(slot * G::STAGE + 8 * wave * G::ROWB);
+    if constexpr (!Q8) {
+      const uint32_t at = stage + (uint32_t)(8 * wave * G::ROWB);
 #pragma unroll
-    for (int i = 0; i < G::NI; ++i) {
-      const int r = G::RPI * i + r_in, row = 8 * wave + r;
-      const int ck = p16 ^ G::swk(row);
-      const int cv = (((p16 >> 2) ^ G::swv(row)) << 2) | (p16 & 3);
-      const uint32_t rc = (uint32_t)min(r, rmax);
-      dma16(kp, rc * (uint32_t)(a.kv.k.st * 2) + (uint32_t)ck * 16u, at + (uint32_t)(G::RPI * i * G::ROWB));
-      dma16(vp, rc * (uint32_t)(a.kv.v.st * 2) + (uint32_t)cv * 16u,
-            at + (uint32_t)(G::HALF + G::RPI * i * G::ROWB));
+      for (int i = 0; i < G::NI; ++i) {
+        const int r = G::RPI * i + r_in, row = 8 * wave + r;
+        const int ck = p16 ^ G::swk(row);
+        const int cv = (((p16 >> 2) ^ G::swv(row)) << 2) | (p16 & 3);
+        const uint32_t rc = (uint32_t)min(r, rmax);
+        dma16(kp, rc * (uint32_t)(a.kv.k.st * 2) + (uint32_t)ck * 16u, at + (uint32_t)(G::RPI * i * G::ROWB));
+        dma16(vp, rc * (uint32_t)(a.kv.v.st * 2) + (uint32_t)cv * 16u,
+              at + (uint32_t)(G::HALF + G::RPI * i * G::ROWB));
+      }
+    } else {
+      // codes of row r at 8 wave HD + r HD (keys, then values), scales of keys and values behind
+      constexpr int L8 = HD / 16, R8 = 64 / L8;  // lanes of a row, rows of a copy
+      const uint32_t at = stage + (uint32_t)(8 * wave * HD);
+      if (R8 <= 8 || lane < 8 * L8) {
+#pragma unroll
+        for (int i = 0; i < (R8 < 8 ? 8 / R8 : 1); ++i) {
+          const uint32_t rc = (uint32_t)min(R8 * i + lane / L8, rmax);
+          const uint32_t c = (uint32_t)(lane % L8) * 16u;
+          dma16(kp, rc * (uint32_t)a.kv.k.st + c, at + (uint32_t)(R8 * i * HD));
+          dma16(vp, rc * (uint32_t)a.kv.v.st + c, at + (uint32_t)(G::KB * HD + R8 * i * HD));
+        }
+      }
+      const float* ks = scale_of(a.kv.k, key8, pid);
+      const float* vs = scale_of(a.kv.v, key8, pid);
+      if (lane < 16) {
+        const int r = min(lane & 7, rmax);
+        const float* p = lane < 8 ? ks + r * a.kv.k.sst : vs + r * a.kv.v.sst;
+        dma4(p, stage + (uint32_t)(G::STAGE / 2 + 64 * wave));
+      }
     }
   };
-  // int8: 16 codes a lane; rows of HD bytes take HD/16 lanes
-  constexpr int L8 = HD / 16, R8 = 64 / L8, N8 = R8 >= 8 ? 1 : 8 / R8;
-  u32x4 ck8[N8], cv8[N8];
-  float sk8[N8], sv8[N8];
-  auto load8 = [&](int kb, int pid) __attribute__((always_inline)) {
-    const int key8 = key8_of(kb);
-    pid = checked(pid);
-    const int rmax = nk - 1 - key8;
-    const uint8_t* kp = base_of(a.kv.k, key8, pid);
-    const uint8_t* vp = base_of(a.kv.v, key8, pid);
-    const long long off = key8 & ((1 << a.kv.page_shift) - 1);
-    const float* ks = a.kv.k.s + pid * a.kv.k.ssp + off * a.kv.k.sst + hk * a.kv.k.ssh;
-    const float* vs = a.kv.v.s + pid * a.kv.v.ssp + off * a.kv.v.sst + hk * a.kv.v.ssh;
+  // int8: this wave's codes of a block as 16-bit whole numbers, to their places in the tile
+  auto widen = [&](uint32_t codes) __attribute__((always_inline)) {
+    constexpr int CH = HD / 16;  // 16-byte chunks of a row of codes
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
 #pragma unroll
-    for (int i = 0; i < N8; ++i) {
-      const int r = min(min(R8 * i + lane / L8, 7), rmax);
-      ck8[i] = ld_global<u32x4>(kp + r * a.kv.k.st + (lane % L8) * 16);
-      cv8[i] = ld_global<u32x4>(vp + r * a.kv.v.st + (lane % L8) * 16);
-      sk8[i] = ks[r * a.kv.k.sst];
-      sv8[i] = vs[r * a.kv.v.sst];
-    }
-  };
-  auto put8 = [&](int slot) __attribute__((always_inline)) {
+    for (int i = 0; i < 8 * CH / 64 || i == 0; ++i) {
+      const int x = i * 64 + lane, r = x / CH, c16 = x % CH, row = 8 * wave + r;
+      if (8 * CH < 64 && x >= 8 * CH) break;
+      const uint32_t from = codes + (uint32_t)(row * HD + c16 * 16);
+      const u32x4 kc = lds_ld<u32x4>(from), vc = lds_ld<u32x4>(from + G::KB * HD);
 #pragma unroll
-    for (int i = 0; i < N8; ++i) {
-      const int r = R8 * i + lane / L8;
-      if (R8 > 8 && r >= 8) break;
-      const int row = 8 * wave + r;
-      auto wide = [&](u32x4 c, float s, int half) {
-        u32x4 o;
+      for (int y = 0; y < 2; ++y) {
+        u32x4 ko, vo;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t w = c[2 * half + e / 2];
+          const uint32_t wk = kc[2 * y + e / 2], wv = vc[2 * y + e / 2];
           const int b = 16 * (e % 2);
-          o[e] = T::pack((float)(int8_t)(w >> b) * s, (float)(int8_t)(w >> (b + 8)) * s);
+          ko[e] = T::pack_exact((float)(int8_t)(wk >> b), (float)(int8_t)(wk >> (b + 8)));
+          vo[e] = TV::pack_exact((float)(int8_t)(wv >> b), (float)(int8_t)(wv >> (b + 8)));
         }
-        return o;
-      };
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int c = 2 * (lane % L8) + x;
-        uint8_t* at = lds + slot * G::STAGE + row * G::ROWB;
-        *(u32x4*)(at + ((c ^ G::swk(row)) << 4)) = wide(ck8[i], sk8[i], x);
-        *(u32x4*)(at + G::HALF + (((((c >> 2) ^ G::swv(row)) << 2) | (c & 3)) << 4)) = wide(cv8[i], sv8[i], x);
+        const int c = 2 * c16 + y;
+        const uint32_t to = lds0 + (uint32_t)(row * G::ROWB);
+        lds_st(to + (uint32_t)((c ^ G::swk(row)) << 4), ko);
+        lds_st(to + (uint32_t)(G::HALF + (((((c >> 2) ^ G::swv(row)) << 2) | (c & 3)) << 4)), vo);
       }
     }
   };
 
-  // this lane's places in a stage: K operand s at row col, V operand (d, k) by two transposing
-  // reads of 4 keys each
-  auto step = [&](int slot, int kb) __attribute__((always_inline)) {
+  // LDS places of this lane's operands: step s of K at ka ^ 32 s (the swizzle reaches 256 bytes),
+  // 32-wide block d of V at va ^ 64 (d % 4), two transposing reads of 4 keys each
+  const int s16 = lane & 15;
+  const uint32_t ka = lds0 + (uint32_t)(col * G::ROWB + ((h ^ G::swk(col)) << 4));
+  const uint32_t va = lds0 + (uint32_t)(G::HALF + (4 * h + (s16 >> 2)) * G::ROWB + (G::swv(s16 >> 2) << 6) +
+                                        ((lane >> 4) & 1) * 32 + (s16 & 3) * 8);
+
+  auto step = [&](auto stage_c, int kb, uint32_t scales) __attribute__((always_inline)) {
+    constexpr uint32_t stage = decltype(stage_c)::value;
     if (kb * G::KB >= wmax) return;
-    const bool masked = kb * G::KB + G::KB > wmin;
-    const uint8_t* st = lds + slot * G::STAGE;
-    f32x16 S[RS];
+    // operands are read kAhead products ahead (the order is fixed: left to itself the compiler
+    // reads each just before its product, and the wave waits for LDS every time)
+    auto k_at = [&](int s) {
+      return lds_ld<u32x4>((ka ^ (uint32_t)((s & 7) << 5)) + stage + (s >= 8 ? 256u : 0u));
+    };
+    f32x16 S = {};
+    {
+      u32x4 k[kAhead];
 #pragma unroll
-    for (int rs = 0; rs < RS; ++rs)
+      for (int s = 0; s < kAhead; ++s) k[s] = k_at(s);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) S[rs][i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < G::NS; ++s) {
-      const u32x4 k = *(const u32x4*)(st + col * G::ROWB + (((2 * s + h) ^ G::swk(col)) << 4));
-#pragma unroll
-      for (int rs = 0; rs < RS; ++rs) S[rs] = T::mma32(k, Q[rs][s], S[rs]);
-    }
-    u32x4 P[RS][2];
-#pragma unroll
-    for (int rs = 0; rs < RS; ++rs) {
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (kb * G::KB + 8 * (i / 4) + 4 * h + i % 4 >= lim[rs]) S[rs][i] = kNegInf;
-      }
-      float mx = S[rs][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, S[rs][i]);
-      float x, y;
-      lane_pair<32>(mx, x, y);
-      mx = fmaxf(x, y) * a.c;
-      if (__any(mx > m[rs] + 8.0f)) {
-        const float mn = fmaxf(m[rs], mx);
-        const float al = exp2_(m[rs] - (mn == kNegInf ? 0.0f : mn));
-        m[rs] = mn;
-        l[rs] *= al;
-#pragma unroll
-        for (int d = 0; d < G::ND; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) O[rs][d][i] *= al;
-      }
-      const float ms = m[rs] == kNegInf ? 0.0f : m[rs];
-      float p[16], sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = exp2_(fmaf(S[rs][i], a.c, -ms));
-        sum += p[i];
-      }
-      l[rs] += sum;
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) P[rs][k][e] = T::pack(p[8 * k + 2 * e], p[8 * k + 2 * e + 1]);
-    }
-    const int s16 = lane & 15, dsub = (lane >> 4) & 1;
-#pragma unroll
-    for (int d = 0; d < G::ND; ++d)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x2 v[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int row = 16 * k + 8 * x + 4 * h + (s16 >> 2);
-          typedef short s16x4 __attribute__((ext_vector_type(4)));
-          auto p = (__attribute__((address_space(3))) s16x4*)(st + G::HALF + row * G::ROWB +
-                                                               ((d ^ G::swv(row)) << 6) + dsub * 32 + (s16 & 3) * 8);
-          v[x] = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
-        }
-        const u32x4 vop = {v[0].x, v[0].y, v[1].x, v[1].y};
-#pragma unroll
-        for (int rs = 0; rs < RS; ++rs) O[rs][d] = T::mma32(vop, P[rs][k], O[rs][d]);
-      }
-  };
-
-  if (kb0 < kb1) {
-    if constexpr (!Q8) {
-      int pid = page_of(kb0);
-#pragma unroll
-      for (int i = 0; i < NST - 1; ++i) {
-        issue(i, kb0 + i, pid);
-        pid = page_of(kb0 + i + 1);
-      }
-      int slot = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int s = 0; s < G::NS; ++s) {
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(wait_vm((NST - 2) * 2 * G::NI));
-        asm volatile("s_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        // the stage that all have read gets the block NST - 1 ahead
-        issue(slot == 0 ? NST - 1 : slot - 1, kb + NST - 1, pid);
-        pid = page_of(kb + NST);
-        step(slot, kb);
-        slot = slot == NST - 1 ? 0 : slot + 1;
+        S = T::mma32(k[s % kAhead], Q[s], S);
+        if (s + kAhead < G::NS) k[s % kAhead] = k_at(s + kAhead);
       }
       __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
-      __builtin_amdgcn_sched_barrier(0);
-    } else {
-      load8(kb0, page_of(kb0));
-      put8(0);
-      load8(kb0 + 1, page_of(kb0 + 1));
-      int slot = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        __syncthreads();
-        put8(slot ^ 1);
-        load8(kb + 2, page_of(kb + 2));
-        step(slot, kb);
-        slot ^= 1;
+    }
+    if constexpr (Q8) {
+      // scales of keys 8 i + 4 h ..: this lane's four runs of scores
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 ks = lds_ld<f32x4>(scales + (uint32_t)(64 * i + 16 * h));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[4 * i + e] *= ks[e];
       }
     }
-  }
-
-  bool again = false;
+    if (kb * G::KB + G::KB > wmin) {
+      const int rel = lim - kb * G::KB - 4 * h;
 #pragma unroll
-  for (int rs = 0; rs < RS; ++rs) {
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 >= rel) S[i] = kNegInf;
+    }
+    float mx = fmaxf(fmaxf(S[0], S[1]), S[2]);
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, S[i]), S[i + 1]);
+    mx = fmaxf(mx, S[15]);
     float x, y;
-    lane_pair<32>(l[rs], x, y);
-    l[rs] = x + y;
-    if (kb1 * G::KB > wmin) {  // masked blocks were among the unit's
-      float z = 0.0f;
+    lane_pair<32>(mx, x, y);
+    mx = fmaxf(x, y) * a.c;
+    if (__any(mx > m + 8.0f)) {
+      const float mn = fmaxf(m, mx);
+      const float al = exp2_(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
 #pragma unroll
       for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) z = fmaf(O[rs][d][i], 0.0f, z);
-      again |= !(z == 0.0f) && tok[rs] >= 0;
+        for (int i = 0; i < 16; ++i) O[d][i] *= al;
     }
+    const float ms = m == kNegInf ? 0.0f : m;
+    u32x4 P[PN][2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = exp2_(fmaf(S[8 * k + e], a.c, -ms));
+        sum += p[e];
+      }
+      f32x4 vs[2];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vs[i] = lds_ld<f32x4>(scales + (uint32_t)(64 * (2 * k + i) + 32 + 16 * h));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float p0 = p[2 * e], p1 = p[2 * e + 1];
+        if constexpr (Q8) {
+          p0 *= vs[e / 2][2 * (e % 2)];
+          p1 *= vs[e / 2][2 * (e % 2) + 1];
+        }
+        P[0][k][e] = TV::pack(p0, p1);
+        if constexpr (PN == 2) {
+          const uint32_t w = P[0][k][e];
+          P[1][k][e] = TV::pack(p0 - bitcast<float>(w << 16), p1 - bitcast<float>(w & 0xFFFF0000u));
+        }
+      }
+    }
+    l += sum;
+    auto v_at = [&](int x) {  // operand of block x / 2, keys 16 (x % 2) ..
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      u32x2 v[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const int d = x / 2, k = x % 2;
+        const uint32_t at = (va ^ (uint32_t)((d & 3) << 6)) + stage +
+                            (uint32_t)((d >> 2) * 256 + (16 * k + 8 * z) * G::ROWB);
+        v[z] = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+      }
+      return u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
+    };
+    u32x4 v[kAhead];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) v[x] = v_at(x);
+#pragma unroll
+    for (int x = 0; x < 2 * G::ND; ++x) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < PN; ++n) O[x / 2] = TV::mma32(v[x % kAhead], P[n][x % 2], O[x / 2]);
+      if (x + kAhead < 2 * G::ND) v[x % kAhead] = v_at(x + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // this wave's copies have landed and its LDS reads returned, and so for all waves
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  if (kb0 < kb1) {
+    int pid = page_of(kb0);
+    if constexpr (!Q8) {
+      constexpr std::integral_constant<uint32_t, 0> s0;
+      constexpr std::integral_constant<uint32_t, G::STAGE> s1;
+      issue(lds0, kb0, pid);
+      pid = page_of(kb0 + 1);
+      for (int kb = kb0;;) {
+        meet();
+        issue(lds0 + G::STAGE, kb + 1, pid);
+        pid = page_of(kb + 2);
+        step(s0, kb, 0);
+        if (++kb >= kb1) break;
+        meet();
+        issue(lds0, kb + 1, pid);
+        pid = page_of(kb + 2);
+        step(s1, kb, 0);
+        if (++kb >= kb1) break;
+      }
+    } else {
+      // codes of block kb + 1 land while block kb is widened and used
+      const uint32_t c0 = lds0 + G::STAGE;
+      constexpr uint32_t CODES = G::STAGE / 2 + G::SCALES;
+      uint32_t codes = c0;
+      issue(codes, kb0, pid);
+      pid = page_of(kb0 + 1);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        meet();  // the tile has been read, this block's codes and scales are there
+        const uint32_t next = codes == c0 ? c0 + CODES : c0;
+        issue(next, kb + 1, pid);
+        pid = page_of(kb + 2);
+        widen(codes);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile is written
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        step(std::integral_constant<uint32_t, 0>{}, kb, codes + G::STAGE / 2);
+        codes = next;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
+    __builtin_amdgcn_sched_barrier(0);
   }
-  float* slot_p = a.part + ((long long)hk * a.units + t.slot + t.part) * prompt_slot_floats(RS, HD);
+
+  // (the row again, from a thread index that the compiler takes for another, so that nothing of
+  // it is kept in registers through the loop)
+  int tid2 = (int)threadIdx.x;
+  asm volatile("" : "+v"(tid2));
+  const int row = R0 + (tid2 & 31), tok = row / a.G;
+  const int head = hk * a.G + (row - tok * a.G);
+  const int h2 = (tid2 >> 5) & 1;
+
+  float x, y;
+  lane_pair<32>(l, x, y);
+  l = x + y;
+  bool again = false;
+  if (kb1 * G::KB > wmin) {  // masked blocks were among the unit's
+    float z = 0.0f;
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z = fmaf(O[d][i], 0.0f, z);
+    again = !(z == 0.0f) && tok < t.s.nq;
+  }
+  float* slot_p = a.part + ((long long)hk * a.units + t.slot + t.part) * prompt_slot_floats(HD);
   float* ml = slot_p + ROWS * HD;
   const bool any_bad = __any(bad);
 
   if (!__any(again)) {
+    if (any_bad) l = __builtin_nanf("");
+    if (t.parts > 1) {
+      float* dst = slot_p + wave * 32 * HD + (tid2 & 63) * 4;
 #pragma unroll
-    for (int rs = 0; rs < RS; ++rs) {
-      if (any_bad) l[rs] = __builtin_nanf("");
-      if (t.parts > 1) {
-        float* dst = slot_p + (wave * RS + rs) * 32 * HD + lane * 4;
+      for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-        for (int d = 0; d < G::ND; ++d)
+        for (int i = 0; i < 4; ++i)
+          *(f32x4*)(dst + (d * 4 + i) * 256) = f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
+      if (h2 == 0) *(float2*)(ml + (wave * 32 + (tid2 & 31)) * 2) = float2{m, l};
+    } else {
+      // a row that sees no key is zero
+      const float f = seen(a, t.s, min(tok, t.s.nq - 1)) > 0 ? 1.0f / l : 0.0f;
+      uint16_t* o = (uint16_t*)a.o + (long long)(t.s.q0 + tok) * a.ot + head * a.oh;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *(f32x4*)(dst + (d * 4 + i) * 256) =
-                f32x4{O[rs][d][4 * i], O[rs][d][4 * i + 1], O[rs][d][4 * i + 2], O[rs][d][4 * i + 3]};
-        if (h == 0) *(float2*)(ml + ((wave * RS + rs) * 32 + col) * 2) = float2{m[rs], l[rs]};
-      } else {
-        const float inv = 1.0f / l[rs];
-        // a row that sees no key is zero
-        const float f = lim[rs] > 0 ? inv : 0.0f;
-        uint16_t* o = (uint16_t*)a.o + (long long)(t.s.q0 + tok[rs]) * a.ot + head[rs] * a.oh;
+      for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-        for (int d = 0; d < G::ND; ++d)
+        for (int i = 0; i < 2; ++i) {
+          // halves hold 4 values each of two runs of 8: exchanged, each stores one run
+          uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            // halves hold 4 values each of two runs of 8: exchanged, each stores one run
-            uint32_t w[4];
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int x = 0; x < 2; ++x)
-                w[2 * e + x] = T::pack(O[rs][d][8 * i + 4 * e + 2 * x] * f, O[rs][d][8 * i + 4 * e + 2 * x + 1] * f);
-            const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-            const auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-            if (tok[rs] >= 0)
-              *(u32x4*)(o + 32 * d + 16 * i + 8 * h) =
-                  u32x4{(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
-          }
-      }
+            for (int z = 0; z < 2; ++z)
+              w[2 * e + z] = T::pack(O[d][8 * i + 4 * e + 2 * z] * f, O[d][8 * i + 4 * e + 2 * z + 1] * f);
+          const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+          const auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+          if (tok < t.s.nq)
+            *(u32x4*)(o + 32 * d + 16 * i + 8 * h2) =
+                u32x4{(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
+        }
     }
     return;
   }
@@ -514,7 +597,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
   // Something non-finite among the sums: the wave's rows again, one at a time, over the keys
   // that each sees (lanes hold HD / 64 adjacent values).
   constexpr int E = HD / 64;
-  for (int r = 0; r < 32 * RS; ++r) {
+  for (int r = 0; r < 32; ++r) {
     const int R = R0 + r, i = R / a.G;
     if (i >= t.s.nq) break;
     const int hq = hk * a.G + (R - i * a.G);
@@ -530,9 +613,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
       const uint8_t* vp = base_of(a.kv.v, key, pc);
       float kv[E], vv[E], dot = 0.0f;
       if constexpr (Q8) {
-        const long long off = key & ((1 << a.kv.page_shift) - 1);
-        const float ks = a.kv.k.s[pc * a.kv.k.ssp + off * a.kv.k.sst + hk * a.kv.k.ssh];
-        const float vs = a.kv.v.s[pc * a.kv.v.ssp + off * a.kv.v.sst + hk * a.kv.v.ssh];
+        const float ks = *scale_of(a.kv.k, key, pc), vs = *scale_of(a.kv.v, key, pc);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           kv[e] = (float)((const int8_t*)kp)[lane * E + e] * ks;
@@ -548,7 +629,7 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
 #pragma unroll
       for (int e = 0; e < E; ++e) dot = fmaf(qv[e], kv[e], dot);
 #pragma unroll
-      for (int x = 1; x < 64; x <<= 1) dot += __shfl_xor(dot, x);
+      for (int z = 1; z < 64; z <<= 1) dot += __shfl_xor(dot, z);
       const float s = dot * a.c;
       const float mn = fmaxf(mr, s), ms = mn == kNegInf ? 0.0f : mn;
       const float al = exp2_(mr - ms), p = exp2_(s - ms);
@@ -559,13 +640,13 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
     }
     if (any_bad) lr = __builtin_nanf("");
     if (t.parts > 1) {
-      float* dst = slot_p + (wave * RS + r / 32) * 32 * HD;
+      float* dst = slot_p + wave * 32 * HD;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int d = lane * E + e;
-        dst[((d / 32) * 4 + (d % 32) / 8) * 256 + ((r % 32) + 32 * ((d % 8) / 4)) * 4 + d % 4] = o[e];
+        dst[((d / 32) * 4 + (d % 32) / 8) * 256 + (r + 32 * ((d % 8) / 4)) * 4 + d % 4] = o[e];
       }
-      if (lane == 0) *(float2*)(ml + ((wave * RS) * 32 + r) * 2) = float2{mr, lr};
+      if (lane == 0) *(float2*)(ml + (wave * 32 + r) * 2) = float2{mr, lr};
     } else {
       uint16_t* out = (uint16_t*)a.o + (long long)(t.s.q0 + i) * a.ot + hq * a.oh + lane * E;
       const bool none = seen(a, t.s, i) == 0;
@@ -576,19 +657,19 @@ __global__ __launch_bounds__(kPromptThreads, 1) void prompt_kernel(const PromptA
 }
 
 // Joins a cut tile's parts in key order: a workgroup takes one row set of 32.
-template <typename T, int HD, int RS>
+template <typename T, int HD>
 __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a) {
-  constexpr int ROWS = prompt_rows(RS);
-  constexpr int SETS = 4 * RS;
+  constexpr int ROWS = kPromptRows;
+  constexpr int SETS = ROWS / 32;
   const int set = (int)blockIdx.x % SETS, u = (int)blockIdx.x / SETS;
   const int hk = u % a.HKV;
   Tile t;
-  if (!find_tile<ROWS, false>(a, u / a.HKV, t) || t.parts == 1) return;
+  if (!find_tile<false>(a, u / a.HKV, t) || t.parts == 1) return;
   const int tid = (int)threadIdx.x;
   const int R = t.tile * ROWS + set * 32 + (tid & 31);
   const int i = R / a.G;
   if (i >= t.s.nq) return;
-  const long long sf = prompt_slot_floats(RS, HD);
+  const long long sf = prompt_slot_floats(HD);
   const float* p0 = a.part + ((long long)hk * a.units + t.slot) * sf;
   const float* ml = p0 + ROWS * HD + (set * 32 + (tid & 31)) * 2;
   float M = kNegInf;
@@ -616,33 +697,33 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const Promp
   }
 }
 
-template <typename T, int HD, int RS, bool Q8, bool PAGED>
+template <typename T, int HD, bool Q8, bool PAGED>
 hipError_t prompt_go(const PromptArgs& a, hipStream_t st) {
-  const size_t lds = (size_t)prompt_stages<Q8>() * PGeo<HD>::STAGE;
-  auto kern = prompt_kernel<T, HD, RS, Q8, PAGED>;
+  const size_t lds = (size_t)prompt_lds<HD, Q8>();
+  auto kern = prompt_kernel<T, HD, Q8, PAGED>;
   static const hipError_t attr = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                      (int)lds);
   if (attr != hipSuccess) return attr;
   hipLaunchKernelGGL(kern, dim3(grid_of(a.HKV, a.units)), dim3(kPromptThreads), lds, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.target == 0) return e;
-  hipLaunchKernelGGL((prompt_join_kernel<T, HD, RS>), dim3((unsigned)(a.tiles * a.HKV * 4 * RS)),
+  hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(a.tiles * a.HKV * (kPromptRows / 32))),
                      dim3(kPromptThreads), 0, st, a);
   return hipGetLastError();
 }
 
-template <typename T, int HD, int RS>
+template <typename T, int HD>
 hipError_t prompt_src(const PromptArgs& a, hipStream_t st) {
-  if (!a.kv.table) return prompt_go<T, HD, RS, false, false>(a, st);
-  if (a.kv.k.s) return prompt_go<T, HD, RS, true, true>(a, st);
-  return prompt_go<T, HD, RS, false, true>(a, st);
+  if (!a.kv.table) return prompt_go<T, HD, false, false>(a, st);
+  if (a.kv.k.s) return prompt_go<T, HD, true, true>(a, st);
+  return prompt_go<T, HD, false, true>(a, st);
 }
 
 template <typename T>
-hipError_t prompt_dispatch(const PromptArgs& a, int hd, int rs, hipStream_t st) {
-  if (hd == 256) return rs == 2 ? prompt_src<T, 256, 2>(a, st) : prompt_src<T, 256, 1>(a, st);
-  if (hd == 128) return rs == 2 ? prompt_src<T, 128, 2>(a, st) : prompt_src<T, 128, 1>(a, st);
-  return rs == 2 ? prompt_src<T, 64, 2>(a, st) : prompt_src<T, 64, 1>(a, st);
+hipError_t prompt_dispatch(const PromptArgs& a, int hd, hipStream_t st) {
+  if (hd == 256) return prompt_src<T, 256>(a, st);
+  if (hd == 128) return prompt_src<T, 128>(a, st);
+  return prompt_src<T, 64>(a, st);
 }
 
 }  // namespace
