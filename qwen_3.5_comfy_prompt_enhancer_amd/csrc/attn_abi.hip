@@ -42,6 +42,7 @@ constexpr int kMaxRows = 1 << 24;             // tokens of a call (rows of a key
 constexpr int kMaxGroup = 64;                 // query heads of a key head
 constexpr long long kMaxKeys = 1LL << 30;     // keys of a sequence
 constexpr long long kMaxTokenStride = 1LL << 26;  // eight rows' offset stays in 32 bits
+constexpr long long kMaxPageStride = (1LL << 31) - 16;  // in bytes below 2^32
 
 // One 16-bit (es = 2) or int8 tensor: n of the outer strides.  `write`: rows must not overlap.
 int check_tensor(const char* fn, const char* name, const void* p, int es, int hd, long long n0, long long s0,
@@ -89,6 +90,8 @@ int check_cache(const char* fn, const qlin_paged_kv* c, int hkv, int hd, int dty
   QA_TRY(check_tensor(fn, "v_cache", c->v, es, hd, c->page, c->v_token, hkv, c->v_head, write));
   if (c->k_page % mult || c->v_page % mult || c->k_page < 0 || c->v_page < 0)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides must be multiples of %d", fn, mult);
+  if (c->k_page > kMaxPageStride || c->v_page > kMaxPageStride)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides above %lld", fn, kMaxPageStride);
   if (write && c->num_pages > 1 && (c->k_page < hd || c->v_page < hd))
     return fail(QLIN_ERR_INVALID, "%s: pages of the cache overlap", fn);
   if (q8) {
@@ -98,7 +101,8 @@ int check_cache(const char* fn, const qlin_paged_kv* c, int hkv, int hd, int dty
     const int64_t st[6] = {c->ks_page, c->ks_token, c->ks_head, c->vs_page, c->vs_token, c->vs_head};
     const int n[3] = {c->num_pages, c->page, hkv};
     for (int i = 0; i < 6; ++i) {
-      if (st[i] < 0) return fail(QLIN_ERR_UNSUPPORTED, "%s: negative stride of the scales", fn);
+      if (st[i] < 0 || st[i] > (i % 3 ? kMaxTokenStride : kMaxPageStride / 2))
+        return fail(QLIN_ERR_UNSUPPORTED, "%s: stride of the scales negative or too large", fn);
       if (write && n[i % 3] > 1 && st[i] < 1) return fail(QLIN_ERR_INVALID, "%s: scales of the cache overlap", fn);
     }
   } else if (c->k_s || c->v_s) {
@@ -152,14 +156,17 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   }
   const long long tiles = (long long)a.T * a.G / kPromptRows + a.B;
   const long long slot = prompt_slot_floats(hd) * 4;
-  if (tiles * a.HKV >= 2048 || max_keys <= kPromptMinBlocks * kPromptBlock) target = 0;
-  // every unit of a key head has a slot: at most 2 target / HKV + tiles of them
-  target = std::min(target, ((long long)avail / slot / a.HKV - tiles - 1) * a.HKV / 2);
-  if (target <= a.HKV) target = 0;
+  if (max_keys <= kPromptMinBlocks * kPromptBlock) target = 0;
+  // every unit of a key head has a slot: at most 2 target / HKV + tiles of them (and two more for
+  // what the device's 32-bit estimate rounds)
+  target = std::min(target, ((long long)avail / slot / a.HKV - tiles - 3) * a.HKV / 2);
+  if (target <= a.HKV || tiles * a.HKV * kPromptCounters * 4 > (long long)counter_bytes()) target = 0;
   a.target = (int)target;
   a.tiles = (int)tiles;
-  a.units = (int)(tiles + (2 * target + a.HKV - 1) / a.HKV);
+  a.join_apart = tiles * a.HKV <= kPromptJoinApart;
+  a.units = (int)(tiles + (target ? (2 * target + a.HKV - 1) / a.HKV + 2 : 0));
   a.part = (float*)part;
+  a.cnt = (unsigned*)ws;
   return QLIN_OK;
 }
 
@@ -319,10 +326,10 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   long long target = std::min(std::max(1LL, total / hg), std::max(1LL, B * ((blocks + kDecodeChunk - 1) / kDecodeChunk)));
   const long long slot = (long long)decode_slot_floats(std::min(16, a.G), hd) * 4;
   // without room for the parts (very many sequences) every sequence is one unit
-  if ((target + B) * hg * slot > (long long)avail || B * hg * kDecodeCounters * 4 > (long long)counter_bytes())
+  if ((target + B + 2) * hg * slot > (long long)avail || B * hg * kDecodeCounters * 4 > (long long)counter_bytes())
     target = 0;
   a.target = (int)target;
-  a.units = (int)(target + B);
+  a.units = (int)(target + B + (target ? 2 : 0));  // (two for what the device's estimate rounds)
   a.part = (float*)part;
   a.cnt = (unsigned*)workspace;
   return status(fn, launch_decode(a, dtype, hd, (hipStream_t)stream));

@@ -42,43 +42,32 @@ struct Unit {
   int base;       // number of part 0
 };
 
-__device__ __forceinline__ long long wave_sum(long long v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-  return v;
-}
-
 __device__ __forceinline__ int blocks_of(int len) { return (len + kDecodeBlock - 1) / kDecodeBlock; }
 
 __device__ __forceinline__ bool find_unit(const DecodeArgs& a, int u, Unit& r) {
   const int lane = (int)threadIdx.x & 63;
-  long long total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) total += b0 + lane < a.B ? blocks_of(kv_length(a.kv, b0 + lane)) : 0;
-  total = wave_sum(total);
+  auto mine = [&](int b0) { return b0 + lane < a.B ? kv_length(a.kv, b0 + lane) : 0; };
+  const int first = mine(0);
   int chunk = 1 << 28;
   if (a.target > 0) {
-    chunk = (int)((total + a.target - 1) / a.target);
-    chunk = (max(chunk, 1) + kDecodeChunk - 1) / kDecodeChunk * kDecodeChunk;
+    float total = 0.0f;  // (rounded up below; the same for all workgroups)
+    for (int b0 = 0; b0 < a.B; b0 += 64) total += (float)blocks_of(b0 ? mine(b0) : first);
+    total = lane_value(wave_scan(total), 63);
+    chunk = max((int)fminf(ceilf(total / (float)a.target), 1e8f), 1);
+    chunk = (chunk + kDecodeChunk - 1) / kDecodeChunk * kDecodeChunk;
   }
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int len = b0 + lane < a.B ? kv_length(a.kv, b0 + lane) : 0;
+    const int len = b0 ? mine(b0) : first;
     // an empty sequence has one part, which writes its zeros
     const int parts = b0 + lane < a.B ? max(1, (blocks_of(len) + chunk - 1) / chunk) : 0;
-    int end = parts;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int o = __shfl_up(end, m);
-      if (lane >= m) end += o;
-    }
-    const int sum = __shfl(end, 63);
+    const int end = wave_scan(parts), sum = lane_value(end, 63);
     if (u < base + sum) {
-      const uint64_t past = __ballot(base + end > u);
-      const int at = __builtin_ctzll(past);
+      const int at = __builtin_ctzll(__ballot(base + end > u));
       r.b = b0 + at;
-      r.len = (int)rfl32((uint32_t)__shfl(len, at));
-      r.parts = (int)rfl32((uint32_t)__shfl(parts, at));
-      r.base = (int)rfl32((uint32_t)(base + __shfl(end - parts, at)));
+      r.len = lane_value(len, at);
+      r.parts = lane_value(parts, at);
+      r.base = base + lane_value(end, at) - r.parts;
       r.s = u - r.base;
       r.chunk = chunk;
       return true;
@@ -131,6 +120,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a)
   const int hh = (int)blockIdx.x % hg, unit = (int)blockIdx.x / hg;
   Unit U;
   if (!find_unit(a, unit, U)) return;
+  for (int* x : {&U.b, &U.s, &U.len, &U.chunk, &U.parts, &U.base}) *x = (int)rfl32((uint32_t)*x);
   const int hk = hh % a.HKV, gi = hh / a.HKV;
   const int rows = min(16, a.G - 16 * gi);
   const int head0 = hk * a.G + 16 * gi;

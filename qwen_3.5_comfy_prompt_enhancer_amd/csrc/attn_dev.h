@@ -59,6 +59,29 @@ __device__ __forceinline__ int kv_length(const KvSrc& kv, int b) {
   return n < 0 ? 0 : (long long)n > most ? (int)most : n;
 }
 
+// Inclusive prefix sum over a wave (rows of 16 by shifts, then across rows), without LDS.
+template <typename N>
+__device__ __forceinline__ N wave_scan(N v) {
+  auto add = [&](auto ctrl, auto rows) {
+    const int m = __builtin_amdgcn_update_dpp(0, bitcast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    v += bitcast<N>(m);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr 1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast 15, 31
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return v;
+}
+
+// The value of one lane (a uniform number), the same on all.
+template <typename N>
+__device__ __forceinline__ N lane_value(N v, int at) {
+  return bitcast<N>(__builtin_amdgcn_readlane(bitcast<int>(v), at));
+}
+
 // 2^x, and the factor between two running maxima (in powers of two) of which the first may be
 // -inf: nothing was seen yet, or scores of -inf alone.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }

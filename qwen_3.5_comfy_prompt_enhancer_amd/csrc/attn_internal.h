@@ -100,11 +100,15 @@ struct PromptArgs {
   float c;                // scale * log2(e)
   int target;             // work units to cut the keys into; 0: no cut
   int units;              // units per key head: the grid's bound
-  int tiles;              // row tiles per key head: the join's bound
+  int tiles;              // row tiles per key head at most
+  int join_apart;         // parts are joined by a launch of its own
   float* part;            // unit partials [key head][unit]
+  unsigned* cnt;          // arrival counters of each tile, zero between calls
 };
 constexpr int kPromptBlock = 32;     // keys of a step
 constexpr int kPromptMinBlocks = 4;  // shortest cut
+constexpr int kPromptJoinApart = 64;  // row tiles of all key heads up to which a second launch joins
+constexpr int kPromptCounters = 32;  // counters of a (key head, row tile)
 constexpr int kPromptRows = 128;     // rows of a tile: tokens x the query heads of a key head
 // a unit's partial: sums of its rows, then (maximum, sum of P) of each
 __host__ __device__ constexpr long long prompt_slot_floats(int hd) { return (long long)kPromptRows * (hd + 2); }

@@ -23,7 +23,7 @@
 //     2^8, which both 16-bit types hold with full relative precision.  P is rounded to the
 //     queries' type for its product; its sum, the maximum and O are 32-bit.
 //   * Keys of all tiles are cut into about equal units where there are fewer tiles than the chip
-//     holds; units leave 32-bit partial sums, which a second launch joins in key order.
+//     holds; units leave 32-bit partial sums, which the last unit of a tile joins in key order.
 //
 // A row's masked keys have no part in it whatever they hold: scores are replaced before the
 // maximum, and as zero times a value that is no number is none, a tile whose sums come out
@@ -49,9 +49,9 @@ __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 
-// 4-byte LDS DMA: lane i copies 4 bytes from its own address to LDS m0 + 4 i.
-__device__ __forceinline__ void dma4(const void* p, uint32_t m0) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(p), "{m0}"(m0) : "memory");
+// 4-byte LDS DMA: lane i copies 4 bytes from sbase + voff to LDS m0 + 4 i.
+__device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, uint32_t m0) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 
 // LDS operands that are read ahead of their products.
@@ -94,65 +94,72 @@ struct Tile {
   int b, tile;        // sequence, row tile
   Seq s;
   int nblk;           // key blocks that the tile sees
+  int chunk;          // blocks of a unit
   int parts, part;    // units of the tile, this one
-  int slot;           // partial of the tile's first unit
+  int slot, step;     // partial of the tile's first unit, and the distance to the next
+  int index;          // number of the tile among those of its key head
   // the same for all lanes, which the compiler cannot see
   __device__ __forceinline__ void uniform() {
-    for (int* x : {&b, &tile, &s.q0, &s.nq, &s.k0, &s.nk, &nblk, &parts, &part, &slot}) *x = (int)rfl32((uint32_t)*x);
+    for (int* x : {&b, &tile, &s.q0, &s.nq, &s.k0, &s.nk, &nblk, &chunk, &parts, &part, &slot, &step, &index})
+      *x = (int)rfl32((uint32_t)*x);
   }
 };
 
-// Work unit u (UNITS) or row tile u of a key head.  Tiles of a sequence are numbered from the
-// last, which sees most keys, so that long units start first.
+// Work unit u (UNITS), or the first unit of row tile u, of a key head.
+//
+// Tiles of a sequence are ranked from its last, which sees most keys.  A unit is `chunk` blocks of
+// a tile's keys, the tile's last unit what is left; units are numbered part by part, by rank
+// within a part.  With chunk the average over the workgroups that run at once, long causal
+// prompts then come out even: whole chunks start first, and the workgroup that gets the
+// shortest rest of one part goes on with the longest of the next.
 template <bool UNITS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
   constexpr int ROWS = kPromptRows;
   const int lane = (int)threadIdx.x & 63;
+  auto mine = [&](int b0) {
+    Seq s = {0, 0, 0, 0};
+    if (b0 + lane < a.B) s = seq_of(a, b0 + lane);
+    return s;
+  };
+  auto tiles_of = [&](const Seq& s) { return (int)(((long long)s.nq * a.G + ROWS - 1) / ROWS); };
+  auto blocks_of = [&](const Seq& s) { return (s.nk + kPromptBlock - 1) / kPromptBlock; };
+  const Seq first = mine(0);
   int chunk = 1 << 30;
   if (a.target > 0) {
-    long long w = 0;
+    float w = 0.0f;  // (an estimate; the same for all workgroups)
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      if (b0 + lane < a.B) {
-        const Seq s = seq_of(a, b0 + lane);
-        const long long t = ((long long)s.nq * a.G + ROWS - 1) / ROWS;
-        const long long n = (s.nk + kPromptBlock - 1) / kPromptBlock;
-        // causal rows see half of their own keys on average (never less than half of all)
-        w += a.causal ? max(t * n - t * (s.nq / (2 * kPromptBlock)), (t * n + 1) / 2) : t * n;
-      }
+      const Seq s = b0 ? mine(b0) : first;
+      const float t = (float)tiles_of(s), n = (float)blocks_of(s);
+      // causal rows see half of their own keys on average (never less than half of all)
+      w += a.causal ? fmaxf(t * (n - (float)(s.nq / (2 * kPromptBlock))), t * n * 0.5f) : t * n;
     }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) w += __shfl_xor(w, m);
-    chunk = (int)min((w * a.HKV + a.target - 1) / a.target, (long long)1 << 30);
-    chunk = max(chunk, kPromptMinBlocks);
+    w = lane_value(wave_scan(w), 63);
+    chunk = max((int)fminf(ceilf(w * (float)a.HKV / (float)a.target), 1e9f), kPromptMinBlocks);
   }
   int ubase = 0, tbase = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    Seq s = {0, 0, 0, 0};
-    if (b0 + lane < a.B) s = seq_of(a, b0 + lane);
-    const int tiles = (int)(((long long)s.nq * a.G + ROWS - 1) / ROWS);
-    const int n = (s.nk + kPromptBlock - 1) / kPromptBlock;
-    const int most = max(1, (n + chunk - 1) / chunk);
-    int ue = tiles * most, te = tiles;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int x = __shfl_up(ue, m), y = __shfl_up(te, m);
-      if (lane >= m) ue += x, te += y;
-    }
-    const int usum = __shfl(ue, 63), tsum = __shfl(te, 63);
+    const Seq s = b0 ? mine(b0) : first;
+    const int tiles = tiles_of(s);
+    const int most = max(1, (blocks_of(s) + chunk - 1) / chunk);
+    const int ue = wave_scan(tiles * most), te = wave_scan(tiles);
+    const int usum = lane_value(ue, 63), tsum = lane_value(te, 63);
     if (u < (UNITS ? ubase + usum : tbase + tsum)) {
       const int at = __builtin_ctzll(__ballot((UNITS ? ubase + ue : tbase + te) > u));
       r.b = b0 + at;
-      r.s.q0 = (int)rfl32((uint32_t)__shfl(s.q0, at));
-      r.s.nq = (int)rfl32((uint32_t)__shfl(s.nq, at));
-      r.s.k0 = (int)rfl32((uint32_t)__shfl(s.k0, at));
-      r.s.nk = (int)rfl32((uint32_t)__shfl(s.nk, at));
-      const int nt = (int)rfl32((uint32_t)__shfl(tiles, at)), mp = (int)rfl32((uint32_t)__shfl(most, at));
-      const int u0 = ubase + (int)rfl32((uint32_t)__shfl(ue, at)) - nt * mp;
-      const int t0 = tbase + (int)rfl32((uint32_t)__shfl(te, at)) - nt;
-      const int rank = UNITS ? (u - u0) / mp : u - t0;
-      r.part = UNITS ? (u - u0) % mp : 0;
+      r.s.q0 = lane_value(s.q0, at);
+      r.s.nq = lane_value(s.nq, at);
+      r.s.k0 = lane_value(s.k0, at);
+      r.s.nk = lane_value(s.nk, at);
+      const int nt = lane_value(tiles, at), mp = lane_value(most, at);
+      const int u0 = ubase + lane_value(ue, at) - nt * mp;
+      const int t0 = tbase + lane_value(te, at) - nt;
+      const int rank = UNITS ? (u - u0) % nt : u - t0;
+      r.part = UNITS ? (u - u0) / nt : 0;
       r.tile = nt - 1 - rank;
-      r.slot = u0 + rank * mp;
+      r.index = t0 + rank;
+      r.slot = u0 + rank;
+      r.step = nt;
+      r.chunk = chunk;
       const int last = min((int)(((long long)(r.tile + 1) * ROWS - 1) / a.G), r.s.nq - 1);
       r.nblk = (seen(a, r.s, last) + kPromptBlock - 1) / kPromptBlock;
       r.parts = max(1, (r.nblk + chunk - 1) / chunk);
@@ -213,11 +220,11 @@ constexpr int prompt_lds() {
 
 template <typename V>
 __device__ __forceinline__ V lds_ld(uint32_t at) {
-  return *(const __attribute__((address_space(3))) V*)at;
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
 }
 template <typename V>
 __device__ __forceinline__ void lds_st(uint32_t at, V v) {
-  *(__attribute__((address_space(3))) V*)at = v;
+  *(__attribute__((address_space(3))) V*)(uintptr_t)at = v;
 }
 
 // Q8: int8 cache.
@@ -241,8 +248,7 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
   const int tid = (int)threadIdx.x;
   const int wave = (int)rfl32((uint32_t)tid >> 6), lane = tid & 63;
   const int col = lane & 31, h = lane >> 5;
-  const int per = (t.nblk + t.parts - 1) / t.parts;
-  const int kb0 = t.part * per, kb1 = min(t.nblk, kb0 + per);
+  const int kb0 = t.part * t.chunk, kb1 = min(t.nblk - kb0, t.chunk) + kb0;
 
   // this lane's row is R0 + col
   const int R0 = t.tile * ROWS + wave * 32;
@@ -275,13 +281,24 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
   auto page_of = [&](int kb) {
     return PAGED ? ((const __attribute__((address_space(4))) int*)table)[key8_of(kb) >> a.kv.page_shift] : 0;
   };
-  auto base_of = [&](const PagedTensor& x, int key8, int pid) {
-    const long long at = PAGED ? pid * x.sp + (key8 & ((1 << a.kv.page_shift) - 1)) * x.st
-                               : (long long)(t.s.k0 + key8) * x.st;
-    return (const uint8_t*)x.p + (at + hk * x.sh) * ES;
+  // places of this head's keys: strides below 2^32 bytes, products of 64 bits
+  struct Place {
+    const uint8_t* p;
+    uint32_t sp, st;
   };
-  auto scale_of = [&](const PagedTensor& x, int key8, int pid) {
-    return x.s + pid * x.ssp + (key8 & ((1 << a.kv.page_shift) - 1)) * x.sst + hk * x.ssh;
+  auto place = [&](const PagedTensor& x) {
+    return Place{(const uint8_t*)x.p + ((PAGED ? 0LL : (long long)t.s.k0 * x.st) + hk * x.sh) * ES,
+                 (uint32_t)x.sp * ES, (uint32_t)x.st * ES};
+  };
+  auto scale_place = [&](const PagedTensor& x) {
+    return Place{(const uint8_t*)(x.s + hk * x.ssh), (uint32_t)x.ssp * 4u, (uint32_t)x.sst * 4u};
+  };
+  const Place kpl = place(a.kv.k), vpl = place(a.kv.v);
+  const Place kspl = scale_place(a.kv.k), vspl = scale_place(a.kv.v);
+  const uint32_t pmask = PAGED ? (1u << a.kv.page_shift) - 1u : 0u;
+  auto base_of = [&](const Place& x, int key, int pid) {
+    return PAGED ? x.p + ((uint64_t)(uint32_t)pid * x.sp + (uint64_t)((uint32_t)key & pmask) * x.st)
+                 : x.p + (uint64_t)(uint32_t)key * x.st;
   };
   auto checked = [&](int pid) {
     if (PAGED && (unsigned)pid >= (unsigned)a.kv.num_pages) {
@@ -301,8 +318,8 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     const int key8 = key8_of(kb);
     pid = checked(pid);
     const int rmax = nk - 1 - key8;
-    const uint8_t* kp = rfl_p(base_of(a.kv.k, key8, pid));
-    const uint8_t* vp = rfl_p(base_of(a.kv.v, key8, pid));
+    const uint8_t* kp = rfl_p(base_of(kpl, key8, pid));
+    const uint8_t* vp = rfl_p(base_of(vpl, key8, pid));
     if constexpr (!Q8) {
       const uint32_t at = stage + (uint32_t)(8 * wave * G::ROWB);
 #pragma unroll
@@ -311,8 +328,8 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
         const int ck = p16 ^ G::swk(row);
         const int cv = (((p16 >> 2) ^ G::swv(row)) << 2) | (p16 & 3);
         const uint32_t rc = (uint32_t)min(r, rmax);
-        dma16(kp, rc * (uint32_t)(a.kv.k.st * 2) + (uint32_t)ck * 16u, at + (uint32_t)(G::RPI * i * G::ROWB));
-        dma16(vp, rc * (uint32_t)(a.kv.v.st * 2) + (uint32_t)cv * 16u,
+        dma16(kp, rc * kpl.st + (uint32_t)ck * 16u, at + (uint32_t)(G::RPI * i * G::ROWB));
+        dma16(vp, rc * vpl.st + (uint32_t)cv * 16u,
               at + (uint32_t)(G::HALF + G::RPI * i * G::ROWB));
       }
     } else {
@@ -324,16 +341,15 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
         for (int i = 0; i < (R8 < 8 ? 8 / R8 : 1); ++i) {
           const uint32_t rc = (uint32_t)min(R8 * i + lane / L8, rmax);
           const uint32_t c = (uint32_t)(lane % L8) * 16u;
-          dma16(kp, rc * (uint32_t)a.kv.k.st + c, at + (uint32_t)(R8 * i * HD));
-          dma16(vp, rc * (uint32_t)a.kv.v.st + c, at + (uint32_t)(G::KB * HD + R8 * i * HD));
+          dma16(kp, rc * kpl.st + c, at + (uint32_t)(R8 * i * HD));
+          dma16(vp, rc * vpl.st + c, at + (uint32_t)(G::KB * HD + R8 * i * HD));
         }
       }
-      const float* ks = scale_of(a.kv.k, key8, pid);
-      const float* vs = scale_of(a.kv.v, key8, pid);
-      if (lane < 16) {
-        const int r = min(lane & 7, rmax);
-        const float* p = lane < 8 ? ks + r * a.kv.k.sst : vs + r * a.kv.v.sst;
-        dma4(p, stage + (uint32_t)(G::STAGE / 2 + 64 * wave));
+      if (lane < 8) {
+        const uint32_t r = (uint32_t)min(lane, rmax);
+        const uint32_t sc = stage + (uint32_t)(G::STAGE / 2 + 64 * wave);
+        dma4(rfl_p(base_of(kspl, key8, pid)), r * kspl.st, sc);
+        dma4(rfl_p(base_of(vspl, key8, pid)), r * vspl.st, sc + 32u);
       }
     }
   };
@@ -465,7 +481,7 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
         const int d = x / 2, k = x % 2;
         const uint32_t at = (va ^ (uint32_t)((d & 3) << 6)) + stage +
                             (uint32_t)((d >> 2) * 256 + (16 * k + 8 * z) * G::ROWB);
-        v[z] = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+        v[z] = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
       }
       return u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
     };
@@ -535,12 +551,15 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // (the row again, from a thread index that the compiler takes for another, so that nothing of
-  // it is kept in registers through the loop)
+  // (the row again, from a thread index that the compiler takes for another, and the arguments read
+  // again, so that nothing of what follows is kept in registers through the loop)
   int tid2 = (int)threadIdx.x;
   asm volatile("" : "+v"(tid2));
-  const int row = R0 + (tid2 & 31), tok = row / a.G;
-  const int head = hk * a.G + (row - tok * a.G);
+  auto kernarg = (const __attribute__((address_space(4))) PromptArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(kernarg));
+  const PromptArgs& ea = *(const PromptArgs*)kernarg;
+  const int row = R0 + (tid2 & 31), tok = row / ea.G;
+  const int head = hk * ea.G + (row - tok * ea.G);
   const int h2 = (tid2 >> 5) & 1;
 
   float x, y;
@@ -555,24 +574,41 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
       for (int i = 0; i < 16; ++i) z = fmaf(O[d][i], 0.0f, z);
     again = !(z == 0.0f) && tok < t.s.nq;
   }
-  float* slot_p = a.part + ((long long)hk * a.units + t.slot + t.part) * prompt_slot_floats(HD);
-  float* ml = slot_p + ROWS * HD;
+  // partials: unit p of the tile at (slot + p step) of the key head's; 32-bit sums by row set,
+  // 32-wide block, run of 8 values and lane, so that a wave moves 1 KiB at a time; then (maximum, sum
+  // of P) of each row
+  constexpr unsigned SLOT = (unsigned)prompt_slot_floats(HD) * 4u;
+  const __amdgpu_buffer_rsrc_t rs =
+      part_rsrc((const char*)ea.part + (long long)hk * ea.units * SLOT + (long long)t.slot * SLOT, 0x7FFFFFF0u);
+  const unsigned stride = (unsigned)t.step * SLOT;
+  constexpr unsigned ML = ROWS * HD * 4;
+  auto st_ml = [&](unsigned part, int r, float M, float ls) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    __builtin_amdgcn_raw_buffer_store_b64(bitcast<u32x2>(f32x2{M, ls}), rs, part * stride + ML + (unsigned)r * 8u, 0,
+                                          kCpolSc1);
+  };
+  auto ld_ml = [&](unsigned part, int r) {
+    return __builtin_amdgcn_raw_buffer_load_b64(rs, part * stride + ML + (unsigned)r * 8u, 0, kCpolSc1);
+  };
   const bool any_bad = __any(bad);
 
   if (!__any(again)) {
     if (any_bad) l = __builtin_nanf("");
     if (t.parts > 1) {
-      float* dst = slot_p + wave * 32 * HD + (tid2 & 63) * 4;
+      if (R0 / ea.G < t.s.nq) {
+        const unsigned at = (unsigned)t.part * stride + (unsigned)(wave * 32 * HD * 4) + (unsigned)(tid2 & 63) * 16u;
 #pragma unroll
-      for (int d = 0; d < G::ND; ++d)
+        for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(f32x4*)(dst + (d * 4 + i) * 256) = f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
-      if (h2 == 0) *(float2*)(ml + (wave * 32 + (tid2 & 31)) * 2) = float2{m, l};
+          for (int i = 0; i < 4; ++i)
+            st_coherent(f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]}, rs,
+                        at + (unsigned)(d * 4 + i) * 1024u);
+        if (h2 == 0) st_ml((unsigned)t.part, wave * 32 + (tid2 & 31), m, l);
+      }
     } else {
       // a row that sees no key is zero
-      const float f = seen(a, t.s, min(tok, t.s.nq - 1)) > 0 ? 1.0f / l : 0.0f;
-      uint16_t* o = (uint16_t*)a.o + (long long)(t.s.q0 + tok) * a.ot + head * a.oh;
+      const float f = seen(ea, t.s, min(tok, t.s.nq - 1)) > 0 ? 1.0f / l : 0.0f;
+      uint16_t* o = (uint16_t*)ea.o + (long long)(t.s.q0 + tok) * ea.ot + head * ea.oh;
 #pragma unroll
       for (int d = 0; d < G::ND; ++d)
 #pragma unroll
@@ -591,29 +627,29 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
                 u32x4{(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
         }
     }
-    return;
   }
 
   // Something non-finite among the sums: the wave's rows again, one at a time, over the keys
   // that each sees (lanes hold HD / 64 adjacent values).
   constexpr int E = HD / 64;
-  for (int r = 0; r < 32; ++r) {
-    const int R = R0 + r, i = R / a.G;
+  const int redo = __any(again) ? 32 : 0;
+  for (int r = 0; r < redo; ++r) {
+    const int R = R0 + r, i = R / ea.G;
     if (i >= t.s.nq) break;
-    const int hq = hk * a.G + (R - i * a.G);
-    const int k1 = min(kb1 * G::KB, seen(a, t.s, i));
-    const uint16_t* q = (const uint16_t*)a.q + (t.s.q0 + i) * a.qt + hq * a.qh + lane * E;
+    const int hq = hk * ea.G + (R - i * ea.G);
+    const int k1 = min(kb1 * G::KB, seen(ea, t.s, i));
+    const uint16_t* q = (const uint16_t*)ea.q + (t.s.q0 + i) * ea.qt + hq * ea.qh + lane * E;
     float qv[E], o[E], mr = kNegInf, lr = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) qv[e] = T::get(q[e]), o[e] = 0.0f;
     for (int key = kb0 * G::KB; key < k1; ++key) {
-      const int pid = PAGED ? table[key >> a.kv.page_shift] : 0;
-      const int pc = (unsigned)pid >= (unsigned)a.kv.num_pages ? 0 : pid;
-      const uint8_t* kp = base_of(a.kv.k, key, pc);
-      const uint8_t* vp = base_of(a.kv.v, key, pc);
+      const int pid = PAGED ? table[key >> ea.kv.page_shift] : 0;
+      const int pc = (unsigned)pid >= (unsigned)ea.kv.num_pages ? 0 : pid;
+      const uint8_t* kp = base_of(kpl, key, pc);
+      const uint8_t* vp = base_of(vpl, key, pc);
       float kv[E], vv[E], dot = 0.0f;
       if constexpr (Q8) {
-        const float ks = *scale_of(a.kv.k, key, pc), vs = *scale_of(a.kv.v, key, pc);
+        const float ks = *(const float*)base_of(kspl, key, pc), vs = *(const float*)base_of(vspl, key, pc);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           kv[e] = (float)((const int8_t*)kp)[lane * E + e] * ks;
@@ -630,7 +666,7 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
       for (int e = 0; e < E; ++e) dot = fmaf(qv[e], kv[e], dot);
 #pragma unroll
       for (int z = 1; z < 64; z <<= 1) dot += __shfl_xor(dot, z);
-      const float s = dot * a.c;
+      const float s = dot * ea.c;
       const float mn = fmaxf(mr, s), ms = mn == kNegInf ? 0.0f : mn;
       const float al = exp2_(mr - ms), p = exp2_(s - ms);
       mr = mn;
@@ -640,61 +676,166 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     }
     if (any_bad) lr = __builtin_nanf("");
     if (t.parts > 1) {
-      float* dst = slot_p + wave * 32 * HD;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int d = lane * E + e;
-        dst[((d / 32) * 4 + (d % 32) / 8) * 256 + (r + 32 * ((d % 8) / 4)) * 4 + d % 4] = o[e];
+        __builtin_amdgcn_raw_buffer_store_b32(
+            bitcast<uint32_t>(o[e]), rs,
+            (unsigned)t.part * stride + (unsigned)(wave * 32 * HD * 4) +
+                (unsigned)(((d / 32) * 4 + (d % 32) / 8) * 256 + (r + 32 * ((d % 8) / 4)) * 4 + d % 4) * 4u,
+            0, kCpolSc1);
       }
-      if (lane == 0) *(float2*)(ml + (wave * 32 + r) * 2) = float2{mr, lr};
+      if (lane == 0) st_ml((unsigned)t.part, wave * 32 + r, mr, lr);
     } else {
-      uint16_t* out = (uint16_t*)a.o + (long long)(t.s.q0 + i) * a.ot + hq * a.oh + lane * E;
-      const bool none = seen(a, t.s, i) == 0;
+      uint16_t* out = (uint16_t*)ea.o + (long long)(t.s.q0 + i) * ea.ot + hq * ea.oh + lane * E;
+      const bool none = seen(ea, t.s, i) == 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) out[e] = to_out16(none ? 0.0f : o[e] / lr, T::DT);
     }
   }
+  if (t.parts == 1 || ea.join_apart) return;
+
+  // The last unit of a group of parts to arrive adds them in key order, the last of the groups adds
+  // the groups' sums: the result does not depend on who was last, and no workgroup adds more than
+  // the square root of the parts (or 4).  Waves share the 32-wide blocks of the row sets there are.
+  __shared__ int s_last;
+  auto last_of = [&](unsigned* c, int n) {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's stores have been made
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (tid == 0) {
+      const unsigned prev = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int last = prev == (unsigned)(n - 1);
+      if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = last;
+    }
+    __syncthreads();
+    const bool r = s_last != 0;
+    __syncthreads();
+    return r;
+  };
+  const int sets = min(4, (int)(((long long)(t.s.nq - 1) * ea.G + ea.G - (long long)t.tile * ROWS + 31) / 32));
+  // parts first, first + by, ... (n): to the output, or in place of the first
+  auto join = [&](int first, int by, int n, bool final) {
+    for (int w = wave; w < sets * G::ND; w += 4) {
+      const int set = w / G::ND, d = w % G::ND;
+      const int R2 = t.tile * ROWS + set * 32 + col, i = R2 / ea.G;
+      f32x4 o[4] = {};
+      float M = kNegInf, ls = 0.0f;
+      const unsigned off = (unsigned)((set * G::ND + d) * 4096 + lane * 16);
+      constexpr int N = 4;  // parts in flight
+      for (int s0 = 0; s0 < n; s0 += N) {
+        f32x4 x[N][4];
+        u32x2 y[N];
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+          const unsigned p = (unsigned)(first + min(s0 + s, n - 1) * by);
+          y[s] = ld_ml(p, set * 32 + col);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) x[s][f] = ld_coherent(rs, p * stride + off + (unsigned)f * 1024u);
+        }
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+          if (s0 + s >= n) break;
+          const float pm = bitcast<float>(y[s].x);
+          const float mn = fmaxf(M, pm), ms = mn == kNegInf ? 0.0f : mn;
+          const float e0 = exp2_(M - ms), e1 = exp2_(pm - ms);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) o[f] = o[f] * e0 + x[s][f] * e1;
+          ls = ls * e0 + bitcast<float>(y[s].y) * e1;
+          M = mn;
+        }
+      }
+      if (final) {
+        if (i < t.s.nq) {
+          const float inv = seen(ea, t.s, i) > 0 ? 1.0f / ls : 0.0f;
+          uint16_t* out = (uint16_t*)ea.o + (long long)(t.s.q0 + i) * ea.ot + (hk * ea.G + (R2 - i * ea.G)) * ea.oh;
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            *(u32x2*)(out + d * 32 + f * 8 + 4 * h) =
+                u32x2{T::pack(o[f][0] * inv, o[f][1] * inv), T::pack(o[f][2] * inv, o[f][3] * inv)};
+        }
+      } else {
+        // (these values were read by this lane alone; maxima and sums by every wave, so they wait)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) st_coherent(o[f], rs, (unsigned)first * stride + off + (unsigned)f * 1024u);
+      }
+    }
+    if (final) return;
+    float M = kNegInf, ls = 0.0f;
+    for (int s = 0; s < n && wave < sets; ++s) {
+      const u32x2 y = ld_ml((unsigned)(first + s * by), wave * 32 + col);
+      const float pm = bitcast<float>(y.x), mn = fmaxf(M, pm), ms = mn == kNegInf ? 0.0f : mn;
+      ls = ls * exp2_(M - ms) + bitcast<float>(y.y) * exp2_(pm - ms);
+      M = mn;
+    }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (wave < sets && h == 0) st_ml((unsigned)first, wave * 32 + col, M, ls);
+  };
+  unsigned* cnt = ea.cnt + ((long long)hk * ea.tiles + t.index) * kPromptCounters;
+  int by = 4;
+  while (by * by < t.parts || by * (kPromptCounters - 1) < t.parts) ++by;
+  const int groups = (t.parts + by - 1) / by, gq = t.part / by;
+  if (!last_of(cnt + 1 + gq, min(by, t.parts - gq * by))) return;
+  if (groups > 1) {
+    join(gq * by, 1, min(by, t.parts - gq * by), false);
+    if (!last_of(cnt, groups)) return;
+    join(0, by, groups, true);
+  } else {
+    join(0, 1, t.parts, true);
+  }
 }
 
-// Joins a cut tile's parts in key order: a workgroup takes one row set of 32.
+// The join as a launch of its own, for few tiles cut many times: a workgroup takes 32 values of 32
+// rows, a thread four, so that the whole chip reads the parts.  (In the kernel above one workgroup
+// would read a tile's: 512 tokens over 6000 keys 86 us against 68 so; an 8192-token prompt's 250
+// tiles of two parts 272 against 304.)
 template <typename T, int HD>
 __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a) {
   constexpr int ROWS = kPromptRows;
-  constexpr int SETS = ROWS / 32;
-  const int set = (int)blockIdx.x % SETS, u = (int)blockIdx.x / SETS;
+  constexpr int SETS = ROWS / 32, ND = HD / 32;
+  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int d = (int)blockIdx.x % ND, set = (int)blockIdx.x / ND % SETS, u = (int)blockIdx.x / (ND * SETS);
   const int hk = u % a.HKV;
   Tile t;
-  if (!find_tile<false>(a, u / a.HKV, t) || t.parts == 1) return;
-  const int tid = (int)threadIdx.x;
-  const int R = t.tile * ROWS + set * 32 + (tid & 31);
-  const int i = R / a.G;
-  if (i >= t.s.nq) return;
-  const long long sf = prompt_slot_floats(HD);
-  const float* p0 = a.part + ((long long)hk * a.units + t.slot) * sf;
-  const float* ml = p0 + ROWS * HD + (set * 32 + (tid & 31)) * 2;
-  float M = kNegInf;
-  for (int s = 0; s < t.parts; ++s) M = fmaxf(M, ml[s * sf]);
-  const float Ms = M == kNegInf ? 0.0f : M;
-  constexpr int F = HD * 8 / kPromptThreads;  // float4s of a thread
-  f32x4 o[F];
-  float l = 0.0f;
+  if (!find_tile<false>(a, u / a.HKV, t)) return;
+  t.uniform();
+  const int R = t.tile * ROWS + set * 32 + (lane & 31), i = R / a.G;
+  if (t.parts == 1 || i >= t.s.nq) return;
+  const long long sf = prompt_slot_floats(HD) * t.step;
+  const float* p0 = a.part + ((long long)hk * a.units + t.slot) * prompt_slot_floats(HD);
+  const float* ml = p0 + ROWS * HD + (set * 32 + (lane & 31)) * 2;
+  const float* po = p0 + set * 32 * HD + d * 1024 + tid * 4;
+  f32x4 o = {0, 0, 0, 0};
+  float M = kNegInf, l = 0.0f;
+  constexpr int N = 8;  // parts in flight
+  for (int s0 = 0; s0 < t.parts; s0 += N) {
+    f32x4 x[N];
+    float2 y[N];
 #pragma unroll
-  for (int f = 0; f < F; ++f) o[f] = f32x4{0, 0, 0, 0};
-  for (int s = 0; s < t.parts; ++s) {
-    const float e = exp2_(ml[s * sf] - Ms);
-    l += ml[s * sf + 1] * e;
-    const float* p = p0 + s * sf + set * 32 * HD + tid * 4;
+    for (int s = 0; s < N; ++s) {
+      const long long at = min(s0 + s, t.parts - 1) * sf;
+      x[s] = *(const f32x4*)(po + at);
+      y[s] = *(const float2*)(ml + at);
+    }
 #pragma unroll
-    for (int f = 0; f < F; ++f) o[f] += *(const f32x4*)(p + f * kPromptThreads * 4) * e;
+    for (int s = 0; s < N; ++s) {
+      if (s0 + s >= t.parts) break;
+      const float mn = fmaxf(M, y[s].x), ms = mn == kNegInf ? 0.0f : mn;
+      const float e0 = exp2_(M - ms), e1 = exp2_(y[s].x - ms);
+      o = o * e0 + x[s] * e1;
+      l = l * e0 + y[s].y * e1;
+      M = mn;
+    }
   }
   const float inv = seen(a, t.s, i) > 0 ? 1.0f / l : 0.0f;
   uint16_t* out = (uint16_t*)a.o + (long long)(t.s.q0 + i) * a.ot + (hk * a.G + (R - i * a.G)) * a.oh;
-#pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int x = (tid + f * kPromptThreads) / 64;  // (32-wide block, run of 8)
-    const int d = (x / 4) * 32 + (x % 4) * 8 + 4 * ((tid & 63) >> 5);
-    *(u32x2*)(out + d) = u32x2{T::pack(o[f][0] * inv, o[f][1] * inv), T::pack(o[f][2] * inv, o[f][3] * inv)};
-  }
+  *(u32x2*)(out + d * 32 + (tid >> 6) * 8 + 4 * (lane >> 5)) =
+      u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
 }
 
 template <typename T, int HD, bool Q8, bool PAGED>
@@ -705,10 +846,9 @@ hipError_t prompt_go(const PromptArgs& a, hipStream_t st) {
                                                      (int)lds);
   if (attr != hipSuccess) return attr;
   hipLaunchKernelGGL(kern, dim3(grid_of(a.HKV, a.units)), dim3(kPromptThreads), lds, st, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.target == 0) return e;
-  hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(a.tiles * a.HKV * (kPromptRows / 32))),
-                     dim3(kPromptThreads), 0, st, a);
+  if (a.target > 0 && a.join_apart)
+    hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(a.tiles * a.HKV * (kPromptRows / 32) * (HD / 32))),
+                       dim3(kPromptThreads), 0, st, a);
   return hipGetLastError();
 }
 
