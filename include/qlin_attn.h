@@ -59,8 +59,7 @@ typedef struct qlin_rope {
   int64_t qo_token, qo_head;
   void* k_out;                 /* rotated keys, may be k itself; NULL: the cache only */
   int64_t ko_token, ko_head;
-  const qlin_paged_kv* cache;  /* NULL: no cache */
-  const void* slots;           /* [T] places in the cache: page * page size + token */
+  const void* slots;           /* [T] places in the cache: page * page size + token; NULL: no cache */
   int slots_64;                /* 1: int64, 0: int32 */
   const void* pos;             /* [axes][T] positions */
   int64_t pos_axis, pos_token;
@@ -83,8 +82,9 @@ typedef struct qlin_rope {
 /* Per head: y = x * rsqrt(mean(x^2) + eps) * (w + 1 or w) for queries and keys, then the
  * pairs (y[i], y[i + rot/2]) turned by pos[axis(i)][t] * freqs[i] (the angle in 64 bits),
  * rounded once to the output's type; keys and values to the cache's slots, as 16 bits or as
- * int8 codes round_half_away(y / s) with s = max(amax / 127, 1e-8) of the token's head. */
-int qlin_qk_norm_rope(const qlin_rope* args, void* stream);
+ * int8 codes round_half_away(y / s) with s = max(amax / 127, 1e-8) of the token's head.
+ * cache NULL: keys go to k_out alone. */
+int qlin_qk_norm_rope(const qlin_rope* args, const qlin_paged_kv* cache, void* stream);
 
 /* Attention of packed prompts: sequence b's queries are rows cu_q[b] .. cu_q[b+1] - 1 of
  * q [T][q_heads][hd], its keys rows cu_k[b] .. of k, v [Tk][kv_heads][hd].

@@ -150,7 +150,7 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   char* part;
   size_t avail;
   QA_TRY(workspace_parts(fn, ws, ws_bytes, &part, &avail));
-  long long target = 1024;
+  long long target = hd == 256 ? 448 : hd == 128 ? 512 : 640;
   if (const char* e = getenv("QLIN_PROMPT_UNITS")) {  // for tuning runs
     if (atoi(e) >= 0) target = atoi(e);
   }
@@ -174,7 +174,7 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
 
 extern "C" {
 
-int qlin_qk_norm_rope(const qlin_rope* r, void* stream) {
+int qlin_qk_norm_rope(const qlin_rope* r, const qlin_paged_kv* cache, void* stream) {
   const char* fn = "qlin_qk_norm_rope";
   set_error(QLIN_OK, "");
   if (!r) return fail(QLIN_ERR_INVALID, "%s: null arguments", fn);
@@ -199,29 +199,29 @@ int qlin_qk_norm_rope(const qlin_rope* r, void* stream) {
   QA_TRY(check_tensor(fn, "k", r->k, 2, r->hd, r->T, r->k_token, r->kv_heads, r->k_head, false));
   QA_TRY(check_tensor(fn, "q_out", r->q_out, 2, r->hd, r->T, r->qo_token, r->q_heads, r->qo_head, true));
   if (r->k_out) QA_TRY(check_tensor(fn, "k_out", r->k_out, 2, r->hd, r->T, r->ko_token, r->kv_heads, r->ko_head, true));
-  if (!r->k_out && !r->cache) return fail(QLIN_ERR_INVALID, "%s: neither k_out nor a cache for the keys", fn);
+  if (!r->k_out && !cache) return fail(QLIN_ERR_INVALID, "%s: neither k_out nor a cache for the keys", fn);
   if (r->rot > 0 && (!r->pos || !r->freqs)) return fail(QLIN_ERR_INVALID, "%s: null positions or frequencies", fn);
   if (!aligned(r->pos, r->pos_64 ? 8 : 4) || !aligned(r->freqs, r->freqs_64 ? 8 : 4))
     return fail(QLIN_ERR_UNSUPPORTED, "%s: positions and frequencies must be aligned to their size", fn);
   if (r->q_w || r->k_w) {
     if (r->w_dtype != QLIN_BF16 && r->w_dtype != QLIN_F16 && r->w_dtype != QLIN_F32)
       return fail(QLIN_ERR_UNSUPPORTED, "%s: norm weight dtype %d", fn, r->w_dtype);
-    if (!aligned(r->q_w, 4) || !aligned(r->k_w, 4))
-      return fail(QLIN_ERR_UNSUPPORTED, "%s: norm weights must be 4-byte aligned", fn);
+    if (!aligned(r->q_w, 16) || !aligned(r->k_w, 16))
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: norm weights must be 16-byte aligned", fn);
   }
   RopeArgs a = {};
-  if (r->cache) {
+  if (cache) {
     if (!r->v || !r->slots) return fail(QLIN_ERR_INVALID, "%s: a cache needs values and slots", fn);
     if (!aligned(r->slots, r->slots_64 ? 8 : 4))
       return fail(QLIN_ERR_UNSUPPORTED, "%s: slots must be aligned to their size", fn);
     QA_TRY(check_tensor(fn, "v", r->v, 2, r->hd, r->T, r->v_token, r->kv_heads, r->v_head, false));
-    QA_TRY(check_cache(fn, r->cache, r->kv_heads, r->hd, r->dtype, true, a.kc, a.vc));
-    a.page_shift = shift_of(r->cache->page);
-    a.nslots = (long long)r->cache->num_pages * r->cache->page;
+    QA_TRY(check_cache(fn, cache, r->kv_heads, r->hd, r->dtype, true, a.kc, a.vc));
+    a.page_shift = shift_of(cache->page);
+    a.nslots = (long long)cache->num_pages * cache->page;
   }
   a.q = r->q, a.qt = r->q_token, a.qh = r->q_head;
   a.k = r->k, a.kt = r->k_token, a.kh = r->k_head;
-  a.v = r->cache ? r->v : nullptr, a.vt = r->v_token, a.vh = r->v_head;
+  a.v = cache ? r->v : nullptr, a.vt = r->v_token, a.vh = r->v_head;
   a.qo = r->q_out, a.qot = r->qo_token, a.qoh = r->qo_head;
   a.ko = r->k_out, a.kot = r->ko_token, a.koh = r->ko_head;
   a.slots = r->slots, a.slots64 = r->slots_64;
@@ -319,16 +319,18 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   a.c = scale * 1.44269504088896340736f;
   const long long hg = (long long)kv_heads * a.gb;
   const long long blocks = ((long long)max_pages * cache->page + kDecodeBlock - 1) / kDecodeBlock;
-  long long total = 512;
+  const long long bound = std::max(1LL, B * ((blocks + kDecodeChunk - 1) / kDecodeChunk));
+  long long few = 256, total = 1536;
   if (const char* e = getenv("QLIN_DECODE_UNITS")) {  // for tuning runs
-    if (atoi(e) > 0) total = atoi(e);
+    if (atoi(e) > 0) few = total = atoi(e);
   }
-  long long target = std::min(std::max(1LL, total / hg), std::max(1LL, B * ((blocks + kDecodeChunk - 1) / kDecodeChunk)));
+  long long target = std::min(std::max(1LL, total / hg), bound);
   const long long slot = (long long)decode_slot_floats(std::min(16, a.G), hd) * 4;
   // without room for the parts (very many sequences) every sequence is one unit
   if ((target + B + 2) * hg * slot > (long long)avail || B * hg * kDecodeCounters * 4 > (long long)counter_bytes())
     target = 0;
   a.target = (int)target;
+  a.few = (int)std::min(std::max(1LL, few / hg), std::max(1LL, target));
   a.units = (int)(target + B + (target ? 2 : 0));  // (two for what the device's estimate rounds)
   a.part = (float*)part;
   a.cnt = (unsigned*)workspace;

@@ -18,8 +18,9 @@
 //   * int8: codes become 16-bit whole numbers (exact); a key's scale multiplies its scores in 32
 //     bits, a value's scale its probability.
 // The running maximum is a column's, hence a lane's own.  P is rounded to 16 bits for its
-// product (half a step of 2^-8 or 2^-11 of each term; the sum of P is of the unrounded); with
-// int8 values P times scale goes as bf16, whose range a small scale cannot leave.
+// product (half a step of 2^-8 or 2^-11 of each term; the sum of P is of the unrounded; where one
+// key has all the weight its P is 1 and exact); with int8 values P times scale goes as the sum of
+// two bf16 numbers, which neither a small scale nor one heavy key can take precision from.
 //
 // Waves join through LDS, units of a sequence through memory: the last of 16 units to arrive
 // adds their parts in unit order, the last of those groups adds the groups', so that the result
@@ -53,7 +54,13 @@ __device__ __forceinline__ bool find_unit(const DecodeArgs& a, int u, Unit& r) {
     float total = 0.0f;  // (rounded up below; the same for all workgroups)
     for (int b0 = 0; b0 < a.B; b0 += 64) total += (float)blocks_of(b0 ? mine(b0) : first);
     total = lane_value(wave_scan(total), 63);
-    chunk = max((int)fminf(ceilf(total / (float)a.target), 1e8f), 1);
+    // one workgroup a CU as long as that makes units of at most kDecodeLong blocks; longer work
+    // goes to more of them, which come out more even and keep more loads in flight (8 sequences
+    // of up to 8192 keys, 256 / 512 / 1024 units: 32 / 37 / 35 us; 64 of up to 16384, 256 / 768 /
+    // 1536: 250 / 189 / 183)
+    const float few = ceilf(total / (float)a.few);
+    const float most = ceilf(total / (float)a.target);
+    chunk = max((int)fminf(few <= (float)kDecodeLong ? few : fmaxf((float)kDecodeLong, most), 1e8f), 1);
     chunk = (chunk + kDecodeChunk - 1) / kDecodeChunk * kDecodeChunk;
   }
   int base = 0;
@@ -93,6 +100,10 @@ __device__ __forceinline__ float group_sum(float v) {
   return x + y;
 }
 
+// Dwords of codes that the compiler must not take apart before they are used (it would carry
+// single bytes, a register each, around the loop).
+__device__ __forceinline__ void opaque(uint32_t& a, uint32_t& b) { asm volatile("" : "+v"(a), "+v"(b)); }
+
 // Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
 template <typename T>
 __device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
@@ -107,7 +118,7 @@ __device__ __forceinline__ unsigned part_ml(int rows) {
 }
 
 template <typename T, int HD, bool Q8>
-__global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a) {
+__global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void decode_kernel(const DecodeArgs a) {
   constexpr int STEPS = HD / 32;                 // score MFMAs of 16 keys
   constexpr int VW = HD >= 128 && !Q8 ? 8 : HD / 16;  // adjacent value columns of a lane
   constexpr int VC = HD / 16 / VW;               // runs of them, 16 VW columns apart
@@ -154,63 +165,94 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a)
   const int len = U.len;
   const int nblk = blocks_of(len);
   const int blk1 = (int)min((long long)nblk, (U.s + 1LL) * U.chunk);
-  const int* table = a.kv.table + U.b * a.kv.table_stride;
-  const long long pmask = (1LL << a.kv.page_shift) - 1;
+  // (constant address space: page numbers come by scalar loads)
+  const auto table = (const __attribute__((address_space(4))) int*)(a.kv.table + U.b * a.kv.table_stride);
+  const uint32_t pmask = (1u << a.kv.page_shift) - 1u;
   constexpr int ES = Q8 ? 1 : 2;
+  const uint32_t kst = (uint32_t)a.kv.k.st * ES, vst = (uint32_t)a.kv.v.st * ES;
 
-  for (int blk = U.s * U.chunk + wave; blk < blk1; blk += kWaves) {
-    const int key0 = blk * kDecodeBlock;
-    // the two halves of 16 keys lie in one page each; keys behind the last are the last again
-    const uint8_t *kp[2], *vp[2];
-    const float *ksp[2], *vsp[2];
-    int top[2];
+  // A block's halves of 16 keys lie in one page each; keys behind the last are the last again.
+  constexpr int VB = VW * ES;  // bytes of a run
+  typedef std::conditional_t<VB == 16, u32x4, std::conditional_t<VB == 8, u32x2, uint32_t>> VReg;
+  u32x4 kr[2][KL];
+  VReg vr[8][VC];
+  float sc = 0.0f;
+  auto half_of = [&](int blk, int h) { return min(blk * kDecodeBlock + 16 * h, (len - 1) & ~15); };
+  auto pages = [&](int blk, int (&pid)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pid[h] = table[half_of(min(blk, nblk - 1), h) >> a.kv.page_shift];
+  };
+  auto valid = [&](int pid) {
+    if ((unsigned)pid < (unsigned)a.kv.num_pages) return pid;
+    bad = true;
+    return 0;
+  };
+  auto base = [&](const PagedTensor& x, int hs, int pid) {
+    return (const uint8_t*)x.p + ((uint64_t)(uint32_t)pid * (uint64_t)x.sp + ((uint32_t)hs & pmask) * (uint64_t)x.st +
+                                  (uint64_t)hk * x.sh) * ES;
+  };
+  auto load_k = [&](int blk, const int (&pid)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int hs = min(key0 + 16 * h, (len - 1) & ~15);
-      top[h] = min(15, len - 1 - hs);
-      int pid = table[hs >> a.kv.page_shift];
-      if ((unsigned)pid >= (unsigned)a.kv.num_pages) {
-        bad = true;
-        pid = 0;
-      }
-      const long long off = hs & pmask;
-      kp[h] = (const uint8_t*)a.kv.k.p + (pid * a.kv.k.sp + off * a.kv.k.st + hk * a.kv.k.sh) * ES;
-      vp[h] = (const uint8_t*)a.kv.v.p + (pid * a.kv.v.sp + off * a.kv.v.st + hk * a.kv.v.sh) * ES;
-      if constexpr (Q8) {
-        ksp[h] = a.kv.k.s + pid * a.kv.k.ssp + off * a.kv.k.sst + hk * a.kv.k.ssh;
-        vsp[h] = a.kv.v.s + pid * a.kv.v.ssp + off * a.kv.v.sst + hk * a.kv.v.ssh;
-      }
+      const int hs = half_of(blk, h);
+      const uint8_t* p = base(a.kv.k, hs, valid(pid[h]));
+      const uint32_t off = (uint32_t)min(j, len - 1 - hs) * kst + (uint32_t)g * 16u;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) kr[h][i] = ld_global_nt<u32x4>(p + off + i * 64);
     }
-    u32x4 kr[2][KL];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < KL; ++i)
-        kr[h][i] = ld_global_nt<u32x4>(kp[h] + min(j, top[h]) * a.kv.k.st * ES + i * 64 + g * 16);
-    // value rows: slot s of lane group g is key 4g + s (s < 4) or 16 + 4g + s - 4
-    constexpr int VB = VW * ES;  // bytes of a run
-    typedef std::conditional_t<VB == 16, u32x4, std::conditional_t<VB == 8, u32x2, uint32_t>> VReg;
-    VReg vr[8][VC];
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-#pragma unroll
-      for (int c = 0; c < VC; ++c)
-        vr[s][c] = ld_global_nt<VReg>(vp[s / 4] + min(4 * g + s % 4, top[s / 4]) * a.kv.v.st * ES + c * 16 * VB +
-                                      j * VB);
-    float ks[8], vs[8];
     if constexpr (Q8) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const int r = min(4 * g + s % 4, top[s / 4]);
-        ks[s] = ksp[s / 4][r * a.kv.k.sst];
-        vs[s] = vsp[s / 4][r * a.kv.v.sst];
-      }
+      // one scale a lane: the 32 keys', then the 32 values'
+      const int h = (lane >> 4) & 1, hs = half_of(blk, h);
+      const int r = min(j, len - 1 - hs), pc = h ? valid(pid[1]) : valid(pid[0]);
+      const PagedTensor& x = lane < 32 ? a.kv.k : a.kv.v;
+      const float* p = x.s + ((uint64_t)(uint32_t)pc * x.ssp + (uint64_t)((uint32_t)(hs & pmask) + r) * x.sst + (uint64_t)hk * x.ssh);
+      sc = ld_global<float>(p);
     }
-
-    float t[8];
+  };
+  // value rows: slot s of lane group g is key 4g + s (s < 4) or 16 + 4g + s - 4
+  auto load_v = [&](int blk, const int (&pid)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      f32x4 S = {0, 0, 0, 0};
+      const int hs = half_of(blk, h);
+      const uint8_t* p = base(a.kv.v, hs, valid(pid[h]));
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t off = (uint32_t)min(4 * g + s, len - 1 - hs) * vst + (uint32_t)j * VB;
+#pragma unroll
+        for (int c = 0; c < VC; ++c) vr[4 * h + s][c] = ld_global_nt<VReg>(p + off + c * 16 * VB);
+      }
+    }
+  };
+
+  // The next block's keys are loaded as soon as this one's are used, its values likewise, so that
+  // a wave's loads are in flight while it computes.
+  int blk = U.s * U.chunk + wave;
+  int pid[2], pin[2];
+  if (blk < blk1) {
+    pages(blk, pid);
+    load_k(blk, pid);
+    load_v(blk, pid);
+    pages(blk + kWaves, pin);
+  }
+  float* lsc = lds + wave * 64;
+  for (; blk < blk1; blk += kWaves) {
+    const bool more = blk + kWaves < blk1;
+    f32x4 S[2];
+    f32x4 ks[2], vs[2];
+    if constexpr (Q8) {
+      // (a wave's LDS instructions take effect in order)
+      lsc[lane] = sc;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ks[h] = *(const f32x4*)(lsc + 16 * h + 4 * g);
+        vs[h] = *(const f32x4*)(lsc + 32 + 16 * h + 4 * g);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      S[h] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
         u32x4 kop;
@@ -219,20 +261,28 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a)
           const uint32_t w0 = s % 2 ? r.z : r.x, w1 = s % 2 ? r.w : r.y;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t w = e < 2 ? w0 : w1;
+            uint32_t w = e < 2 ? w0 : w1;
             const int c = 2 * (e % 2);
+            asm volatile("" : "+v"(w));
             kop[e] = T::pack_exact((float)(int8_t)(w >> (8 * c)), (float)(int8_t)(w >> (8 * c + 8)));
           }
         } else {
           kop = kr[h][s];
         }
-        S = T::mma16(kop, qv[s], S);
+        if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
+        S[h] = T::mma16(kop, qv[s], S[h]);
       }
+    }
+    if (more) load_k(blk + kWaves, pin);
+    float t[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = Q8 ? S[i] * ks[4 * h + i] : S[i];
-        t[4 * h + i] = key0 + 16 * h + 4 * g + i < len ? x * a.c : kNegInf;
-      }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[4 * h + i] = (Q8 ? S[h][i] * ks[h][i] : S[h][i]) * a.c;
+    if (blk * kDecodeBlock + kDecodeBlock > len) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (blk * kDecodeBlock + 16 * (s / 4) + 4 * g + s % 4 >= len) t[s] = kNegInf;
     }
     float mx = t[0];
 #pragma unroll
@@ -248,10 +298,23 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a)
       ps += p[s];
     }
     l = l * al + ps;
-    u32x4 pop;
+    u32x4 pop[Q8 ? 2 : 1];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      pop[e] = Q8 ? TV::pack(p[2 * e] * vs[2 * e], p[2 * e + 1] * vs[2 * e + 1]) : TV::pack(p[2 * e], p[2 * e + 1]);
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (Q8) {
+        const float p0 = p[2 * e] * vs[e / 2][2 * (e % 2)], p1 = p[2 * e + 1] * vs[e / 2][2 * (e % 2) + 1];
+        const uint32_t w = TV::pack(p0, p1);
+        pop[0][e] = w;
+        pop[1][e] = TV::pack(p0 - bitcast<float>(w << 16), p1 - bitcast<float>(w & 0xFFFF0000u));
+      } else {
+        pop[0][e] = TV::pack(p[2 * e], p[2 * e + 1]);
+      }
+    }
+    // (the rescaling is skipped while no row's maximum grows)
+    if (__any(al != 1.0f)) {
+#pragma unroll
+      for (int c = 0; c < VC * VW; ++c) O[c] *= al;
+    }
 #pragma unroll
     for (int c = 0; c < VC; ++c)
 #pragma unroll
@@ -268,15 +331,24 @@ __global__ __launch_bounds__(kThreads, 2) void decode_kernel(const DecodeArgs a)
             w0 = vr[2 * e][c][x / PER];
             w1 = vr[2 * e + 1][c][x / PER];
           }
+          if constexpr (Q8) opaque(w0, w1);
           vop[e] = Q8 ? codes2<TV>(w0, w1, x % PER) : perm(w1, w0, x % 2 ? 0x07060302u : 0x05040100u);
         }
+        // (left to itself the compiler widens every column first, and spills)
+        if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
         f32x4& o = O[c * VW + x];
-        o = TV::mma16(vop, pop, f32x4{o[0] * al, o[1] * al, o[2] * al, o[3] * al});
+#pragma unroll
+        for (int n = 0; n < (Q8 ? 2 : 1); ++n) o = TV::mma16(vop, pop[n], o);
       }
+    if (more) {
+      load_v(blk + kWaves, pin);
+      pages(blk + 2 * kWaves, pin);
+    }
   }
   if (bad) l = __builtin_nanf("");  // a page outside the cache: its sequence's output is NaN
   l = group_sum(l);
 
+  if constexpr (Q8) __syncthreads();  // (the scales' place is taken again)
   // waves join in LDS: wave w's sums at w * rows * HD, maxima and sums of P behind all of them
   float* mlw = lds + kWaves * rows * HD;
   if (j < rows) {

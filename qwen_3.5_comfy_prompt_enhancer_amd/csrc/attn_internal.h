@@ -74,7 +74,8 @@ struct DecodeArgs {
   int B, HQ, HKV, G;      // G = HQ / HKV
   int gb;                 // groups of 16 query heads of a key head
   float c;                // scale * log2(e)
-  int target;             // work units a launch aims at
+  int target;             // most work units of a (key head, group) to cut into; 0: no cut
+  int few;                // units that short work is cut into
   int units;              // units per (key head, group): the grid's bound
   float* part;            // unit partials
   unsigned* cnt;          // arrival counters, zero between calls
@@ -83,6 +84,7 @@ struct DecodeArgs {
 __host__ __device__ constexpr int decode_slot_floats(int rows, int hd) { return rows * hd + rows * 4; }
 constexpr int kDecodeBlock = 32;     // keys a wave takes at a time
 constexpr int kDecodeChunk = 4;      // blocks of a unit come in multiples of this (one per wave)
+constexpr int kDecodeLong = 32;     // blocks of a unit up to which fewer units are better
 constexpr int kDecodeGroup = 16;     // units joined at a time
 constexpr int kDecodeCounters = 32;  // counters of a (sequence, key head, group)
 hipError_t launch_decode(const DecodeArgs& a, int dt, int hd, hipStream_t st);

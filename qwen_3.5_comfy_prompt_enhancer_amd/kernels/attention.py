@@ -30,6 +30,7 @@ stream of their tensors' device and can be captured (see `qlin.capture`).
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -40,48 +41,28 @@ __all__ = ["qk_norm_rope", "attn_prompt", "attn_prompt_paged", "attn_decode"]
 QLIN_I8 = 4
 
 _P, _I, _L, _S, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
+_B = ctypes.c_char_p  # a struct of the ABI, packed (a third of the time of a ctypes.Structure)
 
+# include/qlin_attn.h qlin_paged_kv: four times a pointer and three strides; dtype, pages, page size
+_PAGED_KV = struct.Struct("@" + 4 * "P3q" + "3i0q")
+# qlin_rope: q, k, v, q_out, k_out with two strides; slots; positions; frequencies; norm;
+# sizes
+_ROPE = struct.Struct("@" + 5 * "P2q" + "Pi" + "P2qi" + "Pi" + "PP2if" + "6i" + "3i" + "2i0q")
 
-class _PagedKV(ctypes.Structure):
-    """include/qlin_attn.h qlin_paged_kv."""
-    _fields_ = [
-        ("k", _P), ("k_page", _L), ("k_token", _L), ("k_head", _L),
-        ("v", _P), ("v_page", _L), ("v_token", _L), ("v_head", _L),
-        ("k_s", _P), ("ks_page", _L), ("ks_token", _L), ("ks_head", _L),
-        ("v_s", _P), ("vs_page", _L), ("vs_token", _L), ("vs_head", _L),
-        ("dtype", _I), ("num_pages", _I), ("page", _I),
-    ]
-
-
-class _Rope(ctypes.Structure):
-    """include/qlin_attn.h qlin_rope."""
-    _fields_ = [
-        ("q", _P), ("q_token", _L), ("q_head", _L),
-        ("k", _P), ("k_token", _L), ("k_head", _L),
-        ("v", _P), ("v_token", _L), ("v_head", _L),
-        ("q_out", _P), ("qo_token", _L), ("qo_head", _L),
-        ("k_out", _P), ("ko_token", _L), ("ko_head", _L),
-        ("cache", ctypes.POINTER(_PagedKV)), ("slots", _P), ("slots_64", _I),
-        ("pos", _P), ("pos_axis", _L), ("pos_token", _L), ("pos_64", _I),
-        ("freqs", _P), ("freqs_64", _I),
-        ("q_w", _P), ("k_w", _P), ("w_dtype", _I), ("one_plus", _I), ("eps", _F),
-        ("T", _I), ("q_heads", _I), ("kv_heads", _I), ("hd", _I), ("rot", _I), ("axes", _I),
-        ("sections", _I * 3), ("interleaved", _I), ("dtype", _I),
-    ]
-
-
-_KV = ctypes.POINTER(_PagedKV)
 _SIGS = {
-    "qlin_qk_norm_rope": [ctypes.POINTER(_Rope), _P],
+    "qlin_qk_norm_rope": [_B, _B, _P],
     "qlin_attn_prompt": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _I, _F, _I,
                          _P, _S, _P],
-    "qlin_attn_prompt_paged": [_P, _L, _L, _KV, _P, _L, _I, _P, _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _F, _I,
+    "qlin_attn_prompt_paged": [_P, _L, _L, _B, _P, _L, _I, _P, _P, _P, _L, _L, _I, _I, _I, _I, _I, _I, _F, _I,
                                _P, _S, _P],
-    "qlin_attn_decode": [_P, _L, _L, _KV, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I, _F, _P, _S, _P],
+    "qlin_attn_decode": [_P, _L, _L, _B, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I, _F, _P, _S, _P],
 }
 EXPORTS = tuple(_SIGS)
 
+_DT = {torch.bfloat16: C.QLIN_BF16, torch.float16: C.QLIN_F16}
+_WDT = {**_DT, torch.float32: C.QLIN_F32}
 _fns: dict = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _call(name, device, *args):
@@ -92,7 +73,7 @@ def _call(name, device, *args):
         f.restype = ctypes.c_int
         f.argtypes = _SIGS[name]
         _fns[name] = f
-    if torch.cuda.current_device() == device:
+    if _current_device() == device:
         status = f(*args)
     else:
         with torch.cuda.device(device):
@@ -101,60 +82,84 @@ def _call(name, device, *args):
         C.check(status, name)
 
 
-def _rows(name, t, heads, hd, dtype):
-    """A [rows, heads, hd] tensor of 16-bit values with a contiguous last axis."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd:
-        raise ValueError(f"{name} must be [rows, {heads}, {hd}], not {list(t.shape)}")
+def _strides(name, t, rows, heads, hd, dtype):
+    """Row and head strides of a [rows, heads, hd] tensor of 16-bit values whose last axis is
+    contiguous."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hd:
+        raise ValueError(f"{name} must be [rows, {heads}, {hd}], not {list(shape)}")
+    if shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}")
-    if t.stride(2) != 1:
+    st = t.stride()
+    if st[2] != 1:
         raise ValueError(f"the last axis of {name} must be contiguous")
+    return st[0], st[1]
 
 
 def _queries(q):
-    if q.dim() != 3:
+    """Rows, heads, head size, type code and strides of the queries."""
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError("q must be [rows, heads, hd]")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    dt = _DT.get(q.dtype)
+    if dt is None:
         raise ValueError("q must be bfloat16 or float16")
-    if q.stride(2) != 1:
+    st = q.stride()
+    if st[2] != 1:
         raise ValueError("the last axis of q must be contiguous")
-    return q.shape
+    return *shape, dt, st[0], st[1]
 
 
-def _ints(name, t, shape=None, dtypes=(torch.int32,)):
+def _vector(name, t, n, dtypes=(torch.int32,)):
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"the last axis of {name} must be contiguous")
+    shape = t.shape
+    if len(shape) != 1 or shape[0] != n:
+        raise ValueError(f"{name} must be [{n}], not {list(shape)}")
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _table(table, kv_len, B):
+    """Stride and width of a page table [B, pages]; checks the lengths too."""
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != B:
+        raise ValueError(f"table must be [{B}, pages]")
+    st = table.stride()
+    if table.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
+        raise ValueError("table must be int32 with a contiguous last axis")
+    _vector("kv_len", kv_len, B)
+    return st[0], shape[1]
 
 
 def _cache(k, v, k_s, v_s, dtype, hd):
-    """The C view of a cache, and its key heads."""
-    if k.dim() != 4 or k.shape != v.shape:
+    """The packed C view of a cache, and its key heads."""
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("k_cache and v_cache must both be [pages, page, kv_heads, hd]")
-    pages, page, heads, d = k.shape
-    if d != hd:
-        raise ValueError(f"the cache's head size {d} is not the queries' {hd}")
+    if shape[3] != hd:
+        raise ValueError(f"the cache's head size {shape[3]} is not the queries' {hd}")
     if k.dtype != v.dtype:
         raise ValueError("k_cache and v_cache must share a dtype")
-    if k.stride(3) != 1 or v.stride(3) != 1:
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the last axis of the cache must be contiguous")
-    if k.dtype == torch.int8:
-        if k_s is None or v_s is None:
-            raise ValueError("an int8 cache needs its scales k_s and v_s")
-        for name, s in (("k_s", k_s), ("v_s", v_s)):
-            if s.dtype != torch.float32 or s.shape != k.shape[:3]:
-                raise ValueError(f"{name} must be float32 {[pages, page, heads]}")
-        return _PagedKV(k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], k_s.data_ptr(), *k_s.stride(),
-                        v_s.data_ptr(), *v_s.stride(), QLIN_I8, pages, page), heads
-    if k.dtype != dtype:
+    if k.dtype == dtype:
+        if k_s is not None or v_s is not None:
+            raise ValueError("a 16-bit cache has no scales")
+        return _PAGED_KV.pack(k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], 0, 0, 0, 0, 0, 0,
+                              0, 0, _DT[dtype], shape[0], shape[1]), shape[2]
+    if k.dtype != torch.int8:
         raise ValueError(f"the cache must be int8 or {dtype}")
-    if k_s is not None or v_s is not None:
-        raise ValueError("a 16-bit cache has no scales")
-    return _PagedKV(k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], None, 0, 0, 0, None, 0, 0, 0,
-                    C.dtype_code(k), pages, page), heads
+    if k_s is None or v_s is None:
+        raise ValueError("an int8 cache needs its scales k_s and v_s")
+    for name, s in (("k_s", k_s), ("v_s", v_s)):
+        if s.dtype != torch.float32 or s.shape != shape[:3]:
+            raise ValueError(f"{name} must be float32 {list(shape[:3])}")
+    return _PAGED_KV.pack(k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], k_s.data_ptr(),
+                          *k_s.stride(), v_s.data_ptr(), *v_s.stride(), QLIN_I8, shape[0], shape[1]), shape[2]
 
 
 def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_cache=None, slots=None, k_s=None,
@@ -176,22 +181,21 @@ def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_ca
     the cache, stores nothing; a slot given twice holds one of the two, whole or mixed by
     head).  An int8 cache gets codes round_half_away(y / s) with `s = max(amax / 127,
     1e-8)` of each token's head in k_s / v_s.  Returns q_out."""
-    T, hq, hd = _queries(q)
-    dt = q.dtype
+    T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3:
         raise ValueError("k must be [rows, kv_heads, hd]")
-    hkv = k.shape[1]
-    _rows("k", k, hkv, hd, dt)
-    _rows("q_out", q_out, hq, hd, dt)
-    if k.shape[0] != T or q_out.shape[0] != T:
-        raise ValueError(f"q, k and q_out must have the same rows ({T})")
+    dtype, hkv = q.dtype, k.shape[1]
+    kt, kh = _strides("k", k, T, hkv, hd, dtype)
+    qot, qoh = _strides("q_out", q_out, T, hq, hd, dtype)
     if pos.dim() == 1:
         pos = pos[None]
     if pos.dim() != 2 or pos.shape[1] != T:
         raise ValueError(f"pos must be [{T}] or [axes, {T}]")
-    if pos.dtype not in (torch.int32, torch.int64):
+    pos64 = pos.dtype == torch.int64
+    if not pos64 and pos.dtype != torch.int32:
         raise ValueError("pos must be int32 or int64")
-    if freqs.dim() != 1 or freqs.dtype not in (torch.float32, torch.float64) or not freqs.is_contiguous():
+    freqs64 = freqs.dtype == torch.float64
+    if freqs.dim() != 1 or not (freqs64 or freqs.dtype == torch.float32) or not freqs.is_contiguous():
         raise ValueError("freqs must be a contiguous float32 or float64 vector")
     half, axes = freqs.shape[0], pos.shape[0]
     if sections is None:
@@ -202,43 +206,39 @@ def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_ca
         raise ValueError(f"sections must give one length for each of the {axes} axes")
     if axes > 3:
         raise ValueError("at most 3 position axes")
+    wdt = 0
     for name, w in (("q_w", q_w), ("k_w", k_w)):
-        if w is not None and (w.dim() != 1 or w.shape[0] != hd or not w.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous [{hd}]")
-    if q_w is not None and k_w is not None and q_w.dtype != k_w.dtype:
-        raise ValueError("q_w and k_w must share a dtype")
-    w = q_w if q_w is not None else k_w
-    if k_out is not None:
-        _rows("k_out", k_out, hkv, hd, dt)
-        if k_out.shape[0] != T:
-            raise ValueError(f"k_out must have {T} rows")
+        if w is not None:
+            if w.dim() != 1 or w.shape[0] != hd or not w.is_contiguous() or w.dtype not in _WDT:
+                raise ValueError(f"{name} must be a contiguous [{hd}] of bfloat16, float16 or float32")
+            if wdt and wdt != _WDT[w.dtype]:
+                raise ValueError("q_w and k_w must share a dtype")
+            wdt = _WDT[w.dtype]
+    kot = koh = vt = vh = slots64 = 0
     cache = None
+    if k_out is not None:
+        kot, koh = _strides("k_out", k_out, T, hkv, hd, dtype)
     if k_cache is not None or v_cache is not None or slots is not None:
         if k_cache is None or v_cache is None or v is None or slots is None:
             raise ValueError("a cache takes k_cache, v_cache, v and slots")
-        _rows("v", v, hkv, hd, dt)
-        _ints("slots", slots, (T,), (torch.int32, torch.int64))
-        if v.shape[0] != T:
-            raise ValueError(f"v must have {T} rows")
-        cache, ch = _cache(k_cache, v_cache, k_s, v_s, dt, hd)
+        vt, vh = _strides("v", v, T, hkv, hd, dtype)
+        _vector("slots", slots, T, (torch.int32, torch.int64))
+        slots64 = slots.dtype == torch.int64
+        cache, ch = _cache(k_cache, v_cache, k_s, v_s, dtype, hd)
         if ch != hkv:
             raise ValueError(f"the cache has {ch} key heads, k {hkv}")
     elif k_out is None:
         raise ValueError("give k_out, a cache, or both")
     C.require_cuda(q, k, v, pos, freqs, q_out, k_out, k_cache, v_cache, slots, k_s, v_s, q_w, k_w)
     dev = q.get_device()
-    args = _Rope(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-        C.ptr(v), v.stride(0) if v is not None else 0, v.stride(1) if v is not None else 0,
-        q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-        C.ptr(k_out), k_out.stride(0) if k_out is not None else 0, k_out.stride(1) if k_out is not None else 0,
-        ctypes.pointer(cache) if cache is not None else None, C.ptr(slots),
-        1 if slots is not None and slots.dtype == torch.int64 else 0,
-        pos.data_ptr(), pos.stride(0), pos.stride(1), 1 if pos.dtype == torch.int64 else 0,
-        freqs.data_ptr(), 1 if freqs.dtype == torch.float64 else 0,
-        C.ptr(q_w), C.ptr(k_w), C.dtype_code(w) if w is not None else 0, 1 if one_plus else 0, float(eps),
-        T, hq, hkv, hd, 2 * half, axes, (_I * 3)(*sections), 1 if interleaved else 0, C.dtype_code(q))
-    _call("qlin_qk_norm_rope", dev, ctypes.byref(args), C.current_stream(dev))
+    s = [*sections, 0, 0]
+    args = _ROPE.pack(
+        q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr() if v is not None else 0, vt, vh, q_out.data_ptr(), qot,
+        qoh, k_out.data_ptr() if k_out is not None else 0, kot, koh,
+        slots.data_ptr() if slots is not None else 0, slots64, pos.data_ptr(), pos.stride(0), pos.stride(1), pos64,
+        freqs.data_ptr(), freqs64, q_w.data_ptr() if q_w is not None else 0, k_w.data_ptr() if k_w is not None else 0,
+        wdt, bool(one_plus), eps, T, hq, hkv, hd, 2 * half, axes, s[0], s[1], s[2], bool(interleaved), dt)
+    _call("qlin_qk_norm_rope", dev, args, cache, C.current_stream(dev))
     return q_out
 
 
@@ -249,29 +249,28 @@ def attn_prompt(q, k, v, cu_q, out, cu_k=None, scale=None, causal=True):
     sequence sees its keys j <= i + keys - queries (the last query sees all).  scale:
     hd ** -0.5 unless given.  out [T, q_heads, hd]; a row that sees no key is zero, rows of
     no sequence stay as they were.  Returns out."""
-    T, hq, hd = _queries(q)
+    T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must both be [rows, kv_heads, hd]")
-    hkv = k.shape[1]
-    _rows("k", k, hkv, hd, q.dtype)
-    _rows("v", v, hkv, hd, q.dtype)
-    _rows("out", out, hq, hd, q.dtype)
-    if out.shape[0] != T:
-        raise ValueError(f"out must have {T} rows")
+    Tk, hkv = k.shape[0], k.shape[1]
+    kt, kh = _strides("k", k, Tk, hkv, hd, q.dtype)
+    vt, vh = _strides("v", v, Tk, hkv, hd, q.dtype)
+    ot, oh = _strides("out", out, T, hq, hd, q.dtype)
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q must be [sequences + 1]")
-    _ints("cu_q", cu_q)
+    B = cu_q.shape[0] - 1
+    _vector("cu_q", cu_q, B + 1)
     if cu_k is None:
-        if k.shape[0] != T:
+        if Tk != T:
             raise ValueError("k and v must have the queries' rows, or cu_k be given")
         cu_k = cu_q
-    _ints("cu_k", cu_k, tuple(cu_q.shape))
+    else:
+        _vector("cu_k", cu_k, B + 1)
     C.require_cuda(q, k, v, cu_q, cu_k, out)
     ws, nws, stream = C.scratch(out)
-    _call("qlin_attn_prompt", out.get_device(), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-          k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
-          out.stride(0), out.stride(1), T, k.shape[0], cu_q.shape[0] - 1, hq, hkv, hd, C.dtype_code(q),
-          hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, ws, nws, stream)
+    _call("qlin_attn_prompt", out.get_device(), q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+          cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ot, oh, T, Tk, B, hq, hkv, hd, dt,
+          hd ** -0.5 if scale is None else scale, bool(causal), ws, nws, stream)
     return out
 
 
@@ -280,25 +279,19 @@ def attn_prompt_paged(q, k_cache, v_cache, table, kv_len, cu_q, out, k_s=None, v
     first kv_len[b] tokens of pages table[b, 0], table[b, 1], ... (its chunk's own among
     them: store them first).  table: int32 [B, pages a sequence], kv_len: int32 [B], cu_q:
     int32 [B + 1].  Returns out."""
-    T, hq, hd = _queries(q)
+    T, hq, hd, dt, qt, qh = _queries(q)
     cache, hkv = _cache(k_cache, v_cache, k_s, v_s, q.dtype, hd)
-    _rows("out", out, hq, hd, q.dtype)
-    if out.shape[0] != T:
-        raise ValueError(f"out must have {T} rows")
+    ot, oh = _strides("out", out, T, hq, hd, q.dtype)
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q must be [sequences + 1]")
     B = cu_q.shape[0] - 1
-    _ints("cu_q", cu_q)
-    if table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"table must be [{B}, pages]")
-    _ints("table", table)
-    _ints("kv_len", kv_len, (B,))
+    _vector("cu_q", cu_q, B + 1)
+    tb, pages = _table(table, kv_len, B)
     C.require_cuda(q, k_cache, v_cache, table, kv_len, cu_q, out, k_s, v_s)
     ws, nws, stream = C.scratch(out)
-    _call("qlin_attn_prompt_paged", out.get_device(), q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(cache),
-          table.data_ptr(), table.stride(0), table.shape[1], kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
-          out.stride(0), out.stride(1), T, B, hq, hkv, hd, C.dtype_code(q),
-          hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, ws, nws, stream)
+    _call("qlin_attn_prompt_paged", out.get_device(), q.data_ptr(), qt, qh, cache, table.data_ptr(), tb, pages,
+          kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(), ot, oh, T, B, hq, hkv, hd, dt,
+          hd ** -0.5 if scale is None else scale, bool(causal), ws, nws, stream)
     return out
 
 
@@ -307,19 +300,13 @@ def attn_decode(q, k_cache, v_cache, table, kv_len, out, k_s=None, v_s=None, sca
     keys are the first kv_len[b] tokens (the new one among them) of pages table[b, 0],
     table[b, 1], ...  table: int32 [B, pages a sequence], kv_len: int32 [B].  A sequence
     without keys gives zeros.  scale: hd ** -0.5 unless given.  Returns out."""
-    B, hq, hd = _queries(q)
+    B, hq, hd, dt, qb, qh = _queries(q)
     cache, hkv = _cache(k_cache, v_cache, k_s, v_s, q.dtype, hd)
-    _rows("out", out, hq, hd, q.dtype)
-    if out.shape[0] != B:
-        raise ValueError(f"out must have {B} rows")
-    if table.dim() != 2 or table.shape[0] != B:
-        raise ValueError(f"table must be [{B}, pages]")
-    _ints("table", table)
-    _ints("kv_len", kv_len, (B,))
+    ob, oh = _strides("out", out, B, hq, hd, q.dtype)
+    tb, pages = _table(table, kv_len, B)
     C.require_cuda(q, k_cache, v_cache, table, kv_len, out, k_s, v_s)
     ws, nws, stream = C.scratch(out)
-    _call("qlin_attn_decode", out.get_device(), q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(cache),
-          table.data_ptr(), table.stride(0), table.shape[1], kv_len.data_ptr(), out.data_ptr(), out.stride(0),
-          out.stride(1), B, hq, hkv, hd, C.dtype_code(q), hd ** -0.5 if scale is None else float(scale), ws, nws,
-          stream)
+    _call("qlin_attn_decode", out.get_device(), q.data_ptr(), qb, qh, cache, table.data_ptr(), tb, pages,
+          kv_len.data_ptr(), out.data_ptr(), ob, oh, B, hq, hkv, hd, dt, hd ** -0.5 if scale is None else scale, ws,
+          nws, stream)
     return out

@@ -22,13 +22,51 @@ def A():
     return attention
 
 
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+
+
+class PagedKV(ctypes.Structure):
+    """include/qlin_attn.h qlin_paged_kv."""
+    _fields_ = [(f, t) for x in ("k", "v", "k_s", "v_s")
+                for f, t in ((x, _P), (x.replace("_", "") + "_page", _L), (x.replace("_", "") + "_token", _L),
+                             (x.replace("_", "") + "_head", _L))] + [("dtype", _I), ("num_pages", _I), ("page", _I)]
+
+
+class Rope(ctypes.Structure):
+    """include/qlin_attn.h qlin_rope."""
+    _fields_ = [
+        ("q", _P), ("q_token", _L), ("q_head", _L), ("k", _P), ("k_token", _L), ("k_head", _L), ("v", _P),
+        ("v_token", _L), ("v_head", _L), ("q_out", _P), ("qo_token", _L), ("qo_head", _L), ("k_out", _P),
+        ("ko_token", _L), ("ko_head", _L), ("slots", _P), ("slots_64", _I), ("pos", _P), ("pos_axis", _L),
+        ("pos_token", _L), ("pos_64", _I), ("freqs", _P), ("freqs_64", _I), ("q_w", _P), ("k_w", _P), ("w_dtype", _I),
+        ("one_plus", _I), ("eps", _F), ("T", _I), ("q_heads", _I), ("kv_heads", _I), ("hd", _I), ("rot", _I),
+        ("axes", _I), ("sections", _I * 3), ("interleaved", _I), ("dtype", _I),
+    ]
+
+
 def _lib(A):
+    """The library with this file's own view of the ABI (structs by address)."""
     from qwen35_amd.kernels import qlin
-    L = qlin.lib()
+    L = ctypes.CDLL(str(qlin.LIB_PATH))
+    L.qlin_last_error.restype = ctypes.c_char_p
     for n, sig in A._SIGS.items():
-        getattr(L, n).argtypes = sig
+        getattr(L, n).argtypes = [_P if t is ctypes.c_char_p else t for t in sig]
         getattr(L, n).restype = ctypes.c_int
     return qlin, L
+
+
+def test_packed_structs_are_the_headers(A):
+    """The packing formats give the fields the places that a C compiler does."""
+    assert A._PAGED_KV.size == ctypes.sizeof(PagedKV) and A._ROPE.size == ctypes.sizeof(Rope)
+    kv = PagedKV.from_buffer_copy(A._PAGED_KV.pack(*range(1, 20)))
+    assert [getattr(kv, f) for f, _ in PagedKV._fields_] == list(range(1, 20))
+    vals = list(range(1, 40))
+    r = Rope.from_buffer_copy(A._ROPE.pack(*vals))
+    got = []
+    for f, _ in Rope._fields_:
+        x = getattr(r, f)
+        got += list(x) if f == "sections" else [x]
+    assert got[:len(vals)] == vals and len(got) == len(vals)
 
 
 def test_header_and_library_agree(A):
@@ -43,7 +81,7 @@ def _kv(A, **kw):
     d = dict(k=FAKE, k_page=64 * 256, k_token=256, k_head=64, v=FAKE, v_page=64 * 256, v_token=256, v_head=64,
              dtype=2, num_pages=8, page=64)
     d.update(kw)
-    return A._PagedKV(**d)
+    return PagedKV(**d)
 
 
 def _kv8(A, **kw):
@@ -133,9 +171,8 @@ def _rope(A, cache=None, **kw):
              kv_heads=4, hd=64, rot=64, axes=1, sections=(32, 0, 0), interleaved=0, dtype=2)
     d.update(kw)
     d["sections"] = (ctypes.c_int * 3)(*d["sections"])
-    if cache is not None:
-        d["cache"] = ctypes.pointer(cache)
-    return L.qlin_qk_norm_rope(ctypes.byref(A._Rope(**d)), None), L.qlin_last_error().decode()
+    return (L.qlin_qk_norm_rope(ctypes.byref(Rope(**d)), ctypes.byref(cache) if cache is not None else None, None),
+            L.qlin_last_error().decode())
 
 
 @pytest.mark.parametrize("bad,text", [
