@@ -15,8 +15,9 @@
  * read on the device:
  *   - a slot below 0 or past the cache stores nothing (a padded row);
  *   - kv_len below 0 counts as 0, above what the table's row holds as that;
- *   - a page outside 0 .. num_pages - 1 in front of a sequence's end makes that sequence's
- *     outputs NaN (no memory outside the cache is read);
+ *   - a page outside 0 .. num_pages - 1 in front of a sequence's end makes NaN of every
+ *     output that sees a key of it, and maybe of others of that sequence (no memory outside
+ *     the cache is read);
  *   - row bounds (cu) are clamped to the rows there are.
  */
 #ifndef QLIN_ATTN_H
@@ -91,7 +92,8 @@ int qlin_qk_norm_rope(const qlin_rope* args, const qlin_paged_kv* cache, void* s
  * out = softmax(scale q k^T) v over all keys of the sequence, or where `causal` over the
  * keys j <= i + keys - queries for its query i.  Query head h uses key head
  * h / (q_heads / kv_heads).  A row that sees no key is zero; masked keys have no part in a
- * row whatever they hold.  Rows of no sequence are left as they were. */
+ * row whatever they hold.  Rows of no sequence are left as they were.  out must not overlap
+ * q, k or v. */
 int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head,
                      const void* k, int64_t k_token, int64_t k_head,
                      const void* v, int64_t v_token, int64_t v_head,

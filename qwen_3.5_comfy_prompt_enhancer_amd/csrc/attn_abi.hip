@@ -71,6 +71,11 @@ int check_heads(const char* fn, int hq, int hkv, int hd, int dtype) {
   return QLIN_OK;
 }
 
+int check_apart(const char* fn, const void* q, const void* out) {
+  if (q == out) return fail(QLIN_ERR_INVALID, "%s: out must not be q (queries are read while others' outputs are written)", fn);
+  return QLIN_OK;
+}
+
 int check_scale(const char* fn, float scale) {
   if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(QLIN_ERR_INVALID, "%s: scale must be positive", fn);
   return QLIN_OK;
@@ -251,6 +256,7 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void*
     return fail(QLIN_ERR_UNSUPPORTED, "%s: row bounds must be 4-byte aligned", fn);
   QA_TRY(check_tensor(fn, "q", q, 2, hd, T, q_token, q_heads, q_head, false));
   QA_TRY(check_tensor(fn, "out", out, 2, hd, T, o_token, q_heads, o_head, true));
+  QA_TRY(check_apart(fn, q, out));
   if (Tk > 0) {
     QA_TRY(check_tensor(fn, "k", k, 2, hd, Tk, k_token, kv_heads, k_head, false));
     QA_TRY(check_tensor(fn, "v", v, 2, hd, Tk, v_token, kv_heads, v_head, false));
@@ -284,6 +290,7 @@ int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const
   if (!aligned(cu_q, 4)) return fail(QLIN_ERR_UNSUPPORTED, "%s: row bounds must be 4-byte aligned", fn);
   QA_TRY(check_tensor(fn, "q", q, 2, hd, T, q_token, q_heads, q_head, false));
   QA_TRY(check_tensor(fn, "out", out, 2, hd, T, o_token, q_heads, o_head, true));
+  QA_TRY(check_apart(fn, q, out));
   PromptArgs a = {};
   QA_TRY(check_paged(fn, cache, table, table_stride, max_pages, kv_len, kv_heads, hd, dtype, a.kv));
   a.q = q, a.qt = q_token, a.qh = q_head;
@@ -307,6 +314,7 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   if (B > kMaxRows / kv_heads) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d rows", fn, kMaxRows);
   QA_TRY(check_tensor(fn, "q", q, 2, hd, B, q_seq, q_heads, q_head, false));
   QA_TRY(check_tensor(fn, "out", out, 2, hd, B, o_seq, q_heads, o_head, true));
+  QA_TRY(check_apart(fn, q, out));
   DecodeArgs a = {};
   QA_TRY(check_paged(fn, cache, table, table_stride, max_pages, kv_len, kv_heads, hd, dtype, a.kv));
   char* part;

@@ -488,14 +488,21 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
   join(0, per, groups, [&](int f, f32x4 o, float, float ls) { store_out(f, o, ls); });
 }
 
-template <typename T, int HD>
-hipError_t launch(const DecodeArgs& a, hipStream_t st) {
+template <typename T, int HD, bool Q8>
+hipError_t launch_q(const DecodeArgs& a, hipStream_t st) {
   const int rows = a.G < 16 ? a.G : 16;
   const size_t lds = ((size_t)kWaves * rows * HD + kWaves * 32) * sizeof(float);
-  const dim3 grid((unsigned)(a.units * a.HKV * a.gb));
-  if (a.kv.k.s) hipLaunchKernelGGL((decode_kernel<T, HD, true>), grid, dim3(kThreads), lds, st, a);
-  else hipLaunchKernelGGL((decode_kernel<T, HD, false>), grid, dim3(kThreads), lds, st, a);
+  auto kern = decode_kernel<T, HD, Q8>;
+  static std::atomic<uint64_t> done{0};
+  const hipError_t e = allow_lds((const void*)kern, ((size_t)kWaves * 16 * HD + kWaves * 32) * sizeof(float), done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.units * a.HKV * a.gb)), dim3(kThreads), lds, st, a);
   return hipGetLastError();
+}
+
+template <typename T, int HD>
+hipError_t launch(const DecodeArgs& a, hipStream_t st) {
+  return a.kv.k.s ? launch_q<T, HD, true>(a, st) : launch_q<T, HD, false>(a, st);
 }
 
 template <typename T>

@@ -2,6 +2,8 @@
 // place of a sequence's keys in memory.
 #pragma once
 
+#include <atomic>
+
 #include "attn_internal.h"
 #include "qlin_dev.h"
 
@@ -85,5 +87,18 @@ __device__ __forceinline__ N lane_value(N v, int at) {
 // 2^x, and the factor between two running maxima (in powers of two) of which the first may be
 // -inf: nothing was seen yet, or scores of -inf alone.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Lets a kernel take `bytes` of dynamic LDS on the current device; `done` holds a bit for each
+// device where it may.
+inline hipError_t allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 }  // namespace qlin

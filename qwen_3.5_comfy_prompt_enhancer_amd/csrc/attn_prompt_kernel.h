@@ -272,9 +272,17 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
 #pragma unroll
     for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
 
-  bool bad = false;
   const int* table = PAGED ? a.kv.table + t.b * a.kv.table_stride : nullptr;
   const int nk = t.s.nk;
+  // whether a page of the unit's keys lies outside the cache: looked at once, by every wave (each
+  // fetches a quarter of the keys that all of them use)
+  bool any_bad = false;
+  if constexpr (PAGED) {
+    const int e1 = (min(kb1 * G::KB, nk) - 1) >> a.kv.page_shift;
+    for (int e = (kb0 * G::KB) >> a.kv.page_shift; e <= e1; e += 64)
+      any_bad |= (unsigned)table[min(e + lane, e1)] >= (unsigned)a.kv.num_pages;
+    any_bad = __any(any_bad);
+  }
   // this wave's 8 keys of a block: the first one's place (keys behind the last are the last)
   auto key8_of = [&](int kb) { return min(min(kb, kb1 - 1) * G::KB + 8 * wave, (nk - 1) & ~7); };
   // (a scalar load: a vector one's wait would also wait for the copies in flight)
@@ -300,13 +308,7 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     return PAGED ? x.p + ((uint64_t)(uint32_t)pid * x.sp + (uint64_t)((uint32_t)key & pmask) * x.st)
                  : x.p + (uint64_t)(uint32_t)key * x.st;
   };
-  auto checked = [&](int pid) {
-    if (PAGED && (unsigned)pid >= (unsigned)a.kv.num_pages) {
-      bad = true;
-      return 0;
-    }
-    return pid;
-  };
+  auto checked = [&](int pid) { return PAGED && (unsigned)pid >= (unsigned)a.kv.num_pages ? 0 : pid; };
 
   // Copies of this wave's 8 keys of block kb.  16-bit: to their swizzled places in a stage.
   auto issue = [&](uint32_t stage, int kb, int pid) __attribute__((always_inline)) {
@@ -550,7 +552,6 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
     __builtin_amdgcn_sched_barrier(0);
   }
-
   // (the row again, from a thread index that the compiler takes for another, and the arguments read
   // again, so that nothing of what follows is kept in registers through the loop)
   int tid2 = (int)threadIdx.x;
@@ -590,7 +591,6 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
   auto ld_ml = [&](unsigned part, int r) {
     return __builtin_amdgcn_raw_buffer_load_b64(rs, part * stride + ML + (unsigned)r * 8u, 0, kCpolSc1);
   };
-  const bool any_bad = __any(bad);
 
   if (!__any(again)) {
     if (any_bad) l = __builtin_nanf("");
@@ -842,9 +842,9 @@ template <typename T, int HD, bool Q8, bool PAGED>
 hipError_t prompt_go(const PromptArgs& a, hipStream_t st) {
   const size_t lds = (size_t)prompt_lds<HD, Q8>();
   auto kern = prompt_kernel<T, HD, Q8, PAGED>;
-  static const hipError_t attr = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                     (int)lds);
-  if (attr != hipSuccess) return attr;
+  static std::atomic<uint64_t> done{0};
+  const hipError_t e = allow_lds((const void*)kern, lds, done);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3(grid_of(a.HKV, a.units)), dim3(kPromptThreads), lds, st, a);
   if (a.target > 0 && a.join_apart)
     hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(a.tiles * a.HKV * (kPromptRows / 32) * (HD / 32))),

@@ -248,7 +248,7 @@ def attn_prompt(q, k, v, cu_q, out, cu_k=None, scale=None, causal=True):
     [Tk, kv_heads, hd].  cu_q, cu_k: int32 [B + 1], rising from 0.  `causal`: query i of a
     sequence sees its keys j <= i + keys - queries (the last query sees all).  scale:
     hd ** -0.5 unless given.  out [T, q_heads, hd]; a row that sees no key is zero, rows of
-    no sequence stay as they were.  Returns out."""
+    no sequence stay as they were.  out must not overlap q, k or v.  Returns out."""
     T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must both be [rows, kv_heads, hd]")

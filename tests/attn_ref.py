@@ -3,13 +3,13 @@
 u is half a step of a type relative to the value (`finfo.eps / 2`).  A kernel rounds
 
 * its output once: u |o|;
-* P to 16 bits for its product (bf16 where the cache is int8 and the call a decode):
-  u_p A, with A = sum_j p_j |v_j| / sum_j p_j, as each term moves by at most u_p of itself;
-* where prompts read an int8 cache, code x scale to the queries' type: u A for the values,
-  and for the keys a score off by u S, S = scale max_j sum_d |q_d k_jd|: every p moves by
-  a factor exp(+-u S) and their sum too, 2 u S A in the first order (3 allowed: u S < 0.3);
-* in 32 bits (e = 2^-24): a score's hd products and sums, (hd + 4) e S (twice, as above),
-  exponentials and rescaling (16 e), and sums over n keys of which no accumulator takes
+* P (times a value's scale, where the cache is int8) to 16 bits for its product: u_p A, with
+  A = sum_j p_j |v_j| / sum_j p_j, as each term moves by at most u_p of itself; u_p is that of the
+  queries' type, of bf16 in prompts of bf16 queries over int8, and 2^-16 where P goes as two bf16
+  numbers (decode and fp16 queries over int8);
+* in 32 bits (e = 2^-24): a score's hd products and sums, (hd + 4) e S with
+  S = scale max_j sum_d |q_d k_jd| (every p moves by a factor exp(+-that) and their sum too, hence
+  twice), exponentials and rescaling (16 e), and sums over n keys of which no accumulator takes
   more than n / 8 steps: (n / 8 + 64) e, once for the sum of P and once for O.
 """
 from __future__ import annotations
@@ -23,14 +23,15 @@ def half_step(dt):
     return torch.finfo(dt).eps / 2
 
 
-def attend(q, k, v, scale, seen, dt, p_dt=None, kv8=False):
+def attend(q, k, v, scale, seen, dt, up=None):
     """q [Lq, HQ, D], k / v [Lk, HKV, D] of any type, seen [Lq, Lk] (bool).  Returns the
     output and the allowed error, both in 64 bits, [Lq, HQ, D]."""
     lq, hq, d = q.shape
     lk, hkv = k.shape[:2]
     out = torch.zeros((lq, hq, d), dtype=torch.float64, device=q.device)
     tol = torch.zeros_like(out)
-    u, up = half_step(dt), half_step(p_dt or dt)
+    u = half_step(dt)
+    up = u if up is None else up
     if lk == 0 or lq == 0:
         return out, tol + 1e-30
     some = seen.any(1)
@@ -47,8 +48,6 @@ def attend(q, k, v, scale, seen, dt, p_dt=None, kv8=False):
         a = (p @ torch.nan_to_num(vh, nan=0.0, posinf=0.0, neginf=0.0).abs()) / l
         S = (qh.abs() @ kh.abs().t() * scale).masked_fill(~seen, 0.0).nan_to_num(0.0, 0.0, 0.0).amax(1, keepdim=True)
         t = u * o.abs() + a * (up + 2 * (d + 4) * E32 * S + (16 + 2 * (lk / 8 + 64)) * E32)
-        if kv8:
-            t = t + a * (u + 3 * u * S)
         out[:, h], tol[:, h] = torch.where(some[:, None], o, 0.0), t * 1.01 + 1e-30
     # a subnormal fp16 output is off by half its spacing instead
     if dt == torch.float16:

@@ -90,7 +90,7 @@ def _kv8(A, **kw):
     return _kv(A, **d)
 
 
-DECODE = dict(q=FAKE, qs=512, qh=64, kv=None, table=FAKE, ts=8, mp=8, kv_len=FAKE, out=FAKE, os=512, oh=64, B=2, hq=8,
+DECODE = dict(q=FAKE, qs=512, qh=64, kv=None, table=FAKE, ts=8, mp=8, kv_len=FAKE, out=FAKE + 4096, os=512, oh=64, B=2, hq=8,
               hkv=4, hd=64, dt=2, scale=0.125, ws=FAKE, nws=256 << 20, st=None)
 
 
@@ -109,7 +109,7 @@ def _decode(A, **kw):
     (dict(table=None), "null page table"), (dict(kv_len=None), "null page table"), (dict(kv_len=FAKE + 2), "4-byte"),
     (dict(mp=-1), "negative"), (dict(mp=1 << 28), "keys a sequence"), (dict(ws=None), "workspace"),
     (dict(nws=1 << 20), "workspace"), (dict(ws=FAKE + 8), "256-byte"), (dict(B=1 << 24), "more than"),
-    (dict(qs=1 << 30), "above"),
+    (dict(qs=1 << 30), "above"), (dict(out=FAKE), "must not be q"),
 ])
 def test_decode_refusals(A, bad, text):
     rc, msg = _decode(A, **bad)
@@ -120,7 +120,7 @@ def test_decode_refusals(A, bad, text):
     (dict(page=48), "power of two"), (dict(page=8), "power of two"), (dict(page=2048), "power of two"),
     (dict(num_pages=0), "no pages"), (dict(dtype=1), "cache dtype"), (dict(k=None), "null k_cache"),
     (dict(v=FAKE + 8), "v_cache must be 16-byte"), (dict(k_token=260), "multiples of 8"),
-    (dict(v_page=4), "page strides"), (dict(k_s=FAKE), "no scales"),
+    (dict(v_page=4), "page strides"), (dict(k_s=FAKE), "no scales"), (dict(k_page=1 << 31), "page strides above"),
 ])
 def test_cache_refusals(A, bad, text):
     rc, msg = _decode(A, kv=ctypes.byref(_kv(A, **bad)))
@@ -128,7 +128,7 @@ def test_cache_refusals(A, bad, text):
 
 
 @pytest.mark.parametrize("bad,text", [
-    (dict(k_s=None), "needs k_s"), (dict(v_s=FAKE + 2), "4-byte"), (dict(vs_head=-1), "negative"),
+    (dict(k_s=None), "needs k_s"), (dict(v_s=FAKE + 2), "4-byte"), (dict(vs_head=-1), "negative"), (dict(ks_page=1 << 30), "too large"),
     (dict(k_token=264), "multiples of 16"),
 ])
 def test_int8_cache_refusals(A, bad, text):
@@ -145,7 +145,7 @@ def test_nothing_to_do_is_no_launch(A):
                                     None, 0, None) == 0
 
 
-PROMPT = dict(q=FAKE, qt=512, qh=64, k=FAKE, kt=256, kh=64, v=FAKE, vt=256, vh=64, cu=FAKE, ck=FAKE, out=FAKE, ot=512,
+PROMPT = dict(q=FAKE, qt=512, qh=64, k=FAKE, kt=256, kh=64, v=FAKE, vt=256, vh=64, cu=FAKE, ck=FAKE, out=FAKE + 4096, ot=512,
               oh=64, T=9, Tk=9, B=2, hq=8, hkv=4, hd=64, dt=2, scale=0.125, causal=1, ws=FAKE, nws=256 << 20, st=None)
 
 

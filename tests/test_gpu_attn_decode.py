@@ -32,7 +32,7 @@ def _run(lens, hq, hkv, hd, dt, page=64, int8=False, seed=0, head_major=True, sc
     for b, n in enumerate(lens):
         k, v = R.gathered(c, table, b, n)
         seen = torch.ones((1, n), dtype=torch.bool, device="cuda")
-        ref, tol = R.attend(q[b:b + 1], k, v, scale or hd ** -0.5, seen, dt, BF if int8 else None)
+        ref, tol = R.attend(q[b:b + 1], k, v, scale or hd ** -0.5, seen, dt, 2.0 ** -16 if int8 else None)
         R.check(out[b:b + 1], ref, tol, f"sequence {b} of {n} keys")
     return out
 

@@ -64,7 +64,7 @@ def _paged(nq, past, hq, hkv, hd, dt, page=64, int8=False, causal=True, seed=0, 
     for b, (m, n) in enumerate(zip(nq, lens)):
         k, v = R.gathered(c, table, b, n)
         seen = R.causal(m, n, "cuda") if causal else torch.ones((m, n), dtype=torch.bool, device="cuda")
-        ref, tol = R.attend(q[at:at + m], k, v, hd ** -0.5, seen, dt, kv8=int8)
+        ref, tol = R.attend(q[at:at + m], k, v, hd ** -0.5, seen, dt, 2.0 ** -16 if int8 and dt == FP else None)
         R.check(out[at:at + m], ref, tol, f"sequence {b} ({m}, {n})")
         at += m
     return out
