@@ -18,7 +18,8 @@
  *   - a page outside 0 .. num_pages - 1 in front of a sequence's end makes NaN of every
  *     output that sees a key of it, and maybe of others of that sequence (no memory outside
  *     the cache is read);
- *   - row bounds (cu) are clamped to the rows there are.
+ *   - row bounds (cu) are clamped to the rows there are, and query bounds that fall count as the
+ *     highest before them.
  */
 #ifndef QLIN_ATTN_H
 #define QLIN_ATTN_H

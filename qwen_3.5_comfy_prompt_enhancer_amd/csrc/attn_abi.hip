@@ -161,13 +161,16 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   }
   const long long tiles = (long long)a.T * a.G / kPromptRows + a.B;
   const long long slot = prompt_slot_floats(hd) * 4;
-  if (max_keys <= kPromptMinBlocks * kPromptBlock) target = 0;
+  if (max_keys <= kPromptNoCut) target = 0;
   // every unit of a key head has a slot: at most 2 target / HKV + tiles of them (and two more for
   // what the device's 32-bit estimate rounds)
   target = std::min(target, ((long long)avail / slot / a.HKV - tiles - 3) * a.HKV / 2);
   if (target <= a.HKV || tiles * a.HKV * kPromptCounters * 4 > (long long)counter_bytes()) target = 0;
   a.target = (int)target;
   a.tiles = (int)tiles;
+  // (a cut costs about as much as seven blocks; where most of the chip has a tile already it gives
+  // less than where it has not)
+  a.shortest = tiles * a.HKV <= kPromptFewTiles ? 8 : tiles * a.HKV <= kPromptJoinApart ? 12 : 16;
   a.join_apart = tiles * a.HKV <= kPromptJoinApart;
   a.units = (int)(tiles + (target ? (2 * target + a.HKV - 1) / a.HKV + 2 : 0));
   a.part = (float*)part;

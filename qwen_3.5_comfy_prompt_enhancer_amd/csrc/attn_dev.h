@@ -78,6 +78,34 @@ __device__ __forceinline__ N wave_scan(N v) {
   return v;
 }
 
+// Inclusive prefix maximum of numbers that are not negative.
+__device__ __forceinline__ int wave_scan_max(int v) {
+  auto with = [&](auto ctrl, auto rows) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+  };
+  using std::integral_constant;
+  with(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});
+  with(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  with(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  with(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  with(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});
+  with(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return v;
+}
+
+// Maximum over a wave, on every lane.
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, lane_xor<1>(v));
+  v = fmaxf(v, lane_xor<2>(v));
+  v = fmaxf(v, lane_xor<4>(v));
+  v = fmaxf(v, lane_xor<8>(v));
+  float x, y;
+  lane_pair<16>(v, x, y);
+  v = fmaxf(x, y);
+  lane_pair<32>(v, x, y);
+  return fmaxf(x, y);
+}
+
 // The value of one lane (a uniform number), the same on all.
 template <typename N>
 __device__ __forceinline__ N lane_value(N v, int at) {

@@ -101,6 +101,7 @@ struct PromptArgs {
   int causal;
   float c;                // scale * log2(e)
   int target;             // work units to cut the keys into; 0: no cut
+  int shortest;           // blocks of the shortest cut
   int units;              // units per key head: the grid's bound
   int tiles;              // row tiles per key head at most
   int join_apart;         // parts are joined by a launch of its own
@@ -108,8 +109,9 @@ struct PromptArgs {
   unsigned* cnt;          // arrival counters of each tile, zero between calls
 };
 constexpr int kPromptBlock = 32;     // keys of a step
-constexpr int kPromptMinBlocks = 4;  // shortest cut
-constexpr int kPromptJoinApart = 64;  // row tiles of all key heads up to which a second launch joins
+constexpr int kPromptNoCut = 11 * kPromptBlock;  // keys that are never cut (below 1.5 of the shortest cut)
+constexpr int kPromptFewTiles = 96;
+constexpr int kPromptJoinApart = 256;  // row tiles of all key heads up to which a second launch joins
 constexpr int kPromptCounters = 32;  // counters of a (key head, row tile)
 constexpr int kPromptRows = 128;     // rows of a tile: tokens x the query heads of a key head
 // a unit's partial: sums of its rows, then (maximum, sum of P) of each

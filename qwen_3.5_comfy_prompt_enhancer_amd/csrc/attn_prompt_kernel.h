@@ -69,19 +69,27 @@ struct Seq {
   int k0, nk;   // first packed row of its keys, keys
 };
 
-__device__ __forceinline__ Seq seq_of(const PromptArgs& a, int b) {
-  Seq s;
-  const int c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], 0), a.T);
-  s.q0 = c0;
-  s.nq = max(0, c1 - c0);
-  if (a.kv.table) {
-    s.k0 = 0;
-    s.nk = kv_length(a.kv, b);
-  } else {
-    const int e0 = min(max(a.kv.cu[b], 0), a.kv.rows), e1 = min(max(a.kv.cu[b + 1], 0), a.kv.rows);
-    s.k0 = e0;
-    s.nk = max(0, e1 - e0);
+// Sequences b0 + lane (none behind the last).  Bounds are clamped to the rows there are and taken as
+// rising: a sequence starts no earlier than any bound before it, so that sequences share no rows
+// and never have more row tiles than the grid was made for, whatever `cu` holds.  `start`: the
+// highest bound so far, for calls with rising b0.
+__device__ __forceinline__ Seq seq_of(const PromptArgs& a, int b0, int& start) {
+  const int b = b0 + ((int)threadIdx.x & 63);
+  Seq s = {0, 0, 0, 0};
+  int c0 = 0, c1 = 0;
+  if (b < a.B) {
+    c0 = min(max(a.cu[b], 0), a.T);
+    c1 = min(max(a.cu[b + 1], 0), a.T);
+    if (a.kv.table) {
+      s.nk = kv_length(a.kv, b);
+    } else {
+      s.k0 = min(max(a.kv.cu[b], 0), a.kv.rows);
+      s.nk = max(0, min(max(a.kv.cu[b + 1], 0), a.kv.rows) - s.k0);
+    }
   }
+  s.q0 = max(wave_scan_max(c0), start);
+  s.nq = max(0, c1 - s.q0);
+  start = lane_value(s.q0, 63);
   return s;
 }
 
@@ -115,30 +123,32 @@ struct Tile {
 template <bool UNITS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
   constexpr int ROWS = kPromptRows;
-  const int lane = (int)threadIdx.x & 63;
-  auto mine = [&](int b0) {
-    Seq s = {0, 0, 0, 0};
-    if (b0 + lane < a.B) s = seq_of(a, b0 + lane);
-    return s;
-  };
   auto tiles_of = [&](const Seq& s) { return (int)(((long long)s.nq * a.G + ROWS - 1) / ROWS); };
   auto blocks_of = [&](const Seq& s) { return (s.nk + kPromptBlock - 1) / kPromptBlock; };
-  const Seq first = mine(0);
+  int start = 0;
+  const Seq first = seq_of(a, 0, start);
+  const int start1 = start;
   int chunk = 1 << 30;
   if (a.target > 0) {
-    float w = 0.0f;  // (an estimate; the same for all workgroups)
+    float w = 0.0f, longest = 0.0f;  // (an estimate; the same for all workgroups)
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const Seq s = b0 ? mine(b0) : first;
+      const Seq s = b0 ? seq_of(a, b0, start) : first;
       const float t = (float)tiles_of(s), n = (float)blocks_of(s);
       // causal rows see half of their own keys on average (never less than half of all)
       w += a.causal ? fmaxf(t * (n - (float)(s.nq / (2 * kPromptBlock))), t * n * 0.5f) : t * n;
+      if (t > 0.0f) longest = fmaxf(longest, n);
     }
     w = lane_value(wave_scan(w), 63);
-    chunk = max((int)fminf(ceilf(w * (float)a.HKV / (float)a.target), 1e9f), kPromptMinBlocks);
+    longest = wave_max(longest);
+    // a cut that takes less than a third off the longest tile costs more than it gives
+    const float c = fmaxf(ceilf(w * (float)a.HKV / (float)a.target), (float)a.shortest);
+    if (longest >= 1.5f * c) chunk = (int)fminf(c, 1e9f);
+    else if (!UNITS) return false;  // (nothing to join)
   }
   int ubase = 0, tbase = 0;
+  start = start1;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const Seq s = b0 ? mine(b0) : first;
+    const Seq s = b0 ? seq_of(a, b0, start) : first;
     const int tiles = tiles_of(s);
     const int most = max(1, (blocks_of(s) + chunk - 1) / chunk);
     const int ue = wave_scan(tiles * most), te = wave_scan(tiles);
@@ -724,7 +734,7 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
       f32x4 o[4] = {};
       float M = kNegInf, ls = 0.0f;
       const unsigned off = (unsigned)((set * G::ND + d) * 4096 + lane * 16);
-      constexpr int N = 4;  // parts in flight
+      constexpr int N = HD == 64 ? 4 : 8;  // parts in flight
       for (int s0 = 0; s0 < n; s0 += N) {
         f32x4 x[N][4];
         u32x2 y[N];
@@ -795,11 +805,12 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
 // would read a tile's: 512 tokens over 6000 keys 86 us against 68 so; an 8192-token prompt's 250
 // tiles of two parts 272 against 304.)
 template <typename T, int HD>
-__global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a) {
+__global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a, int per) {
   constexpr int ROWS = kPromptRows;
   constexpr int SETS = ROWS / 32, ND = HD / 32;
   const int tid = (int)threadIdx.x, lane = tid & 63;
-  const int d = (int)blockIdx.x % ND, set = (int)blockIdx.x / ND % SETS, u = (int)blockIdx.x / (ND * SETS);
+  const int runs = ND / per;  // workgroups of a row set, `per` 32-wide blocks each
+  const int d0 = (int)blockIdx.x % runs * per, set = (int)blockIdx.x / runs % SETS, u = (int)blockIdx.x / (runs * SETS);
   const int hk = u % a.HKV;
   Tile t;
   if (!find_tile<false>(a, u / a.HKV, t)) return;
@@ -809,33 +820,36 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const Promp
   const long long sf = prompt_slot_floats(HD) * t.step;
   const float* p0 = a.part + ((long long)hk * a.units + t.slot) * prompt_slot_floats(HD);
   const float* ml = p0 + ROWS * HD + (set * 32 + (lane & 31)) * 2;
-  const float* po = p0 + set * 32 * HD + d * 1024 + tid * 4;
-  f32x4 o = {0, 0, 0, 0};
-  float M = kNegInf, l = 0.0f;
-  constexpr int N = 8;  // parts in flight
-  for (int s0 = 0; s0 < t.parts; s0 += N) {
-    f32x4 x[N];
-    float2 y[N];
-#pragma unroll
-    for (int s = 0; s < N; ++s) {
-      const long long at = min(s0 + s, t.parts - 1) * sf;
-      x[s] = *(const f32x4*)(po + at);
-      y[s] = *(const float2*)(ml + at);
-    }
-#pragma unroll
-    for (int s = 0; s < N; ++s) {
-      if (s0 + s >= t.parts) break;
-      const float mn = fmaxf(M, y[s].x), ms = mn == kNegInf ? 0.0f : mn;
-      const float e0 = exp2_(M - ms), e1 = exp2_(y[s].x - ms);
-      o = o * e0 + x[s] * e1;
-      l = l * e0 + y[s].y * e1;
-      M = mn;
-    }
-  }
-  const float inv = seen(a, t.s, i) > 0 ? 1.0f / l : 0.0f;
   uint16_t* out = (uint16_t*)a.o + (long long)(t.s.q0 + i) * a.ot + (hk * a.G + (R - i * a.G)) * a.oh;
-  *(u32x2*)(out + d * 32 + (tid >> 6) * 8 + 4 * (lane >> 5)) =
-      u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+  const bool some = seen(a, t.s, i) > 0;
+  for (int d = d0; d < d0 + per; ++d) {
+    const float* po = p0 + set * 32 * HD + d * 1024 + tid * 4;
+    f32x4 o = {0, 0, 0, 0};
+    float M = kNegInf, l = 0.0f;
+    constexpr int N = 8;  // parts in flight
+    for (int s0 = 0; s0 < t.parts; s0 += N) {
+      f32x4 x[N];
+      float2 y[N];
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        const long long at = min(s0 + s, t.parts - 1) * sf;
+        x[s] = *(const f32x4*)(po + at);
+        y[s] = *(const float2*)(ml + at);
+      }
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        if (s0 + s >= t.parts) break;
+        const float mn = fmaxf(M, y[s].x), ms = mn == kNegInf ? 0.0f : mn;
+        const float e0 = exp2_(M - ms), e1 = exp2_(y[s].x - ms);
+        o = o * e0 + x[s] * e1;
+        l = l * e0 + y[s].y * e1;
+        M = mn;
+      }
+    }
+    const float inv = some ? 1.0f / l : 0.0f;
+    *(u32x2*)(out + d * 32 + (tid >> 6) * 8 + 4 * (lane >> 5)) =
+        u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
+  }
 }
 
 template <typename T, int HD, bool Q8, bool PAGED>
@@ -846,9 +860,13 @@ hipError_t prompt_go(const PromptArgs& a, hipStream_t st) {
   const hipError_t e = allow_lds((const void*)kern, lds, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3(grid_of(a.HKV, a.units)), dim3(kPromptThreads), lds, st, a);
-  if (a.target > 0 && a.join_apart)
-    hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(a.tiles * a.HKV * (kPromptRows / 32) * (HD / 32))),
-                       dim3(kPromptThreads), 0, st, a);
+  if (a.target > 0 && a.join_apart) {
+    const int sets = a.tiles * a.HKV * (kPromptRows / 32);
+    int per = 1;  // at most about as many workgroups as run at once
+    while (per < HD / 32 && sets * (HD / 32 / per) > 2048) per *= 2;
+    hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(sets * (HD / 32 / per))), dim3(kPromptThreads), 0,
+                       st, a, per);
+  }
   return hipGetLastError();
 }
 

@@ -325,6 +325,28 @@ def test_contents_that_name_no_page_or_too_many_keys(int8):
     assert torch.equal(xp, op)
     x, xp = both(table, kv, _ints([-3, 40, 40, 40]))
     assert torch.equal(xp[:40], op[:40]) and (xp[40:] == 7).all()
+    # bounds that fall count as the highest before them
+    x, xp = both(table, kv, _ints([0, 40, 20, 90]))
+    y, yp = both(table, kv, _ints([0, 40, 40, 90]))
+    assert torch.equal(xp, yp)
+
+
+def test_bounds_that_fall_leave_the_workspace_as_it_was():
+    """Many sequences that would all have every row: one has them, and the next calls are right."""
+    from qwen35_amd.kernels import attention as A
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n, B = 700, 80
+    q, k, v = (torch.randn((n, h, HD), generator=g, device="cuda").to(BF) for h in (HQ, HKV, HKV))
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    A.attn_prompt(q, k, v, _ints([0, n]), want)
+    bad = _ints([0, n] * (B // 2) + [0])
+    A.attn_prompt(q, k, v, bad, out, cu_k=bad)
+    torch.cuda.synchronize()
+    ref, tol = R.attend(q, k, v, HD ** -0.5, R.causal(n, n, "cuda"), BF)
+    R.check(out, ref, tol)
+    A.attn_prompt(q, k, v, _ints([0, n]), out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
 
 
 def test_strided_queries_and_outputs():
