@@ -155,12 +155,29 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   char* part;
   size_t avail;
   QA_TRY(workspace_parts(fn, ws, ws_bytes, &part, &avail));
+  // Units: about as many as run at once (two, three or four workgroups a CU by head size), fewer
+  // where their sums are the larger; 8192 tokens, 256 values, 320 / 384 / 448 / 512 / 640 units: 288 / 266 /
+  // 258 / 264 / 283 us.
+  a.rows = kPromptRows;
   long long target = hd == 256 ? 448 : hd == 128 ? 512 : 640;
+  // Few tiles (of 16-bit keys) are halved, two groups of waves sharing their keys: 512 tokens 20.6
+  // -> 18.6 us, four prompts of 512 27.3 -> 19.4.  Beyond a halved tile for each CU, or with work
+  // enough to fill the chip with whole ones (by what the host knows of it), that only moves twice the
+  // keys (2048 tokens 44.8 -> 50.0, four chunks of 700 over 3000 keys 69 -> 94); sequences of few
+  // rows leave half of a whole tile empty.  A CU then holds one workgroup, and units stay below
+  // the CUs (100-token chunks, 192 / 256 units: 25.5 / 35.4).
+  const long long rows = (long long)a.T * a.G, halves = (rows * 2 / kPromptRows + a.B) * a.HKV;
+  const long long blocks = a.kv.table ? max_keys / kPromptBlock : max_keys / a.B / kPromptBlock / (a.causal ? 2 : 1);
+  if (!a.kv.k.s && halves <= kPromptHalves &&
+      (rows <= (long long)a.B * kPromptRows / 2 || halves * blocks / 2 <= kPromptFill)) {
+    a.rows = kPromptRows / 2;
+    target = 192;
+  }
   if (const char* e = getenv("QLIN_PROMPT_UNITS")) {  // for tuning runs
     if (atoi(e) >= 0) target = atoi(e);
   }
-  const long long tiles = (long long)a.T * a.G / kPromptRows + a.B;
-  const long long slot = prompt_slot_floats(hd) * 4;
+  const long long tiles = (long long)a.T * a.G / a.rows + a.B;
+  const long long slot = prompt_slot_floats(hd, a.rows) * 4;
   if (max_keys <= kPromptNoCut) target = 0;
   // every unit of a key head has a slot: at most 2 target / HKV + tiles of them (and two more for
   // what the device's 32-bit estimate rounds)

@@ -103,6 +103,7 @@ struct PromptArgs {
   int target;             // work units to cut the keys into; 0: no cut
   int shortest;           // blocks of the shortest cut
   int units;              // units per key head: the grid's bound
+  int rows;               // rows of a tile: kPromptRows, or half as many with two key groups
   int tiles;              // row tiles per key head at most
   int join_apart;         // parts are joined by a launch of its own
   float* part;            // unit partials [key head][unit]
@@ -110,12 +111,14 @@ struct PromptArgs {
 };
 constexpr int kPromptBlock = 32;     // keys of a step
 constexpr int kPromptNoCut = 11 * kPromptBlock;  // keys that are never cut (below 1.5 of the shortest cut)
-constexpr int kPromptFewTiles = 96;
+constexpr int kPromptFewTiles = 96;  // tiles of all key heads up to which short cuts pay
+constexpr int kPromptHalves = 272;   // halved tiles of all key heads up to which tiles are halved
+constexpr int kPromptFill = 3000;    // (tile, block) pairs that fill the chip with whole tiles
 constexpr int kPromptJoinApart = 256;  // row tiles of all key heads up to which a second launch joins
 constexpr int kPromptCounters = 32;  // counters of a (key head, row tile)
 constexpr int kPromptRows = 128;     // rows of a tile: tokens x the query heads of a key head
 // a unit's partial: sums of its rows, then (maximum, sum of P) of each
-__host__ __device__ constexpr long long prompt_slot_floats(int hd) { return (long long)kPromptRows * (hd + 2); }
+__host__ __device__ constexpr long long prompt_slot_floats(int hd, int rows) { return (long long)rows * (hd + 2); }
 hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, hipStream_t st);
 hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, hipStream_t st);
 hipError_t launch_prompt_f16(const PromptArgs& a, int hd, hipStream_t st);

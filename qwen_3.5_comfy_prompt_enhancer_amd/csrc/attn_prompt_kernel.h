@@ -120,9 +120,8 @@ struct Tile {
 // within a part.  With chunk the average over the workgroups that run at once, long causal
 // prompts then come out even: whole chunks start first, and the workgroup that gets the
 // shortest rest of one part goes on with the longest of the next.
-template <bool UNITS>
+template <int ROWS, bool UNITS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
-  constexpr int ROWS = kPromptRows;
   auto tiles_of = [&](const Seq& s) { return (int)(((long long)s.nq * a.G + ROWS - 1) / ROWS); };
   auto blocks_of = [&](const Seq& s) { return (s.nk + kPromptBlock - 1) / kPromptBlock; };
   int start = 0;
@@ -221,11 +220,11 @@ struct PGeo {
   static __device__ __forceinline__ int swv(int r) { return HD >= 128 ? r & 3 : (r >> 1) & 1; }
 };
 
-// LDS of a workgroup.  16-bit keys: a ring of two stages.  int8: one 16-bit tile, made from a
+// LDS of a workgroup.  16-bit keys: a ring of two stages of KG blocks.  int8: one 16-bit tile, made from a
 // ring of two tiles of codes and their scales.
-template <int HD, bool Q8>
+template <int HD, bool Q8, int KG>
 constexpr int prompt_lds() {
-  return Q8 ? PGeo<HD>::STAGE + 2 * (PGeo<HD>::STAGE / 2 + PGeo<HD>::SCALES) : 2 * PGeo<HD>::STAGE;
+  return Q8 ? PGeo<HD>::STAGE + 2 * (PGeo<HD>::STAGE / 2 + PGeo<HD>::SCALES) : 2 * KG * PGeo<HD>::STAGE;
 }
 
 template <typename V>
@@ -237,15 +236,19 @@ __device__ __forceinline__ void lds_st(uint32_t at, V v) {
   *(__attribute__((address_space(3))) V*)(uintptr_t)at = v;
 }
 
-// Q8: int8 cache.
-template <typename T, int HD, bool Q8, bool PAGED>
-__global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) void prompt_kernel(const PromptArgs a) {
+// Q8: int8 cache.  KG = 2: two waves hold the rows of a tile of 64, the other two the same rows
+// over every second block, and their sums are added through LDS at the end: for few tiles, each of
+// which then takes half as long.
+template <typename T, int HD, bool Q8, bool PAGED, int KG>
+__global__ __launch_bounds__(kPromptThreads, KG == 2 ? 1 : HD == 64 ? 4 : HD == 128 ? 3 : 2)
+void prompt_kernel(const PromptArgs a) {
+  static_assert(KG == 1 || !Q8, "int8 keys: one group");
   using G = PGeo<HD>;
   using TV = std::conditional_t<Q8, Bf16, T>;  // type of P and V in their product
   // fp16 queries over int8 values: P x scale as two bf16 numbers, so that neither range nor
   // precision is lost
   constexpr int PN = Q8 && T::DT == DT_F16 ? 2 : 1;
-  constexpr int ROWS = kPromptRows;
+  constexpr int ROWS = kPromptRows / KG;
   constexpr int ES = Q8 ? 1 : 2;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
@@ -253,15 +256,16 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
   int hk, unit;
   split_grid(a.HKV, a.units, hk, unit);
   Tile t;
-  if (hk >= a.HKV || unit >= a.units || !find_tile<true>(a, unit, t)) return;
+  if (hk >= a.HKV || unit >= a.units || !find_tile<ROWS, true>(a, unit, t)) return;
   t.uniform();
   const int tid = (int)threadIdx.x;
   const int wave = (int)rfl32((uint32_t)tid >> 6), lane = tid & 63;
   const int col = lane & 31, h = lane >> 5;
   const int kb0 = t.part * t.chunk, kb1 = min(t.nblk - kb0, t.chunk) + kb0;
 
-  // this lane's row is R0 + col
-  const int R0 = t.tile * ROWS + wave * 32;
+  // this lane's row is R0 + col; its wave takes blocks kb0 + kg, kb0 + kg + KG, ...
+  const int rg = wave % (4 / KG), kg = wave / (4 / KG);
+  const int R0 = t.tile * ROWS + rg * 32;
   u32x4 Q[G::NS];
   int lim;
   {
@@ -397,13 +401,14 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
   // LDS places of this lane's operands: step s of K at ka ^ 32 s (the swizzle reaches 256 bytes),
   // 32-wide block d of V at va ^ 64 (d % 4), two transposing reads of 4 keys each
   const int s16 = lane & 15;
-  const uint32_t ka = lds0 + (uint32_t)(col * G::ROWB + ((h ^ G::swk(col)) << 4));
-  const uint32_t va = lds0 + (uint32_t)(G::HALF + (4 * h + (s16 >> 2)) * G::ROWB + (G::swv(s16 >> 2) << 6) +
+  const uint32_t mine = lds0 + (uint32_t)(kg * G::STAGE);
+  const uint32_t ka = mine + (uint32_t)(col * G::ROWB + ((h ^ G::swk(col)) << 4));
+  const uint32_t va = mine + (uint32_t)(G::HALF + (4 * h + (s16 >> 2)) * G::ROWB + (G::swv(s16 >> 2) << 6) +
                                         ((lane >> 4) & 1) * 32 + (s16 & 3) * 8);
 
   auto step = [&](auto stage_c, int kb, uint32_t scales) __attribute__((always_inline)) {
     constexpr uint32_t stage = decltype(stage_c)::value;
-    if (kb * G::KB >= wmax) return;
+    if (kb * G::KB >= wmax || (KG > 1 && kb >= kb1)) return;
     // operands are read kAhead products ahead (the order is fixed: left to itself the compiler
     // reads each just before its product, and the wave waits for LDS every time)
     auto k_at = [&](int s) {
@@ -519,25 +524,36 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
   };
 
   if (kb0 < kb1) {
-    int pid = page_of(kb0);
     if constexpr (!Q8) {
+      constexpr uint32_t RING = KG * G::STAGE;
       constexpr std::integral_constant<uint32_t, 0> s0;
-      constexpr std::integral_constant<uint32_t, G::STAGE> s1;
-      issue(lds0, kb0, pid);
-      pid = page_of(kb0 + 1);
+      constexpr std::integral_constant<uint32_t, RING> s1;
+      int pid[KG];
+      auto pages = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < KG; ++x) pid[x] = page_of(kb + x);
+      };
+      auto fetch = [&](uint32_t stage, int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < KG; ++x) issue(stage + (uint32_t)(x * G::STAGE), kb + x, pid[x]);
+      };
+      pages(kb0);
+      fetch(lds0, kb0);
+      pages(kb0 + KG);
       for (int kb = kb0;;) {
         meet();
-        issue(lds0 + G::STAGE, kb + 1, pid);
-        pid = page_of(kb + 2);
-        step(s0, kb, 0);
-        if (++kb >= kb1) break;
+        fetch(lds0 + RING, kb + KG);
+        pages(kb + 2 * KG);
+        step(s0, kb + kg, 0);
+        if ((kb += KG) >= kb1) break;
         meet();
-        issue(lds0, kb + 1, pid);
-        pid = page_of(kb + 2);
-        step(s1, kb, 0);
-        if (++kb >= kb1) break;
+        fetch(lds0, kb + KG);
+        pages(kb + 2 * KG);
+        step(s1, kb + kg, 0);
+        if ((kb += KG) >= kb1) break;
       }
     } else {
+      int pid = page_of(kb0);
       // codes of block kb + 1 land while block kb is widened and used
       const uint32_t c0 = lds0 + G::STAGE;
       constexpr uint32_t CODES = G::STAGE / 2 + G::SCALES;
@@ -562,6 +578,39 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
     __builtin_amdgcn_sched_barrier(0);
   }
+  if constexpr (KG == 2) {
+    // the second group's sums, then its maxima and sums of P, to LDS (every wave has read its last
+    // stage); the first group adds them
+    const uint32_t at = lds0 + (uint32_t)(rg * (32 * HD * 4 + 512) + lane * 16);
+    const uint32_t aml = lds0 + (uint32_t)(rg * (32 * HD * 4 + 512) + 32 * HD * 4 + lane * 8);
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          lds_st(at + (uint32_t)((d * 4 + i) * 1024),
+                 f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]});
+      lds_st(aml, u32x2{bitcast<uint32_t>(m), bitcast<uint32_t>(l)});
+    }
+    __syncthreads();
+    if (kg == 0) {
+      const u32x2 o1 = lds_ld<u32x2>(aml);
+      const float m1 = bitcast<float>(o1.x), mn = fmaxf(m, m1), ms = mn == kNegInf ? 0.0f : mn;
+      const float e0 = exp2_(m - ms), e1 = exp2_(m1 - ms);
+      l = l * e0 + bitcast<float>(o1.y) * e1;
+      m = mn;
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = lds_ld<f32x4>(at + (uint32_t)((d * 4 + i) * 1024));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[d][4 * i + e] = O[d][4 * i + e] * e0 + x[e] * e1;
+        }
+    }
+  }
+
   // (the row again, from a thread index that the compiler takes for another, and the arguments read
   // again, so that nothing of what follows is kept in registers through the loop)
   int tid2 = (int)threadIdx.x;
@@ -583,12 +632,12 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     for (int d = 0; d < G::ND; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) z = fmaf(O[d][i], 0.0f, z);
-    again = !(z == 0.0f) && tok < t.s.nq;
+    again = !(z == 0.0f) && tok < t.s.nq && kg == 0;
   }
   // partials: unit p of the tile at (slot + p step) of the key head's; 32-bit sums by row set,
   // 32-wide block, run of 8 values and lane, so that a wave moves 1 KiB at a time; then (maximum, sum
   // of P) of each row
-  constexpr unsigned SLOT = (unsigned)prompt_slot_floats(HD) * 4u;
+  constexpr unsigned SLOT = (unsigned)prompt_slot_floats(HD, ROWS) * 4u;
   const __amdgpu_buffer_rsrc_t rs =
       part_rsrc((const char*)ea.part + (long long)hk * ea.units * SLOT + (long long)t.slot * SLOT, 0x7FFFFFF0u);
   const unsigned stride = (unsigned)t.step * SLOT;
@@ -602,18 +651,18 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     return __builtin_amdgcn_raw_buffer_load_b64(rs, part * stride + ML + (unsigned)r * 8u, 0, kCpolSc1);
   };
 
-  if (!__any(again)) {
+  if (kg == 0 && !__any(again)) {
     if (any_bad) l = __builtin_nanf("");
     if (t.parts > 1) {
       if (R0 / ea.G < t.s.nq) {
-        const unsigned at = (unsigned)t.part * stride + (unsigned)(wave * 32 * HD * 4) + (unsigned)(tid2 & 63) * 16u;
+        const unsigned at = (unsigned)t.part * stride + (unsigned)(rg * 32 * HD * 4) + (unsigned)(tid2 & 63) * 16u;
 #pragma unroll
         for (int d = 0; d < G::ND; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             st_coherent(f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]}, rs,
                         at + (unsigned)(d * 4 + i) * 1024u);
-        if (h2 == 0) st_ml((unsigned)t.part, wave * 32 + (tid2 & 31), m, l);
+        if (h2 == 0) st_ml((unsigned)t.part, rg * 32 + (tid2 & 31), m, l);
       }
     } else {
       // a row that sees no key is zero
@@ -691,11 +740,11 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
         const int d = lane * E + e;
         __builtin_amdgcn_raw_buffer_store_b32(
             bitcast<uint32_t>(o[e]), rs,
-            (unsigned)t.part * stride + (unsigned)(wave * 32 * HD * 4) +
+            (unsigned)t.part * stride + (unsigned)(rg * 32 * HD * 4) +
                 (unsigned)(((d / 32) * 4 + (d % 32) / 8) * 256 + (r + 32 * ((d % 8) / 4)) * 4 + d % 4) * 4u,
             0, kCpolSc1);
       }
-      if (lane == 0) st_ml((unsigned)t.part, wave * 32 + r, mr, lr);
+      if (lane == 0) st_ml((unsigned)t.part, rg * 32 + r, mr, lr);
     } else {
       uint16_t* out = (uint16_t*)ea.o + (long long)(t.s.q0 + i) * ea.ot + hq * ea.oh + lane * E;
       const bool none = seen(ea, t.s, i) == 0;
@@ -725,7 +774,7 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
     __syncthreads();
     return r;
   };
-  const int sets = min(4, (int)(((long long)(t.s.nq - 1) * ea.G + ea.G - (long long)t.tile * ROWS + 31) / 32));
+  const int sets = min(ROWS / 32, (int)(((long long)(t.s.nq - 1) * ea.G + ea.G - (long long)t.tile * ROWS + 31) / 32));
   // parts first, first + by, ... (n): to the output, or in place of the first
   auto join = [&](int first, int by, int n, bool final) {
     for (int w = wave; w < sets * G::ND; w += 4) {
@@ -804,21 +853,20 @@ __global__ __launch_bounds__(kPromptThreads, HD == 64 ? 4 : HD == 128 ? 3 : 2) v
 // rows, a thread four, so that the whole chip reads the parts.  (In the kernel above one workgroup
 // would read a tile's: 512 tokens over 6000 keys 86 us against 68 so; an 8192-token prompt's 250
 // tiles of two parts 272 against 304.)
-template <typename T, int HD>
+template <typename T, int HD, int ROWS>
 __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a, int per) {
-  constexpr int ROWS = kPromptRows;
   constexpr int SETS = ROWS / 32, ND = HD / 32;
   const int tid = (int)threadIdx.x, lane = tid & 63;
   const int runs = ND / per;  // workgroups of a row set, `per` 32-wide blocks each
   const int d0 = (int)blockIdx.x % runs * per, set = (int)blockIdx.x / runs % SETS, u = (int)blockIdx.x / (runs * SETS);
   const int hk = u % a.HKV;
   Tile t;
-  if (!find_tile<false>(a, u / a.HKV, t)) return;
+  if (!find_tile<ROWS, false>(a, u / a.HKV, t)) return;
   t.uniform();
   const int R = t.tile * ROWS + set * 32 + (lane & 31), i = R / a.G;
   if (t.parts == 1 || i >= t.s.nq) return;
-  const long long sf = prompt_slot_floats(HD) * t.step;
-  const float* p0 = a.part + ((long long)hk * a.units + t.slot) * prompt_slot_floats(HD);
+  const long long sf = prompt_slot_floats(HD, ROWS) * t.step;
+  const float* p0 = a.part + ((long long)hk * a.units + t.slot) * prompt_slot_floats(HD, ROWS);
   const float* ml = p0 + ROWS * HD + (set * 32 + (lane & 31)) * 2;
   uint16_t* out = (uint16_t*)a.o + (long long)(t.s.q0 + i) * a.ot + (hk * a.G + (R - i * a.G)) * a.oh;
   const bool some = seen(a, t.s, i) > 0;
@@ -852,29 +900,31 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const Promp
   }
 }
 
-template <typename T, int HD, bool Q8, bool PAGED>
+template <typename T, int HD, bool Q8, bool PAGED, int KG>
 hipError_t prompt_go(const PromptArgs& a, hipStream_t st) {
-  const size_t lds = (size_t)prompt_lds<HD, Q8>();
-  auto kern = prompt_kernel<T, HD, Q8, PAGED>;
+  constexpr int ROWS = kPromptRows / KG;
+  const size_t lds = (size_t)prompt_lds<HD, Q8, KG>();
+  auto kern = prompt_kernel<T, HD, Q8, PAGED, KG>;
   static std::atomic<uint64_t> done{0};
   const hipError_t e = allow_lds((const void*)kern, lds, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3(grid_of(a.HKV, a.units)), dim3(kPromptThreads), lds, st, a);
   if (a.target > 0 && a.join_apart) {
-    const int sets = a.tiles * a.HKV * (kPromptRows / 32);
+    const int sets = a.tiles * a.HKV * (ROWS / 32);
     int per = 1;  // at most about as many workgroups as run at once
     while (per < HD / 32 && sets * (HD / 32 / per) > 2048) per *= 2;
-    hipLaunchKernelGGL((prompt_join_kernel<T, HD>), dim3((unsigned)(sets * (HD / 32 / per))), dim3(kPromptThreads), 0,
-                       st, a, per);
+    hipLaunchKernelGGL((prompt_join_kernel<T, HD, ROWS>), dim3((unsigned)(sets * (HD / 32 / per))),
+                       dim3(kPromptThreads), 0, st, a, per);
   }
   return hipGetLastError();
 }
 
 template <typename T, int HD>
 hipError_t prompt_src(const PromptArgs& a, hipStream_t st) {
-  if (!a.kv.table) return prompt_go<T, HD, false, false>(a, st);
-  if (a.kv.k.s) return prompt_go<T, HD, true, true>(a, st);
-  return prompt_go<T, HD, false, true>(a, st);
+  if (a.kv.table && a.kv.k.s) return prompt_go<T, HD, true, true, 1>(a, st);
+  if (a.kv.table) return a.rows == kPromptRows ? prompt_go<T, HD, false, true, 1>(a, st)
+                                               : prompt_go<T, HD, false, true, 2>(a, st);
+  return a.rows == kPromptRows ? prompt_go<T, HD, false, false, 1>(a, st) : prompt_go<T, HD, false, false, 2>(a, st);
 }
 
 template <typename T>
