@@ -11,13 +11,17 @@
  *
  * Strides are in elements; the last axis (hd values) is contiguous.  Every 16-bit tensor
  * is 16-byte aligned with strides that are multiples of 8; int8 tensors have strides that
- * are multiples of 16.  hd is 64, 128 or 256.  Lengths, page tables, slots and positions are
+ * are multiples of 16.  hd is 64, 128 or 256; a key head has at most 64 query heads, a call
+ * at most 65536 query heads, 2^24 - 1 tokens and 65536 sequences, a sequence 2^30 keys.  Lengths, page tables, slots and positions are
  * read on the device:
- *   - a slot below 0 or past the cache stores nothing (a padded row);
+ *   - a slot below 0 or past the cache stores nothing (a padded row); the others of a call
+ *     differ: what a slot given twice holds is of no one token;
  *   - kv_len below 0 counts as 0, above what the table's row holds as that;
  *   - a page outside 0 .. num_pages - 1 in front of a sequence's end makes NaN of every
  *     output that sees a key of it, and maybe of others of that sequence (no memory outside
  *     the cache is read);
+ *   - a scale of an int8 cache that is not finite makes numbers of no output that sees its
+ *     key; elsewhere infinities and NaN go through the formulas;
  *   - row bounds (cu) are clamped to the rows there are, and query bounds that fall count as the
  *     highest before them.
  */

@@ -38,7 +38,10 @@ int status(const char* fn, hipError_t e) {
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-constexpr int kMaxRows = 1 << 24;             // tokens of a call (rows of a key head stay below 2^31)
+constexpr int kMaxRows = (1 << 24) - 1;       // tokens of a call (rows of a key head stay below 2^31), and its
+                                              // workgroups (a launch has less than 2^32 threads)
+constexpr int kMaxHeads = 1 << 16;
+constexpr int kMaxSeqs = 1 << 16;             // sequences of a call: every workgroup scans them for its own
 constexpr int kMaxGroup = 64;                 // query heads of a key head
 constexpr long long kMaxKeys = 1LL << 30;     // keys of a sequence
 constexpr long long kMaxTokenStride = 1LL << 26;  // eight rows' offset stays in 32 bits
@@ -64,6 +67,7 @@ int check_heads(const char* fn, int hq, int hkv, int hd, int dtype) {
     return fail(QLIN_ERR_INVALID, "%s: %d query heads must be a multiple of %d key heads", fn, hq, hkv);
   if (hq / hkv > kMaxGroup)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d query heads to a key head", fn, kMaxGroup);
+  if (hq > kMaxHeads) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d query heads", fn, kMaxHeads);
   if (hd != 64 && hd != 128 && hd != 256)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: head size %d (need 64, 128 or 256)", fn, hd);
   if (dtype != QLIN_BF16 && dtype != QLIN_F16)
@@ -73,6 +77,16 @@ int check_heads(const char* fn, int hq, int hkv, int hd, int dtype) {
 
 int check_apart(const char* fn, const void* q, const void* out) {
   if (q == out) return fail(QLIN_ERR_INVALID, "%s: out must not be q (queries are read while others' outputs are written)", fn);
+  return QLIN_OK;
+}
+
+int check_seqs(const char* fn, int B) {
+  if (B > kMaxSeqs) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d sequences", fn, kMaxSeqs);
+  return QLIN_OK;
+}
+
+int check_grid(const char* fn, long long workgroups) {
+  if (workgroups > kMaxRows) return fail(QLIN_ERR_UNSUPPORTED, "%s: too many rows for one launch", fn);
   return QLIN_OK;
 }
 
@@ -189,7 +203,10 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   // less than where it has not)
   a.shortest = tiles * a.HKV <= kPromptFewTiles ? 8 : tiles * a.HKV <= kPromptJoinApart ? 12 : 16;
   a.join_apart = tiles * a.HKV <= kPromptJoinApart;
-  a.units = (int)(tiles + (target ? (2 * target + a.HKV - 1) / a.HKV + 2 : 0));
+  const long long units = tiles + (target ? (2 * target + a.HKV - 1) / a.HKV + 2 : 0);
+  // (the grid is rounded up to the XCDs; few key heads share them)
+  QA_TRY(check_grid(fn, units * a.HKV + 8));
+  a.units = (int)units;
   a.part = (float*)part;
   a.cnt = (unsigned*)ws;
   return QLIN_OK;
@@ -269,8 +286,8 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void*
   QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
   QA_TRY(check_scale(fn, scale));
   if (T == 0 || B == 0) return QLIN_OK;
-  if (T > kMaxRows || Tk > kMaxRows || B > kMaxRows)
-    return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens or sequences", fn, kMaxRows);
+  if (T > kMaxRows || Tk > kMaxRows) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens", fn, kMaxRows);
+  QA_TRY(check_seqs(fn, B));
   if (!cu_q || !cu_k) return fail(QLIN_ERR_INVALID, "%s: null row bounds", fn);
   if (!aligned(cu_q, 4) || !aligned(cu_k, 4))
     return fail(QLIN_ERR_UNSUPPORTED, "%s: row bounds must be 4-byte aligned", fn);
@@ -304,8 +321,8 @@ int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const
   QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
   QA_TRY(check_scale(fn, scale));
   if (T == 0 || B == 0) return QLIN_OK;
-  if (T > kMaxRows || B > kMaxRows)
-    return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens or sequences", fn, kMaxRows);
+  if (T > kMaxRows) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens", fn, kMaxRows);
+  QA_TRY(check_seqs(fn, B));
   if (!cu_q) return fail(QLIN_ERR_INVALID, "%s: null row bounds", fn);
   if (!aligned(cu_q, 4)) return fail(QLIN_ERR_UNSUPPORTED, "%s: row bounds must be 4-byte aligned", fn);
   QA_TRY(check_tensor(fn, "q", q, 2, hd, T, q_token, q_heads, q_head, false));
@@ -331,7 +348,7 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
   QA_TRY(check_scale(fn, scale));
   if (B == 0) return QLIN_OK;
-  if (B > kMaxRows / kv_heads) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d rows", fn, kMaxRows);
+  QA_TRY(check_seqs(fn, B));
   QA_TRY(check_tensor(fn, "q", q, 2, hd, B, q_seq, q_heads, q_head, false));
   QA_TRY(check_tensor(fn, "out", out, 2, hd, B, o_seq, q_heads, o_head, true));
   QA_TRY(check_apart(fn, q, out));
@@ -357,6 +374,7 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   // without room for the parts (very many sequences) every sequence is one unit
   if ((target + B + 2) * hg * slot > (long long)avail || B * hg * kDecodeCounters * 4 > (long long)counter_bytes())
     target = 0;
+  QA_TRY(check_grid(fn, (target + B + 2) * hg));
   a.target = (int)target;
   a.few = (int)std::min(std::max(1LL, few / hg), std::max(1LL, target));
   a.units = (int)(target + B + (target ? 2 : 0));  // (two for what the device's estimate rounds)

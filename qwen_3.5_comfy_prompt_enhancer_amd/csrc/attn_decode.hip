@@ -280,9 +280,16 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
 #pragma unroll
       for (int i = 0; i < 4; ++i) t[4 * h + i] = (Q8 ? S[h][i] * ks[h][i] : S[h][i]) * a.c;
     if (blk * kDecodeBlock + kDecodeBlock > len) {
+      // (places behind the last key hold it again: its value may be infinite, which times zero is
+      // no number)
 #pragma unroll
       for (int s = 0; s < 8; ++s)
-        if (blk * kDecodeBlock + 16 * (s / 4) + 4 * g + s % 4 >= len) t[s] = kNegInf;
+        if (blk * kDecodeBlock + 16 * (s / 4) + 4 * g + s % 4 >= len) {
+          t[s] = kNegInf;
+          if constexpr (Q8) vs[s / 4][s % 4] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < VC; ++c) vr[s][c] = VReg{};
+        }
     }
     float mx = t[0];
 #pragma unroll

@@ -178,8 +178,8 @@ def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_ca
     q_out [T, q_heads, hd] and k_out [T, kv_heads, hd] (optional with a cache) may be q
     and k themselves.  With k_cache / v_cache, token t's key and v [T, kv_heads, hd] go to
     slot slots[t] = page * page_size + place (int32 or int64; a negative slot, or one past
-    the cache, stores nothing; a slot given twice holds one of the two, whole or mixed by
-    head).  An int8 cache gets codes round_half_away(y / s) with `s = max(amax / 127,
+    the cache, stores nothing; the others must differ: what a slot given twice holds is of
+    no one token).  An int8 cache gets codes round_half_away(y / s) with `s = max(amax / 127,
     1e-8)` of each token's head in k_s / v_s.  Returns q_out."""
     T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3:

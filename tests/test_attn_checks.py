@@ -109,7 +109,8 @@ def _decode(A, **kw):
     (dict(table=None), "null page table"), (dict(kv_len=None), "null page table"), (dict(kv_len=FAKE + 2), "4-byte"),
     (dict(mp=-1), "negative"), (dict(mp=1 << 28), "keys a sequence"), (dict(ws=None), "workspace"),
     (dict(nws=1 << 20), "workspace"), (dict(ws=FAKE + 8), "256-byte"), (dict(B=1 << 24), "more than"),
-    (dict(qs=1 << 30), "above"), (dict(out=FAKE), "must not be q"),
+    (dict(B=(1 << 16) + 1), "more than 65536 sequences"), (dict(hq=1 << 17, hkv=1 << 16), "more than 65536 query heads"),
+    (dict(B=1 << 16, hq=512, hkv=512), "too many rows"), (dict(qs=1 << 30), "above"), (dict(out=FAKE), "must not be q"),
 ])
 def test_decode_refusals(A, bad, text):
     rc, msg = _decode(A, **bad)
@@ -153,7 +154,8 @@ PROMPT = dict(q=FAKE, qt=512, qh=64, k=FAKE, kt=256, kh=64, v=FAKE, vt=256, vh=6
     (dict(T=-1), "negative"), (dict(T=1 << 25), "more than"), (dict(cu=None), "null row bounds"),
     (dict(ck=FAKE + 1), "4-byte"), (dict(k=None), "null k"), (dict(v=FAKE + 4), "v must be 16-byte"),
     (dict(ot=8), "rows of out overlap"), (dict(ws=None), "workspace"), (dict(hd=32), "head size"),
-    (dict(scale=-1.0), "scale"), (dict(kt=1 << 27), "above"),
+    (dict(scale=-1.0), "scale"), (dict(kt=1 << 27), "above"), (dict(B=(1 << 16) + 1), "more than 65536 sequences"),
+    (dict(T=(1 << 24) - 1, hq=512, hkv=8), "too many rows"),
 ])
 def test_prompt_refusals(A, bad, text):
     qlin, L = _lib(A)

@@ -78,3 +78,34 @@ def test_repeats_are_the_same_bits():
     a = _run([9001, 40, 0, 3000], 8, 2, 256, BF, seed=12)
     for _ in range(5):
         assert torch.equal(a, _run([9001, 40, 0, 3000], 8, 2, 256, BF, seed=12))
+
+
+@pytest.mark.parametrize("n", [1, 37, 5000])
+@pytest.mark.parametrize("int8", [False, True])
+def test_an_infinite_value_is_of_its_own_column(n, int8):
+    """The last key's place is taken again behind it: its infinity must not meet a weight of zero
+    there."""
+    from qwen35_amd.kernels import attention as A
+    table, pages = R.pages_of([n], 64, 2, n, "cuda")
+    c = R.cache(pages, 64, 2, 128, BF, n + 1, int8)
+    last = (int(table[0, (n - 1) // 64]), (n - 1) % 64)
+    rest = torch.ones((2, 128), dtype=torch.bool, device="cuda")
+    if int8:
+        c[3][last][0] = torch.inf
+        rest[0] = False
+    else:
+        c[1][last][1, 77] = torch.inf
+        rest[1, 77] = False
+    q = torch.randn((1, 8, 128), device="cuda").to(BF)
+    out = torch.empty_like(q)
+    kv_len = torch.tensor([n], dtype=torch.int32, device="cuda")
+    A.attn_decode(q, c[0], c[1], table, kv_len, out, k_s=c[2], v_s=c[3])
+    k, v = R.gathered(c, table, 0, n)
+    rest = rest.repeat_interleave(4, 0)[None]
+    if int8:
+        assert not out[~rest].isfinite().any()
+    else:
+        assert (out[~rest] == torch.inf).all()
+    seen = torch.ones((1, n), dtype=torch.bool, device="cuda")
+    ref, tol = R.attend(q, k, v, 128 ** -0.5, seen, BF, 2.0 ** -16 if int8 else None)
+    R.check(out[rest], ref[rest], tol[rest])

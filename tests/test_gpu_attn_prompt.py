@@ -134,6 +134,22 @@ def test_a_masked_key_has_no_part_whatever_it_holds():
         assert out[bad, 4:].isfinite().all()
 
 
+@pytest.mark.parametrize("nq,nk", [(1, 1), (3, 37), (90, 90), (40, 3000)])
+def test_an_infinite_value_is_of_its_own_column(nq, nk):
+    """The last key's place is taken again behind it: its infinity must not meet a weight of zero
+    there."""
+    def spoil(q, k, v):
+        v[-1, 1, 77] = torch.inf
+
+    out, q, k, v = _packed([nq], 8, 2, 128, BF, nk=[nk], seed=14, spoil=spoil, causal=False)
+    assert (out[:, 4:, 77] == torch.inf).all()
+    seen = torch.ones((nq, nk), dtype=torch.bool, device="cuda")
+    ref, tol = R.attend(q, k, v, 128 ** -0.5, seen, BF)
+    rest = torch.ones_like(ref, dtype=torch.bool)
+    rest[:, 4:, 77] = False
+    R.check(out[rest], ref[rest], tol[rest])
+
+
 def test_a_score_of_minus_infinity_is_no_weight():
     def spoil(q, k, v):
         k[:40, :, 0] = -torch.inf
