@@ -127,7 +127,8 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
   int start = 0;
   const Seq first = seq_of(a, 0, start);
   const int start1 = start;
-  int chunk = 1 << 30;
+  constexpr int kUncut = 1 << 30;
+  int chunk = kUncut;
   if (a.target > 0) {
     float w = 0.0f, longest = 0.0f;  // (an estimate; the same for all workgroups)
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -144,6 +145,37 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
     if (longest >= 1.5f * c) chunk = (int)fminf(c, 1e9f);
     else if (!UNITS) return false;  // (nothing to join)
   }
+  auto take = [&](const Seq& s, int b0, int at, int nt, int rank, int part) {
+    r.b = b0 + at;
+    r.s.q0 = lane_value(s.q0, at);
+    r.s.nq = lane_value(s.nq, at);
+    r.s.k0 = lane_value(s.k0, at);
+    r.s.nk = lane_value(s.nk, at);
+    r.part = part;
+    r.tile = nt - 1 - rank;
+    r.step = nt;
+    r.chunk = chunk;
+    const int last = min((int)(((long long)(r.tile + 1) * ROWS - 1) / a.G), r.s.nq - 1);
+    r.nblk = (seen(a, r.s, last) + kPromptBlock - 1) / kPromptBlock;
+    r.parts = max(1, (r.nblk + chunk - 1) / chunk);
+    return r.part < r.parts;
+  };
+  if (UNITS && chunk == kUncut && a.B > 1 && a.B <= 64) {
+    const int tiles = tiles_of(first);
+    auto before = [&](int rank) { return lane_value(wave_scan(min(tiles, rank)), 63); };
+    int lo = 0, hi = lane_value(wave_scan_max(tiles), 63);  // before(lo) <= u < before(hi)
+    if (u >= before(hi)) return false;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before(mid) <= u) lo = mid;
+      else hi = mid;
+    }
+    const uint64_t have = __ballot(tiles > lo);
+    const int mine = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0u));
+    const int at = __builtin_ctzll(have & __ballot(mine == u - before(lo)));
+    r.slot = r.index = 0;  // (of parts, which there are none of)
+    return take(first, 0, at, lane_value(tiles, at), lo, 0);
+  }
   int ubase = 0, tbase = 0;
   start = start1;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -154,25 +186,13 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
     const int usum = lane_value(ue, 63), tsum = lane_value(te, 63);
     if (u < (UNITS ? ubase + usum : tbase + tsum)) {
       const int at = __builtin_ctzll(__ballot((UNITS ? ubase + ue : tbase + te) > u));
-      r.b = b0 + at;
-      r.s.q0 = lane_value(s.q0, at);
-      r.s.nq = lane_value(s.nq, at);
-      r.s.k0 = lane_value(s.k0, at);
-      r.s.nk = lane_value(s.nk, at);
       const int nt = lane_value(tiles, at), mp = lane_value(most, at);
       const int u0 = ubase + lane_value(ue, at) - nt * mp;
       const int t0 = tbase + lane_value(te, at) - nt;
       const int rank = UNITS ? (u - u0) % nt : u - t0;
-      r.part = UNITS ? (u - u0) / nt : 0;
-      r.tile = nt - 1 - rank;
       r.index = t0 + rank;
       r.slot = u0 + rank;
-      r.step = nt;
-      r.chunk = chunk;
-      const int last = min((int)(((long long)(r.tile + 1) * ROWS - 1) / a.G), r.s.nq - 1);
-      r.nblk = (seen(a, r.s, last) + kPromptBlock - 1) / kPromptBlock;
-      r.parts = max(1, (r.nblk + chunk - 1) / chunk);
-      return r.part < r.parts;
+      return take(s, b0, at, nt, rank, UNITS ? (u - u0) / nt : 0);
     }
     ubase += usum;
     tbase += tsum;
