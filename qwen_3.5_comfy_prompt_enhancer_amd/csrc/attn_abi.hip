@@ -190,19 +190,25 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   if (const char* e = getenv("QLIN_PROMPT_UNITS")) {  // for tuning runs
     if (atoi(e) >= 0) target = atoi(e);
   }
-  const long long tiles = (long long)a.T * a.G / a.rows + a.B;
+  const long long tiles = (long long)a.T * a.G / a.rows + a.B, all = tiles * a.HKV;
   const long long slot = prompt_slot_floats(hd, a.rows) * 4;
-  if (max_keys <= kPromptNoCut) target = 0;
+  // A cut costs about as much as seven blocks, and gives less where most of the chip has a tile
+  // already: so many blocks it has to take off the longest tile (128-row tiles; uncut / cut: 192
+  // of 32 blocks 41 / 41 us, 188 of 47 56 / 48; 512 of 64 89 / 104, of 128 165 / 168, 534 of up to
+  // 125 158 / 148, 314 of 157 171 / 129).
+  a.shortest = all <= kPromptFewTiles ? 8 : all <= kPromptJoinApart ? 12 : 16;
+  a.gain = all <= kPromptFewTiles ? 4 : all <= kPromptJoinApart ? 20 : 52;
+  if (max_keys < (long long)(a.shortest + a.gain) * kPromptBlock) target = 0;
   // every unit of a key head has a slot: at most 2 target / HKV + tiles of them (and two more for
   // what the device's 32-bit estimate rounds)
   target = std::min(target, ((long long)avail / slot / a.HKV - tiles - 3) * a.HKV / 2);
-  if (target <= a.HKV || tiles * a.HKV * kPromptCounters * 4 > (long long)counter_bytes()) target = 0;
+  if (target <= a.HKV || all * kPromptCounters * 4 > (long long)counter_bytes()) target = 0;
   a.target = (int)target;
   a.tiles = (int)tiles;
-  // (a cut costs about as much as seven blocks; where most of the chip has a tile already it gives
-  // less than where it has not)
-  a.shortest = tiles * a.HKV <= kPromptFewTiles ? 8 : tiles * a.HKV <= kPromptJoinApart ? 12 : 16;
-  a.join_apart = tiles * a.HKV <= kPromptJoinApart;
+  // (not where sequences of the average length are too short for a cut: a launch that finds nothing
+  // to join costs 3 us, but joins the 192 tiles of three 1000-token prompts in 5 us less)
+  const long long average = a.kv.table ? max_keys : max_keys / a.B;
+  a.join_apart = all <= kPromptJoinApart && average >= (long long)(a.shortest + a.gain) * kPromptBlock * 3 / 4;
   const long long units = tiles + (target ? (2 * target + a.HKV - 1) / a.HKV + 2 : 0);
   // (the grid is rounded up to the XCDs; few key heads share them)
   QA_TRY(check_grid(fn, units * a.HKV + 8));

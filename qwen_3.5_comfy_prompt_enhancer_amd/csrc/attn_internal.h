@@ -102,6 +102,7 @@ struct PromptArgs {
   float c;                // scale * log2(e)
   int target;             // work units to cut the keys into; 0: no cut
   int shortest;           // blocks of the shortest cut
+  int gain;               // blocks that a cut has to take off the longest tile
   int units;              // units per key head: the grid's bound
   int rows;               // rows of a tile: kPromptRows, or half as many with two key groups
   int tiles;              // row tiles per key head at most
@@ -110,7 +111,6 @@ struct PromptArgs {
   unsigned* cnt;          // arrival counters of each tile, zero between calls
 };
 constexpr int kPromptBlock = 32;     // keys of a step
-constexpr int kPromptNoCut = 11 * kPromptBlock;  // keys that are never cut (below 1.5 of the shortest cut)
 constexpr int kPromptFewTiles = 96;  // tiles of all key heads up to which short cuts pay
 constexpr int kPromptHalves = 272;   // halved tiles of all key heads up to which tiles are halved
 constexpr int kPromptFill = 3000;    // (tile, block) pairs that fill the chip with whole tiles

@@ -140,9 +140,10 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
     }
     w = lane_value(wave_scan(w), 63);
     longest = wave_max(longest);
-    // a cut that takes less than a third off the longest tile costs more than it gives
+    // a cut that takes less than a third off the longest tile, or too few blocks, costs more than
+    // it gives
     const float c = fmaxf(ceilf(w * (float)a.HKV / (float)a.target), (float)a.shortest);
-    if (longest >= 1.5f * c) chunk = (int)fminf(c, 1e9f);
+    if (longest >= fmaxf(1.5f * c, c + (float)a.gain)) chunk = (int)fminf(c, 1e9f);
     else if (!UNITS) return false;  // (nothing to join)
   }
   auto take = [&](const Seq& s, int b0, int at, int nt, int rank, int part) {

@@ -101,6 +101,18 @@ def test_long_prompt_is_cut_and_joined():
     _packed([1500], 2, 1, 64, BF, seed=6)
 
 
+def test_many_tiles_are_cut_and_joined_by_their_last_part():
+    _packed([4200, 0, 1700, 33], 8, 2, 256, BF, seed=15, tail=5)
+    _packed([5000, 700], 16, 2, 64, FP, seed=16)
+    _packed([17] * 70 + [4500], 8, 2, 128, BF, seed=17)
+
+
+def test_ragged_batches_in_one_piece():
+    _packed([900, 3, 0, 899, 450, 64, 1, 700], 8, 2, 256, BF, seed=18, tail=3)
+    _packed([(i * 37) % 400 for i in range(64)], 16, 4, 64, FP, seed=19)
+    _packed([(i * 37) % 400 for i in range(65)], 16, 4, 64, FP, seed=19, causal=False)
+
+
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("hd,dt", [(64, BF), (128, FP), (256, BF), (256, FP)])
 @pytest.mark.parametrize("page", [16, 64, 256])
