@@ -170,14 +170,14 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   size_t avail;
   QA_TRY(workspace_parts(fn, ws, ws_bytes, &part, &avail));
   // Units: about as many as run at once (two, three or four workgroups a CU by head size), fewer
-  // where their sums are the larger; 8192 tokens, 256 values, 320 / 384 / 448 / 512 / 640 units: 288 / 266 /
-  // 258 / 264 / 283 us.
+  // where their sums are the larger; 8192 tokens, 256 values, 384 / 448 / 512 / 640 units: 315 (not
+  // cut) / 258 / 265 / 283 us.
   a.rows = kPromptRows;
   long long target = hd == 256 ? 448 : hd == 128 ? 512 : 640;
-  // Few tiles (of 16-bit keys) are halved, two groups of waves sharing their keys: 512 tokens 20.6
-  // -> 18.6 us, four prompts of 512 27.3 -> 19.4.  Beyond a halved tile for each CU, or with work
+  // Few tiles (of 16-bit keys) are halved, two groups of waves sharing their keys: 512 tokens 20.8
+  // -> 18.6 us, four prompts of 512 24.7 -> 19.9.  Beyond a halved tile for each CU, or with work
   // enough to fill the chip with whole ones (by what the host knows of it), that only moves twice the
-  // keys (2048 tokens 44.8 -> 50.0, four chunks of 700 over 3000 keys 69 -> 94); sequences of few
+  // keys (2048 tokens 44.5 -> 49.9, four chunks of 700 over 3000 keys 69 -> 94); sequences of few
   // rows leave half of a whole tile empty.  A CU then holds one workgroup, and units stay below
   // the CUs (100-token chunks, 192 / 256 units: 25.5 / 35.4).
   const long long rows = (long long)a.T * a.G, halves = (rows * 2 / kPromptRows + a.B) * a.HKV;
@@ -310,7 +310,7 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void*
   a.kv.k = PagedTensor{const_cast<void*>(k), 0, k_token, k_head, nullptr, 0, 0, 0};
   a.kv.v = PagedTensor{const_cast<void*>(v), 0, v_token, v_head, nullptr, 0, 0, 0};
   a.kv.cu = cu_k, a.kv.rows = Tk;
-  a.cu = cu_q, a.T = T, a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
+  a.cu = cu_q, a.T = T, a.B = B, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
   QA_TRY(plan_prompt(fn, a, hd, Tk, workspace, workspace_bytes));
   return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
@@ -338,7 +338,7 @@ int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const
   QA_TRY(check_paged(fn, cache, table, table_stride, max_pages, kv_len, kv_heads, hd, dtype, a.kv));
   a.q = q, a.qt = q_token, a.qh = q_head;
   a.o = out, a.ot = o_token, a.oh = o_head;
-  a.cu = cu_q, a.T = T, a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
+  a.cu = cu_q, a.T = T, a.B = B, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
   QA_TRY(plan_prompt(fn, a, hd, (long long)max_pages * cache->page, workspace, workspace_bytes));
   return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
@@ -365,7 +365,7 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   QA_TRY(workspace_parts(fn, workspace, workspace_bytes, &part, &avail));
   a.q = q, a.qb = q_seq, a.qh = q_head;
   a.o = out, a.ob = o_seq, a.oh = o_head;
-  a.B = B, a.HQ = q_heads, a.HKV = kv_heads, a.G = q_heads / kv_heads;
+  a.B = B, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.gb = (a.G + 15) / 16;
   a.c = scale * 1.44269504088896340736f;
   const long long hg = (long long)kv_heads * a.gb;

@@ -112,8 +112,7 @@ __device__ __forceinline__ N lane_value(N v, int at) {
   return bitcast<N>(__builtin_amdgcn_readlane(bitcast<int>(v), at));
 }
 
-// 2^x, and the factor between two running maxima (in powers of two) of which the first may be
-// -inf: nothing was seen yet, or scores of -inf alone.
+// 2^x; of -inf (nothing seen yet, or scores of -inf alone) zero.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Lets a kernel take `bytes` of dynamic LDS on the current device; `done` holds a bit for each

@@ -71,7 +71,7 @@ struct DecodeArgs {
   void* o;
   long long ob, oh;
   KvSrc kv;
-  int B, HQ, HKV, G;      // G = HQ / HKV
+  int B, HKV, G;          // G: query heads of a key head
   int gb;                 // groups of 16 query heads of a key head
   float c;                // scale * log2(e)
   int target;             // most work units of a (key head, group) to cut into; 0: no cut
@@ -84,7 +84,7 @@ struct DecodeArgs {
 __host__ __device__ constexpr int decode_slot_floats(int rows, int hd) { return rows * hd + rows * 4; }
 constexpr int kDecodeBlock = 32;     // keys a wave takes at a time
 constexpr int kDecodeChunk = 4;      // blocks of a unit come in multiples of this (one per wave)
-constexpr int kDecodeLong = 32;     // blocks of a unit up to which fewer units are better
+constexpr int kDecodeLong = 32;      // blocks of a unit up to which fewer units are better
 constexpr int kDecodeGroup = 16;     // units joined at a time
 constexpr int kDecodeCounters = 32;  // counters of a (sequence, key head, group)
 hipError_t launch_decode(const DecodeArgs& a, int dt, int hd, hipStream_t st);
@@ -97,7 +97,7 @@ struct PromptArgs {
   long long ot, oh;
   KvSrc kv;               // table == nullptr: packed keys, sequence b's at kv.cu
   const int* cu;          // [B + 1] rows of q of each sequence
-  int T, B, HQ, HKV, G;
+  int T, B, HKV, G;
   int causal;
   float c;                // scale * log2(e)
   int target;             // work units to cut the keys into; 0: no cut

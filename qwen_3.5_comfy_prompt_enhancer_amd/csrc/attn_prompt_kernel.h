@@ -4,10 +4,10 @@
 //   o[i, h] = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max_i)
 //   over the keys j <= i + Lk - Lq of the row's sequence (all keys where not causal)
 //
-// One pass over the keys with a running maximum and sum.  A workgroup's four waves hold a tile
-// of rows: the tokens' rows of all G query heads of one key head next to each other (row = token
-// G + head), so that a key tile serves G heads and a causal tile spans few tokens.  A wave owns
-// 32 or 64 rows; keys come in blocks of 32 through an LDS ring.
+// One pass over the keys with a running maximum and sum.  A workgroup holds a tile of 128 rows: the
+// tokens' rows of all G query heads of one key head next to each other (row = token G + head), so
+// that a key block serves G heads and a causal tile spans few tokens.  Each of its four waves owns 32
+// rows; keys come in blocks of 32 through an LDS ring of two stages.
 //   * S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs with Q (as the B operand) and O in
 //     registers: a lane holds one row (column of S^T), so its maximum and sum are its own but
 //     for one exchange between the wave's halves, and P^T becomes the B operand of the second
@@ -15,15 +15,31 @@
 //     operand is read.
 //   * K rows are read from LDS as 16-byte operands, V columns by the transposing 8-byte reads.
 //     Both land by 16-byte LDS DMA whose lanes fetch swizzled chunks, so that a read's lanes
-//     meet different banks.  int8 caches pass through registers: code x scale, rounded once to
-//     the queries' type, as a 16-bit cache would have held it.
-//   * With 64 rows a wave, each K and V operand feeds two MFMAs: LDS (128 bytes a clock and CU)
-//     then needs half the time of the MFMAs; with 32 rows as long as they do.
+//     meet different banks (16-bit keys: no bank conflict is counted).
+//   * int8 caches: codes land in a ring of their own and each wave widens its 8 keys to 16-bit whole
+//     numbers (exact) in LDS; a key's scale multiplies its scores, a value's its probability, both
+//     in 32 bits.  P x scale is rounded once for its product (to bf16; for fp16 queries it goes as
+//     the sum of two bf16 numbers, as fp16 may not hold it).
 //   * The sums are rescaled only when a row's maximum has grown by more than 2^8: P stays below
 //     2^8, which both 16-bit types hold with full relative precision.  P is rounded to the
 //     queries' type for its product; its sum, the maximum and O are 32-bit.
-//   * Keys of all tiles are cut into about equal units where there are fewer tiles than the chip
-//     holds; units leave 32-bit partial sums, which the last unit of a tile joins in key order.
+//
+// What bounds it: the MFMAs (of 256 values, 32 of 32 cycles a block and wave), then the softmax's
+// vector work and LDS.  32 rows a wave, operands read three products ahead and two workgroups a CU (256
+// values; three or four of smaller heads) took 310 us for an 8192-token prompt of 8 heads of 256 values
+// where 64 rows a wave, each operand feeding two MFMAs, took 696: two waves a SIMD hide each other's
+// softmax and waits, and a wave of 64 rows has no registers left to read ahead.  With the cuts and the
+// order below 253 us now: 275 Gflop at 1.09 Pflop/s, where an 8192^3 library product reaches 1.20.
+// Even batches that fill the chip reach 1.06 - 1.1 Pflop/s at 256 values, 0.95 at 128, 0.78 at 64
+// (the softmax's work is the same for fewer products), over int8 caches 0.75 - 0.8 and 0.63 (widening
+// takes as many vector instructions as the softmax).
+//
+//   * Where there are fewer or less even tiles than the chip holds, keys of all tiles are cut into
+//     units of about equal length; units leave 32-bit partial sums, which are joined in key order by
+//     the last unit of a tile to arrive, or by a second launch where tiles are few.  512 tokens over
+//     6000 int8 keys: 52 us and 13.5 for the join of 60 MB of parts.
+//   * Few tiles of 16-bit keys are halved (KG = 2): two waves hold 64 rows, the other two the same rows
+//     over every second block, and their sums are added in LDS.
 //
 // A row's masked keys have no part in it whatever they hold: scores are replaced before the
 // maximum, and as zero times a value that is no number is none, a tile whose sums come out
@@ -120,6 +136,9 @@ struct Tile {
 // within a part.  With chunk the average over the workgroups that run at once, long causal
 // prompts then come out even: whole chunks start first, and the workgroup that gets the
 // shortest rest of one part goes on with the longest of the next.
+//
+// Uncut tiles of up to 64 sequences start by rank over all of them, longest first (sequence by
+// sequence: nine ragged prompts of up to 1500 tokens 66.8 us, by rank 61.8).
 template <int ROWS, bool UNITS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int u, Tile& r) {
   auto tiles_of = [&](const Seq& s) { return (int)(((long long)s.nq * a.G + ROWS - 1) / ROWS); };
@@ -872,8 +891,8 @@ void prompt_kernel(const PromptArgs a) {
 
 // The join as a launch of its own, for few tiles cut many times: a workgroup takes 32 values of 32
 // rows, a thread four, so that the whole chip reads the parts.  (In the kernel above one workgroup
-// would read a tile's: 512 tokens over 6000 keys 86 us against 68 so; an 8192-token prompt's 250
-// tiles of two parts 272 against 304.)
+// would read a tile's: 512 tokens over 6000 int8 keys 80 us against 61 so, three prompts of 1000 tokens
+// 44 against 40; above 256 tiles of two or three parts it gives nothing, 148 against 150 for 534.)
 template <typename T, int HD, int ROWS>
 __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a, int per) {
   constexpr int SETS = ROWS / 32, ND = HD / 32;

@@ -11,8 +11,10 @@
 // bits a position of 200000 would leave an error of 0.01 radians.  All else is 32 bits,
 // rounded once, on the store; int8 codes are made of the unrounded values.
 //
-// Bound: bytes for long prompts (each value read and written once), a launch and two
-// dependent memory round trips for a decode step.
+// Bound: a launch and two dependent memory round trips for a decode step (4.8 us for one token of 8 + 2
+// heads of 256 values); for long prompts the bytes (each value read and written once) and, about as
+// much, the vector work of the angles and of int8 codes: 4097 tokens of 16 + 4 heads into an int8
+// cache, 92 MB, in 25 us, 3.7 TB/s where a large copy reaches 5.1.
 #include "attn_dev.h"
 
 namespace qlin {
