@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) am = max(am, bitcast<uint32_t>(y[e]) & 0x7FFFFFFFu);
       const float amf = bitcast<float>(team_max<TEAM>(am));
-      const float s = amf == amf ? fmaxf(amf * (1.0f / 127.0f), 1e-8f) : amf;
+      const float s = amf == amf ? fmaxf(amf / 127.0f, 1e-8f) : amf;
       const float inv = __builtin_amdgcn_rcpf(s);  // (quant_i8 divides where the product is near a tie)
       uint32_t q[2] = {0u, 0u};
 #pragma unroll

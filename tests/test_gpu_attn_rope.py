@@ -154,3 +154,30 @@ def test_empty():
     from qwen35_amd.kernels import attention as A
     q = torch.empty((0, 2, 64), dtype=BF, device="cuda")
     A.qk_norm_rope(q, q, torch.empty(0, dtype=torch.int64, device="cuda"), torch.ones(8, device="cuda"), q, k_out=q)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_codes_of_values_are_the_formulas(hd, dt):
+    """Values are not turned: their scales and codes come out bit for bit, ties included."""
+    from qwen35_amd.kernels import attention as A
+    T, hkv, page = 300, 2, 16
+    q, k, v, g = _inputs(T, 4, hkv, hd, dt, 31)
+    v = v.clone()
+    v[:100, :, 0] = 127 / 64  # scales of a power of two, and values that lie on ties
+    v[:100, :, 1:] = torch.randint(-253, 254, (100, hkv, hd - 1), generator=g, device="cuda").to(dt) / 128
+    v[100:110] = 0
+    pages = -(-T // page)
+    kc, vc = (torch.zeros((pages, page, hkv, hd), dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros((pages, page, hkv), device="cuda") for _ in range(2))
+    slots = torch.randperm(pages * page, generator=g, device="cuda")[:T]
+    A.qk_norm_rope(q, k, torch.arange(T, device="cuda"), torch.ones(16, device="cuda") * 0.1, torch.empty_like(q), v=v,
+                   k_cache=kc, v_cache=vc, slots=slots, k_s=ks, v_s=vs)
+    # quotients in 64 bits, rounded (53 bits are more than twice 24 and two: as divided in 32; torch
+    # multiplies by the reciprocal of a number)
+    x = v.double()
+    s = (x.abs().amax(-1) / 127).float().clamp_min(1e-8)
+    r = (x / s[..., None].double()).float()
+    code = torch.trunc(r + torch.where(r >= 0, 0.5, -0.5)).to(torch.int8)
+    assert torch.equal(vs.view(-1, hkv)[slots], s)
+    assert torch.equal(vc.view(-1, hkv, hd)[slots], code)
