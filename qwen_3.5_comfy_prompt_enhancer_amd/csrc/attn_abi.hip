@@ -205,10 +205,13 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   if (target <= a.HKV || all * kPromptCounters * 4 > (long long)counter_bytes()) target = 0;
   a.target = (int)target;
   a.tiles = (int)tiles;
-  // (not where sequences of the average length are too short for a cut: a launch that finds nothing
-  // to join costs 3 us, but joins the 192 tiles of three 1000-token prompts in 5 us less)
+  // A second launch joins where parts are many (see prompt_join_kernel): not where sequences of the average
+  // length are too short for a cut (a launch that finds nothing to join costs 3 us), nor for halved
+  // tiles of small heads, whose few small parts their last one joins as quickly (1300 tokens, a
+  // launch / the last part: 64 values 15.2 / 13.4 us, 128 20.2 / 18.4, 256 31.8 / 32.8).
   const long long average = a.kv.table ? max_keys : max_keys / a.B;
-  a.join_apart = all <= kPromptJoinApart && average >= (long long)(a.shortest + a.gain) * kPromptBlock * 3 / 4;
+  a.join_apart = all <= kPromptJoinApart && average >= (long long)(a.shortest + a.gain) * kPromptBlock * 7 / 8 &&
+                 (a.kv.table || hd == 256 || a.rows == kPromptRows);
   const long long units = tiles + (target ? (2 * target + a.HKV - 1) / a.HKV + 2 : 0);
   // (the grid is rounded up to the XCDs; few key heads share them)
   QA_TRY(check_grid(fn, units * a.HKV + 8));

@@ -893,6 +893,7 @@ void prompt_kernel(const PromptArgs a) {
 // rows, a thread four, so that the whole chip reads the parts.  (In the kernel above one workgroup
 // would read a tile's: 512 tokens over 6000 int8 keys 80 us against 61 so, three prompts of 1000 tokens
 // 44 against 40; above 256 tiles of two or three parts it gives nothing, 148 against 150 for 534.)
+// Eight parts are in flight, sixteen made few parts dearer (four chunks of 700 over 3000 keys 67 -> 69).
 template <typename T, int HD, int ROWS>
 __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const PromptArgs a, int per) {
   constexpr int SETS = ROWS / 32, ND = HD / 32;
@@ -905,35 +906,48 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(const Promp
   t.uniform();
   const int R = t.tile * ROWS + set * 32 + (lane & 31), i = R / a.G;
   if (t.parts == 1 || i >= t.s.nq) return;
-  const long long sf = prompt_slot_floats(HD, ROWS) * t.step;
-  const float* p0 = a.part + ((long long)hk * a.units + t.slot) * prompt_slot_floats(HD, ROWS);
-  const float* ml = p0 + ROWS * HD + (set * 32 + (lane & 31)) * 2;
+  // a part's place in scalars, this thread's in it: all of a key head's parts lie below 2^31 bytes
+  constexpr unsigned SLOT = (unsigned)prompt_slot_floats(HD, ROWS) * 4u;
+  const __amdgpu_buffer_rsrc_t rs =
+      part_rsrc((const char*)a.part + ((long long)hk * a.units + t.slot) * SLOT, 0x7FFFFFF0u);
+  const unsigned stride = (unsigned)t.step * SLOT;
+  const unsigned ml = (unsigned)(ROWS * HD + (set * 32 + (lane & 31)) * 2) * 4u;
   uint16_t* out = (uint16_t*)a.o + (long long)(t.s.q0 + i) * a.ot + (hk * a.G + (R - i * a.G)) * a.oh;
   const bool some = seen(a, t.s, i) > 0;
   for (int d = d0; d < d0 + per; ++d) {
-    const float* po = p0 + set * 32 * HD + d * 1024 + tid * 4;
+    const unsigned px = (unsigned)(set * 32 * HD + d * 1024 + tid * 4) * 4u;
     f32x4 o = {0, 0, 0, 0};
     float M = kNegInf, l = 0.0f;
-    constexpr int N = 8;  // parts in flight
-    for (int s0 = 0; s0 < t.parts; s0 += N) {
-      f32x4 x[N];
-      float2 y[N];
+    auto add = [&](auto in_flight) __attribute__((always_inline)) {
+      constexpr int N = decltype(in_flight)::value;
+      for (int s0 = 0; s0 < t.parts; s0 += N) {
+        f32x4 x[N];
+        u32x2 y[N];
 #pragma unroll
-      for (int s = 0; s < N; ++s) {
-        const long long at = min(s0 + s, t.parts - 1) * sf;
-        x[s] = *(const f32x4*)(po + at);
-        y[s] = *(const float2*)(ml + at);
-      }
+        for (int s = 0; s < N; ++s) {
+          const unsigned at = (unsigned)min(s0 + s, t.parts - 1) * stride;
+          x[s] = bitcast<f32x4>(__builtin_amdgcn_raw_buffer_load_b128(rs, px, at, 0));
+          y[s] = __builtin_amdgcn_raw_buffer_load_b64(rs, ml, at, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // (no branch: the compiler would move each load behind it, next to its use, and wait for
+        // every part: a 16-token chunk over 30000 keys, 94 parts, 57 us against 32)
 #pragma unroll
-      for (int s = 0; s < N; ++s) {
-        if (s0 + s >= t.parts) break;
-        const float mn = fmaxf(M, y[s].x), ms = mn == kNegInf ? 0.0f : mn;
-        const float e0 = exp2_(M - ms), e1 = exp2_(y[s].x - ms);
-        o = o * e0 + x[s] * e1;
-        l = l * e0 + y[s].y * e1;
-        M = mn;
+        for (int s = 0; s < N; ++s) {
+          const bool more = s0 + s < t.parts;
+          const float pm = more ? bitcast<float>(y[s].x) : kNegInf, pl = more ? bitcast<float>(y[s].y) : 0.0f;
+          const f32x4 po = more ? x[s] : f32x4{0, 0, 0, 0};
+          const float mn = fmaxf(M, pm), ms = mn == kNegInf ? 0.0f : mn;
+          const float e0 = exp2_(M - ms), e1 = exp2_(pm - ms);
+          o = o * e0 + po * e1;
+          l = l * e0 + pl * e1;
+          M = mn;
+        }
       }
-    }
+    };
+    if (t.parts == 2) add(std::integral_constant<int, 2>{});
+    else if (t.parts <= 4) add(std::integral_constant<int, 4>{});
+    else add(std::integral_constant<int, 8>{});
     const float inv = some ? 1.0f / l : 0.0f;
     *(u32x2*)(out + d * 32 + (tid >> 6) * 8 + 4 * (lane >> 5)) =
         u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
