@@ -421,22 +421,29 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
       const unsigned ml = part_ml<HD>(rows) + (unsigned)(f / (HD / 4)) * 16u;
       f32x4 o = {0, 0, 0, 0};
       float M = kNegInf, ls = 0.0f;
-      for (int i0 = 0; i0 < n; i0 += 8) {
-        f32x4 x[8], y[8];
+      constexpr int N = 8;  // parts in flight
+      for (int i0 = 0; i0 < n; i0 += N) {
+        f32x4 x[N];
+        u32x2 y[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
           const unsigned at = (unsigned)(first + min(i0 + i, n - 1) * step) * slot_bytes;
-          x[i] = ld_coherent(rs, at + (unsigned)f * 16u);
-          y[i] = ld_coherent(rs, at + ml);
+          x[i] = bitcast<f32x4>(__builtin_amdgcn_raw_buffer_load_b128(rs, (unsigned)f * 16u, at, kCpolSc1));
+          y[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, ml, at, kCpolSc1);
         }
+        // (no branch: the compiler would move each load behind it, next to its use, and wait for
+        // every part by itself)
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i0 + i >= n) break;
-          const float mn = fmaxf(M, y[i][0]);
+        for (int i = 0; i < N; ++i) {
+          const bool more = i0 + i < n;
+          const float pm = more ? bitcast<float>(y[i].x) : kNegInf, pl = more ? bitcast<float>(y[i].y) : 0.0f;
+          const f32x4 px = more ? x[i] : f32x4{0, 0, 0, 0};
+          const float mn = fmaxf(M, pm);
           const float ms = mn == kNegInf ? 0.0f : mn;
-          const float e0 = exp2_(M - ms), e1 = exp2_(y[i][0] - ms);
-          o = o * e0 + x[i] * e1;
-          ls = ls * e0 + y[i][1] * e1;
+          const float e0 = exp2_(M - ms), e1 = exp2_(pm - ms);
+          o = o * e0 + px * e1;
+          ls = ls * e0 + pl * e1;
           M = mn;
         }
       }
