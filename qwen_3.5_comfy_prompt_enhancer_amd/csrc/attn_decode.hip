@@ -7,8 +7,8 @@
 // cut into units of about the same number of 32-key blocks, so that a ragged batch fills the
 // chip evenly; every workgroup finds its unit from the sequences' lengths on the device.
 // 64 sequences of up to 16384 keys (4 key heads of 128 16-bit values, 1.01 GB) take 182 us, 5.5 TB/s,
-// 8 of up to 8192 (2 of 256, 136 MB) 31 us, 4.4 TB/s, where a copy of 1 GiB reaches 5.1; one of
-// 131072 int8 keys (136 MB) 37 us, 3.7 TB/s, with widening and joins; one of 1000 keys 10 us, the
+// 8 of up to 8192 (2 of 256, 136 MB) 29 us, 4.6 TB/s, where a copy of 1 GiB reaches 5.1; one of
+// 131072 int8 keys (136 MB) 33 us, 4.1 TB/s, with widening and joins; one of 1000 keys 9 us, the
 // latency of lengths, pages, keys and joins one after the other.
 //
 // A workgroup's four waves take blocks in turn.  A block runs without LDS:
@@ -60,8 +60,8 @@ __device__ __forceinline__ bool find_unit(const DecodeArgs& a, int u, Unit& r) {
     total = lane_value(wave_scan(total), 63);
     // one workgroup a CU as long as that makes units of at most kDecodeLong blocks; longer work
     // goes to more of them, which come out more even and keep more loads in flight (8 sequences
-    // of up to 8192 keys, 256 / 512 / 1024 units: 32 / 37 / 35 us; 64 of up to 16384, 256 / 768 /
-    // 1536: 250 / 189 / 183)
+    // of up to 8192 keys, 256 / 512 / 1024 units: 29 / 35 / 33 us; 64 of up to 16384, 256 / 768 /
+    // 1536: 250 / 188 / 181)
     const float few = ceilf(total / (float)a.few);
     const float most = ceilf(total / (float)a.target);
     chunk = max((int)fminf(few <= (float)kDecodeLong ? few : fmaxf((float)kDecodeLong, most), 1e8f), 1);
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
           y[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, ml, at, kCpolSc1);
         }
         // (no branch: the compiler would move each load behind it, next to its use, and wait for
-        // every part by itself)
+        // every part by itself: 1000 keys 10.3 us against 8.8, 32768 of 128 values 27 against 17)
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {

@@ -37,7 +37,7 @@
 //   * Where there are fewer or less even tiles than the chip holds, keys of all tiles are cut into
 //     units of about equal length; units leave 32-bit partial sums, which are joined in key order by
 //     the last unit of a tile to arrive, or by a second launch where tiles are few.  512 tokens over
-//     6000 int8 keys: 52 us and 13.5 for the join of 60 MB of parts.
+//     6000 int8 keys: 52 us and 13 for the join of 60 MB of parts.
 //   * Few tiles of 16-bit keys are halved (KG = 2): two waves hold 64 rows, the other two the same rows
 //     over every second block, and their sums are added in LDS.
 //
