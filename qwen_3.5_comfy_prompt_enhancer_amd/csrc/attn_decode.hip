@@ -28,7 +28,8 @@
 //
 // Waves join through LDS, units of a sequence through memory: the last of 16 units to arrive
 // adds their parts in unit order, the last of those groups adds the groups', so that the result
-// does not depend on the order of arrival and no workgroup reads more than 16 parts.
+// does not depend on the order of arrival and no workgroup reads more than 16 parts (or as many as it
+// takes to keep a sequence's groups within its counters).
 #include "attn_dev.h"
 
 namespace qlin {

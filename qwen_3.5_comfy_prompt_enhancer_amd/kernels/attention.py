@@ -61,6 +61,7 @@ EXPORTS = tuple(_SIGS)
 
 _DT = {torch.bfloat16: C.QLIN_BF16, torch.float16: C.QLIN_F16}
 _WDT = {**_DT, torch.float32: C.QLIN_F32}
+_INTS = (torch.int32, torch.int64)
 _fns: dict = {}
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -120,6 +121,14 @@ def _vector(name, t, n, dtypes=(torch.int32,)):
         raise ValueError(f"{name} must be [{n}], not {list(shape)}")
     if n > 1 and t.stride(0) != 1:
         raise ValueError(f"{name} must be contiguous")
+
+
+def _weight(name, w, hd):
+    """Type code of a norm's weights."""
+    shape, dt = w.shape, _WDT.get(w.dtype)
+    if dt is None or len(shape) != 1 or shape[0] != hd or not w.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{hd}] of bfloat16, float16 or float32")
+    return dt
 
 
 def _table(table, kv_len, B):
@@ -182,22 +191,25 @@ def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_ca
     no one token).  An int8 cache gets codes round_half_away(y / s) with `s = max(amax / 127,
     1e-8)` of each token's head in k_s / v_s.  Returns q_out."""
     T, hq, hd, dt, qt, qh = _queries(q)
-    if k.dim() != 3:
+    kshape = k.shape
+    if len(kshape) != 3:
         raise ValueError("k must be [rows, kv_heads, hd]")
-    dtype, hkv = q.dtype, k.shape[1]
+    dtype, hkv = q.dtype, kshape[1]
     kt, kh = _strides("k", k, T, hkv, hd, dtype)
     qot, qoh = _strides("q_out", q_out, T, hq, hd, dtype)
-    if pos.dim() == 1:
-        pos = pos[None]
-    if pos.dim() != 2 or pos.shape[1] != T:
+    pshape, pst = pos.shape, pos.stride()
+    if len(pshape) == 1:
+        pshape, pst = (1, pshape[0]), (0, pst[0])
+    if len(pshape) != 2 or pshape[1] != T:
         raise ValueError(f"pos must be [{T}] or [axes, {T}]")
-    pos64 = pos.dtype == torch.int64
-    if not pos64 and pos.dtype != torch.int32:
+    pdt, fdt, fshape = pos.dtype, freqs.dtype, freqs.shape
+    pos64 = pdt is torch.int64
+    if not pos64 and pdt is not torch.int32:
         raise ValueError("pos must be int32 or int64")
-    freqs64 = freqs.dtype == torch.float64
-    if freqs.dim() != 1 or not (freqs64 or freqs.dtype == torch.float32) or not freqs.is_contiguous():
+    freqs64 = fdt is torch.float64
+    if len(fshape) != 1 or not (freqs64 or fdt is torch.float32) or not freqs.is_contiguous():
         raise ValueError("freqs must be a contiguous float32 or float64 vector")
-    half, axes = freqs.shape[0], pos.shape[0]
+    half, axes = fshape[0], pshape[0]
     if sections is None:
         if axes != 1:
             raise ValueError(f"{axes} position axes need sections")
@@ -206,24 +218,25 @@ def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_ca
         raise ValueError(f"sections must give one length for each of the {axes} axes")
     if axes > 3:
         raise ValueError("at most 3 position axes")
-    wdt = 0
-    for name, w in (("q_w", q_w), ("k_w", k_w)):
-        if w is not None:
-            if w.dim() != 1 or w.shape[0] != hd or not w.is_contiguous() or w.dtype not in _WDT:
-                raise ValueError(f"{name} must be a contiguous [{hd}] of bfloat16, float16 or float32")
-            if wdt and wdt != _WDT[w.dtype]:
-                raise ValueError("q_w and k_w must share a dtype")
-            wdt = _WDT[w.dtype]
-    kot = koh = vt = vh = slots64 = 0
+    wdt = qwp = kwp = 0
+    if q_w is not None:
+        wdt, qwp = _weight("q_w", q_w, hd), q_w.data_ptr()
+    if k_w is not None:
+        kdt, kwp = _weight("k_w", k_w, hd), k_w.data_ptr()
+        if wdt and wdt != kdt:
+            raise ValueError("q_w and k_w must share a dtype")
+        wdt = kdt
+    kop = kot = koh = vp = vt = vh = sp = slots64 = 0
     cache = None
     if k_out is not None:
         kot, koh = _strides("k_out", k_out, T, hkv, hd, dtype)
+        kop = k_out.data_ptr()
     if k_cache is not None or v_cache is not None or slots is not None:
         if k_cache is None or v_cache is None or v is None or slots is None:
             raise ValueError("a cache takes k_cache, v_cache, v and slots")
         vt, vh = _strides("v", v, T, hkv, hd, dtype)
-        _vector("slots", slots, T, (torch.int32, torch.int64))
-        slots64 = slots.dtype == torch.int64
+        _vector("slots", slots, T, _INTS)
+        vp, sp, slots64 = v.data_ptr(), slots.data_ptr(), slots.dtype is torch.int64
         cache, ch = _cache(k_cache, v_cache, k_s, v_s, dtype, hd)
         if ch != hkv:
             raise ValueError(f"the cache has {ch} key heads, k {hkv}")
@@ -231,13 +244,11 @@ def qk_norm_rope(q, k, pos, freqs, q_out, k_out=None, v=None, k_cache=None, v_ca
         raise ValueError("give k_out, a cache, or both")
     C.require_cuda(q, k, v, pos, freqs, q_out, k_out, k_cache, v_cache, slots, k_s, v_s, q_w, k_w)
     dev = q.get_device()
-    s = [*sections, 0, 0]
+    s0, s1, s2 = (*sections, 0, 0)[:3]
     args = _ROPE.pack(
-        q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr() if v is not None else 0, vt, vh, q_out.data_ptr(), qot,
-        qoh, k_out.data_ptr() if k_out is not None else 0, kot, koh,
-        slots.data_ptr() if slots is not None else 0, slots64, pos.data_ptr(), pos.stride(0), pos.stride(1), pos64,
-        freqs.data_ptr(), freqs64, q_w.data_ptr() if q_w is not None else 0, k_w.data_ptr() if k_w is not None else 0,
-        wdt, bool(one_plus), eps, T, hq, hkv, hd, 2 * half, axes, s[0], s[1], s[2], bool(interleaved), dt)
+        q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, vp, vt, vh, q_out.data_ptr(), qot, qoh, kop, kot, koh, sp, slots64,
+        pos.data_ptr(), pst[0], pst[1], pos64, freqs.data_ptr(), freqs64, qwp, kwp, wdt, bool(one_plus), eps, T, hq,
+        hkv, hd, 2 * half, axes, s0, s1, s2, bool(interleaved), dt)
     _call("qlin_qk_norm_rope", dev, args, cache, C.current_stream(dev))
     return q_out
 
