@@ -181,6 +181,41 @@ def test_a_captured_decode_step_replays():
         assert torch.equal(L.cache[0], E.cache[0]) and torch.equal(L.cache[1], E.cache[1]), t
 
 
+@pytest.mark.parametrize("hd,T,bounds", [
+    (256, 3333, [[0, 3333, 3333], [0, 1, 3000], [0, 1700, 3333], [0, 0, 0], [0, 3333, 3333]]),  # joined by a launch
+    (256, 6000, [[0, 5900, 6000], [0, 3000, 6000], [0, 17, 33], [0, 5900, 6000]]),                # by the last part
+    (64, 700, [[0, 700, 700], [0, 350, 700], [0, 699, 700]]),                                     # halved tiles
+])
+def test_a_captured_prompt_replays_with_other_bounds(hd, T, bounds):
+    """Cuts and joins follow the bounds that the device holds: every replay equals the eager call bit
+    for bit, and rows of no sequence stay as they were."""
+    from qwen35_amd.kernels import attention as A, qlin as C
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v = (torch.randn((T, h, hd), generator=g, device="cuda").to(BF) for h in (8, 2, 2))
+    out, want, cu = torch.empty_like(q), torch.empty_like(q), _ints(bounds[0])
+    A.attn_prompt(q, k, v, cu, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with C.capture(graph):
+        A.attn_prompt(q, k, v, cu, out)
+    for n, b in enumerate(bounds):
+        cu.copy_(_ints(b))
+        out.fill_(7)
+        want.fill_(7)
+        graph.replay()
+        if n % 2:
+            torch.cuda.synchronize()
+        A.attn_prompt(q, k, v, cu, want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), b
+        assert (out[b[-1]:] == 7).all()
+        one = b[1]
+        if one:  # the first sequence by itself
+            ref, tol = R.attend(q[one - 1:one], k[:one], v[:one], hd ** -0.5,
+                                torch.ones((1, one), dtype=torch.bool, device="cuda"), BF)
+            R.check(out[one - 1:one], ref, tol, f"bounds {b}")
+
+
 def test_two_graphs_of_one_stream_share_its_workspace():
     """A decode call and a prompt call cut into parts, captured apart and replayed in turn."""
     from qwen35_amd.kernels import attention as A, qlin as C
