@@ -195,9 +195,11 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   // A cut costs about as much as seven blocks, and gives less where most of the chip has a tile
   // already: so many blocks it has to take off the longest tile (128-row tiles; uncut / cut: 192
   // of 32 blocks 41 / 41 us, 188 of 47 56 / 48; 512 of 64 89 / 104, of 128 165 / 168, 534 of up to
-  // 125 158 / 148, 314 of 157 171 / 129).
+  // 125 158 / 148, 314 of 157 171 / 129; halved tiles: 100 of 25 blocks 25.0 / 23.4, 116 of 29
+  // 27.2 / 24.5, 264 of up to 29 28 / 37).
+  const bool halved = a.rows < kPromptRows;
   a.shortest = all <= kPromptFewTiles ? 8 : all <= kPromptJoinApart ? 12 : 16;
-  a.gain = all <= kPromptFewTiles ? 4 : all <= kPromptJoinApart ? 20 : 52;
+  a.gain = all <= kPromptFewTiles ? 4 : halved ? 13 : all <= kPromptJoinApart ? 20 : 52;
   if (max_keys < (long long)(a.shortest + a.gain) * kPromptBlock) target = 0;
   // every unit of a key head has a slot: at most 2 target / HKV + tiles of them (and two more for
   // what the device's 32-bit estimate rounds)
