@@ -36,15 +36,9 @@ THETA = 1e7
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
 
-_module = None
-
-
 def _attention():
-    """The package's kernels.attention, imported once as a program does; its directory is no
-    Python identifier, so it is loaded under an alias."""
-    global _module
-    if _module is not None:
-        return _module
+    """The package's kernels.attention; its directory is no Python identifier, so it is
+    loaded under an alias."""
     if ALIAS not in sys.modules:
         pkg = ROOT / "qwen_3.5_comfy_prompt_enhancer_amd"
         spec = importlib.util.spec_from_file_location(ALIAS, pkg / "__init__.py",
@@ -52,8 +46,7 @@ def _attention():
         mod = importlib.util.module_from_spec(spec)
         sys.modules[ALIAS] = mod
         spec.loader.exec_module(mod)
-    _module = importlib.import_module(f"{ALIAS}.kernels.attention")
-    return _module
+    return importlib.import_module(f"{ALIAS}.kernels.attention")
 
 
 # ------------------------------------------------------------------ the cases
