@@ -22,9 +22,10 @@
 //   * int8: codes become 16-bit whole numbers (exact); a key's scale multiplies its scores in 32
 //     bits, a value's scale its probability.
 // The running maximum is a column's, hence a lane's own.  P is rounded to 16 bits for its
-// product (half a step of 2^-8 or 2^-11 of each term; the sum of P is of the unrounded; where one
-// key has all the weight its P is 1 and exact); with int8 values P times scale goes as the sum of
-// two bf16 numbers, which neither a small scale nor one heavy key can take precision from.
+// product (half a step of 2^-8 or 2^-11 of each term; the sum of P is of the unrounded); in fp16 it is
+// taken against a reference that keeps a block's largest P between 2^4 and 2^15, as light keys would
+// else leave fp16's range (fp16_reference).  With int8 values P times scale goes as the sum of two bf16
+// numbers, which neither a small scale nor one heavy key can take precision from.
 //
 // Waves join through LDS, units of a sequence through memory: the last of 16 units to arrive
 // adds their parts in unit order, the last of those groups adds the groups', so that the result
@@ -299,7 +300,12 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
     float mx = t[0];
 #pragma unroll
     for (int s = 1; s < 8; ++s) mx = fmaxf(mx, t[s]);
-    const float mn = fmaxf(m, group_max(mx));
+    const float top = group_max(mx);
+    float mn = fmaxf(m, top);
+    if constexpr (TV::DT == DT_F16) {
+      mn = m;
+      if (__any(off_window(top - m, 4.0f, 15.0f))) mn = fp16_reference(m, top, group_sum(l), 4.0f, 14.0f, 15.0f);
+    }
     const float ms = mn == kNegInf ? 0.0f : mn;
     const float al = exp2_(m - ms);
     m = mn;
@@ -322,7 +328,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
         pop[0][e] = TV::pack(p[2 * e], p[2 * e + 1]);
       }
     }
-    // (the rescaling is skipped while no row's maximum grows)
+    // (the rescaling is skipped while no row's reference moves)
     if (__any(al != 1.0f)) {
 #pragma unroll
       for (int c = 0; c < VC * VW; ++c) O[c] *= al;

@@ -115,6 +115,25 @@ __device__ __forceinline__ N lane_value(N v, int at) {
 // 2^x; of -inf (nothing seen yet, or scores of -inf alone) zero.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// P = 2^(t - reference) of scores t, where P is an fp16 number for its product: 5 bits of exponent
+// hold neither 2^16 nor, with all 11 bits of precision, less than 2^-14.  With the maximum so far as the
+// reference, as 32-bit and bf16 numbers allow, many light keys beside a heavy one (25 octaves above
+// them) would be rounded to multiples of 2^-24 or to zero, while the 32-bit sum of P has them.  So
+// the reference follows the scores both ways: a block of keys whose largest score lies `lo` to `hi` above
+// it (as powers of two) leaves it, any other moves it to `at` below that score.  A key as far as
+// 14 + lo octaves below its block's largest keeps its precision, and what is lost of those further below
+// is at most 2^-(25 + lo) of the block's largest P each.  The sums, of 32 bits, are rescaled with the
+// reference; it stays where they are below 2^64, so that neither they nor the factors that join them
+// leave 32 bits (keys 56 octaves lighter than the sum lose precision then).
+__device__ __forceinline__ bool off_window(float d, float lo, float hi) {
+  return fabsf(d - 0.5f * (lo + hi)) > 0.5f * (hi - lo);  // (no number: nothing seen yet on either side)
+}
+// The reference after a block of largest score `top`; l: the sum of P so far.
+__device__ __forceinline__ float fp16_reference(float m, float top, float l, float lo, float at, float hi) {
+  const float mn = off_window(top - m, lo, hi) && top != kNegInf ? top - at : m;
+  return fmaxf(mn, m + __builtin_amdgcn_logf(l) - 64.0f);
+}
+
 // Lets a kernel take `bytes` of dynamic LDS on the current device; `done` holds a bit for each
 // device where it may.
 inline hipError_t allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {

@@ -20,9 +20,10 @@
 //     numbers (exact) in LDS; a key's scale multiplies its scores, a value's its probability, both
 //     in 32 bits.  P x scale is rounded once for its product (to bf16; for fp16 queries it goes as
 //     the sum of two bf16 numbers, as fp16 may not hold it).
-//   * The sums are rescaled only when a row's maximum has grown by more than 2^8: P stays below
-//     2^8, which both 16-bit types hold with full relative precision.  P is rounded to the
-//     queries' type for its product; its sum, the maximum and O are 32-bit.
+//   * The sums are rescaled only when a row's maximum has grown by more than 2^8 (P stays below 2^8,
+//     which bf16 holds with full relative precision), in fp16 when a block's largest P would leave
+//     2^-8 .. 2^15 on either side (fp16_reference).  P is rounded to the queries' type for its product;
+//     its sum, the maximum and O are 32-bit.
 //
 // What bounds it: the MFMAs (of 256 values, 32 of 32 cycles a block and wave), then the softmax's
 // vector work and LDS.  32 rows a wave, operands read three products ahead and two workgroups a CU (256
@@ -489,8 +490,15 @@ void prompt_kernel(const PromptArgs a) {
     float x, y;
     lane_pair<32>(mx, x, y);
     mx = fmaxf(x, y) * a.c;
-    if (__any(mx > m + 8.0f)) {
-      const float mn = fmaxf(m, mx);
+    // (fp16: a block's largest P stays between 2^-8 and 2^15, see fp16_reference; every score of a deviation
+    // below 3 then rescales about as seldom as the line of 2^8)
+    constexpr bool NARROW = TV::DT == DT_F16;
+    if (NARROW ? __any(off_window(mx - m, -8.0f, 15.0f)) : __any(mx > m + 8.0f)) {
+      float mn = fmaxf(m, mx);
+      if constexpr (NARROW) {
+        lane_pair<32>(l, x, y);
+        mn = fp16_reference(m, mx, x + y, -8.0f, 8.0f, 15.0f);
+      }
       const float al = exp2_(m - (mn == kNegInf ? 0.0f : mn));
       m = mn;
       l *= al;
