@@ -42,9 +42,11 @@
 //   * Few tiles of 16-bit keys are halved (KG = 2): two waves hold 64 rows, the other two the same rows
 //     over every second block, and their sums are added in LDS.
 //
-// A row's masked keys have no part in it whatever they hold: scores are replaced before the
-// maximum, and as zero times a value that is no number is none, a tile whose sums come out
-// non-finite after masked blocks is computed again row by row over its visible keys alone.
+// A row's masked keys have no part in it whatever they hold.  Scores are replaced before the maximum.  An
+// int8 value's scale that is not finite is taken out, and makes its key's score no number instead.  A 16-bit
+// value that is no number is none times a P of zero either: a unit whose sums come out non-finite after
+// masked blocks is computed again, finite values apart from the others (split), in about twice the time
+// (prompts of 512 / 2048 tokens whose first value is NaN 66 / 170 us, of numbers 22 / 48).
 #pragma once
 
 #include "attn_dev.h"
@@ -277,6 +279,34 @@ __device__ __forceinline__ void lds_st(uint32_t at, V v) {
   *(__attribute__((address_space(3))) V*)(uintptr_t)at = v;
 }
 
+// Values that are no numbers, in the pass that looks out for them.  A pair of 16-bit values is split into
+// its finite ones (zero in the others' place) and marks of the others; the product of marks and weights
+// (1 for a key that a row sees, kOddNan where its P is zero, 0 for masked ones) adds up, exactly, to what
+// a row's sum becomes: of at most 32 keys each, infinities of either sign stay below kOddNan.
+constexpr float kOddPlus = 1.0f, kOddMinus = 64.0f, kOddNan = 4096.0f;
+
+template <typename T>
+__device__ __forceinline__ u32x2 split(uint32_t w) {
+  constexpr uint32_t EXP = T::DT == DT_BF16 ? 0x7F80u : 0x7C00u, MANT = 0x7FFFu & ~EXP;
+  constexpr uint32_t ONE = T::DT == DT_BF16 ? 0x3F80u : 0x3C00u, STEP = ONE == 0x3F80u ? 6u << 7 : 6u << 10;  // 2^6
+  uint32_t finite = 0u, odd = 0u;
+#pragma unroll
+  for (int z = 0; z < 32; z += 16) {  // (without branches: the sums would be copied around them)
+    const uint32_t x = (w >> z) & 0xFFFFu;
+    const uint32_t mark = ONE + ((x & MANT) != 0u ? 2u * STEP : (x >> 15) * STEP);
+    const bool number = (x & EXP) != EXP;
+    finite |= (number ? x : 0u) << z;
+    odd |= (number ? 0u : mark) << z;
+  }
+  return u32x2{finite, odd};
+}
+
+// What marks add up to: 0, an infinity, or no number.
+__device__ __forceinline__ float odd_sum(float n) {
+  const float minus = n < kOddNan && floorf(n / kOddMinus) * kOddMinus == n ? kNegInf : __builtin_nanf("");
+  return n == 0.0f ? 0.0f : n < kOddMinus ? __builtin_inff() : minus;
+}
+
 // Q8: int8 cache.  KG = 2: two waves hold the rows of a tile of 64, the other two the same rows
 // over every second block, and their sums are added through LDS at the end: for few tiles, each of
 // which then takes half as long.
@@ -308,14 +338,14 @@ void prompt_kernel(const PromptArgs a) {
   const int rg = wave % (4 / KG), kg = wave / (4 / KG);
   const int R0 = t.tile * ROWS + rg * 32;
   u32x4 Q[G::NS];
-  int lim;
-  {
+  auto load_q = [&](const PromptArgs& a, int col, int h) __attribute__((always_inline)) {
     const int i = (R0 + col) / a.G, ic = min(i, t.s.nq - 1);
-    lim = seen(a, t.s, ic);
     const uint16_t* q = (const uint16_t*)a.q + (t.s.q0 + ic) * a.qt + (hk * a.G + (R0 + col - i * a.G)) * a.qh + 8 * h;
 #pragma unroll
     for (int s = 0; s < G::NS; ++s) Q[s] = ld_global<u32x4>(q + 16 * s);
-  }
+    return seen(a, t.s, ic);
+  };
+  const int lim = load_q(a, col, h);
   // what every row of the wave sees, and what some row sees
   const int wmin = seen(a, t.s, min(R0 / a.G, t.s.nq - 1));
   const int wmax = R0 / a.G >= t.s.nq ? 0 : seen(a, t.s, min((R0 + 31) / a.G, t.s.nq - 1));
@@ -415,6 +445,9 @@ void prompt_kernel(const PromptArgs a) {
     constexpr int CH = HD / 16;  // 16-byte chunks of a row of codes
     int lane = (int)threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
+    // this wave's scales: keys', then values'
+    const uint32_t scales = codes + (uint32_t)(G::STAGE / 2 + 64 * wave + 4 * (lane & 15));
+    const uint64_t odd = __ballot(!(fabsf(lds_ld<float>(scales)) < __builtin_inff()));
 #pragma unroll
     for (int i = 0; i < 8 * CH / 64 || i == 0; ++i) {
       const int x = i * 64 + lane, r = x / CH, c16 = x % CH, row = 8 * wave + r;
@@ -437,6 +470,9 @@ void prompt_kernel(const PromptArgs a) {
         lds_st(to + (uint32_t)(G::HALF + (((((c >> 2) ^ G::swv(row)) << 2) | (c & 3)) << 4)), vo);
       }
     }
+    // a scale that is not finite makes no number of its key's score, hence of every row that sees it; as a
+    // value's it would make none of the rows that do not, either
+    if (odd && ((odd | odd >> 8) >> (lane & 7) & 1)) lds_st(scales, lane & 8 ? 0.0f : __builtin_nanf(""));
   };
 
   // LDS places of this lane's operands: step s of K at ka ^ 32 s (the swizzle reaches 256 bytes),
@@ -447,8 +483,9 @@ void prompt_kernel(const PromptArgs a) {
   const uint32_t va = mine + (uint32_t)(G::HALF + (4 * h + (s16 >> 2)) * G::ROWB + (G::swv(s16 >> 2) << 6) +
                                         ((lane >> 4) & 1) * 32 + (s16 & 3) * 8);
 
-  auto step = [&](auto stage_c, int kb, uint32_t scales) __attribute__((always_inline)) {
+  auto step = [&](auto stage_c, int kb, uint32_t scales, auto careful_c) __attribute__((always_inline)) {
     constexpr uint32_t stage = decltype(stage_c)::value;
+    constexpr bool CAREFUL = decltype(careful_c)::value;
     if (kb * G::KB >= wmax || (KG > 1 && kb >= kb1)) return;
     // operands are read kAhead products ahead (the order is fixed: left to itself the compiler
     // reads each just before its product, and the wave waits for LDS every time)
@@ -508,7 +545,7 @@ void prompt_kernel(const PromptArgs a) {
         for (int i = 0; i < 16; ++i) O[d][i] *= al;
     }
     const float ms = m == kNegInf ? 0.0f : m;
-    u32x4 P[PN][2];
+    u32x4 P[PN][2], W[2];
     float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -531,6 +568,11 @@ void prompt_kernel(const PromptArgs a) {
           p1 *= vs[e / 2][2 * (e % 2) + 1];
         }
         P[0][k][e] = TV::pack(p0, p1);
+        if constexpr (CAREFUL) {
+          const int i = 8 * k + 2 * e, key = 8 * (i / 4) + i % 4, rel = lim - kb * G::KB - 4 * h;
+          W[k][e] = TV::pack(key < rel ? p0 == 0.0f ? kOddNan : kOddPlus : 0.0f,
+                             key + 1 < rel ? p1 == 0.0f ? kOddNan : kOddPlus : 0.0f);
+        }
         if constexpr (PN == 2) {
           const uint32_t w = P[0][k][e];
           P[1][k][e] = TV::pack(p0 - bitcast<float>(w << 16), p1 - bitcast<float>(w & 0xFFFF0000u));
@@ -550,6 +592,30 @@ void prompt_kernel(const PromptArgs a) {
       }
       return u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
     };
+    if constexpr (CAREFUL) {
+      // finite values as ever; of the others, a second product counts what each row sees (see split)
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d) {
+        f32x16 seen_odd = {};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const u32x4 v = v_at(2 * d + k);
+          u32x4 finite, odd;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const u32x2 s = split<TV>(v[e]);
+            finite[e] = s.x, odd[e] = s.y;
+          }
+          O[d] = TV::mma32(finite, P[0][k], O[d]);
+          seen_odd = TV::mma32(odd, W[k], seen_odd);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[d][i] += odd_sum(seen_odd[i]);
+        asm volatile("" : "+v"(O[d]));  // (now, not behind all others)
+      }
+      return;
+    }
     u32x4 v[kAhead];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -571,20 +637,21 @@ void prompt_kernel(const PromptArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  // 16-bit keys: KG blocks of a stage
+  constexpr uint32_t RING = KG * G::STAGE;
+  constexpr std::integral_constant<uint32_t, 0> s0;
+  constexpr std::integral_constant<uint32_t, RING> s1;
+  int pid[KG];
+  auto pages = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < KG; ++x) pid[x] = page_of(kb + x);
+  };
+  auto fetch = [&](uint32_t stage, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < KG; ++x) issue(stage + (uint32_t)(x * G::STAGE), kb + x, pid[x]);
+  };
   if (kb0 < kb1) {
     if constexpr (!Q8) {
-      constexpr uint32_t RING = KG * G::STAGE;
-      constexpr std::integral_constant<uint32_t, 0> s0;
-      constexpr std::integral_constant<uint32_t, RING> s1;
-      int pid[KG];
-      auto pages = [&](int kb) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < KG; ++x) pid[x] = page_of(kb + x);
-      };
-      auto fetch = [&](uint32_t stage, int kb) __attribute__((always_inline)) {
-#pragma unroll
-        for (int x = 0; x < KG; ++x) issue(stage + (uint32_t)(x * G::STAGE), kb + x, pid[x]);
-      };
       pages(kb0);
       fetch(lds0, kb0);
       pages(kb0 + KG);
@@ -592,39 +659,82 @@ void prompt_kernel(const PromptArgs a) {
         meet();
         fetch(lds0 + RING, kb + KG);
         pages(kb + 2 * KG);
-        step(s0, kb + kg, 0);
+        step(s0, kb + kg, 0, std::false_type{});
         if ((kb += KG) >= kb1) break;
         meet();
         fetch(lds0, kb + KG);
         pages(kb + 2 * KG);
-        step(s1, kb + kg, 0);
+        step(s1, kb + kg, 0, std::false_type{});
         if ((kb += KG) >= kb1) break;
       }
     } else {
-      int pid = page_of(kb0);
+      pages(kb0);
       // codes of block kb + 1 land while block kb is widened and used
       const uint32_t c0 = lds0 + G::STAGE;
       constexpr uint32_t CODES = G::STAGE / 2 + G::SCALES;
       uint32_t codes = c0;
-      issue(codes, kb0, pid);
-      pid = page_of(kb0 + 1);
+      issue(codes, kb0, pid[0]);
+      pages(kb0 + 1);
       for (int kb = kb0; kb < kb1; ++kb) {
         meet();  // the tile has been read, this block's codes and scales are there
         const uint32_t next = codes == c0 ? c0 + CODES : c0;
-        issue(next, kb + 1, pid);
-        pid = page_of(kb + 2);
+        issue(next, kb + 1, pid[0]);
+        pages(kb + 2);
         widen(codes);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile is written
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        step(std::integral_constant<uint32_t, 0>{}, kb, codes + G::STAGE / 2);
+        step(s0, kb, codes + G::STAGE / 2, std::false_type{});
         codes = next;
       }
     }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
     __builtin_amdgcn_sched_barrier(0);
+  }
+  // (the row again, from a thread index that the compiler takes for another, and the arguments read
+  // again, so that nothing of what follows is kept in registers through the loop)
+  int tid2 = (int)threadIdx.x;
+  asm volatile("" : "+v"(tid2));
+  auto kernarg = (const __attribute__((address_space(4))) PromptArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(kernarg));
+  const PromptArgs& ea = *(const PromptArgs*)kernarg;
+
+  // Sums that are no numbers, after blocks that are masked for the wave: the unit again, a stage at a time,
+  // finite values apart from the others.  (A row that sees such a value gets there too; its second
+  // computation changes nothing.)
+  const bool masked = kb1 * G::KB > seen(ea, t.s, min(t.tile * ROWS / ea.G, t.s.nq - 1));  // for some row of the tile
+  if (!Q8 && masked) {
+    __shared__ int s_spoiled[4];
+    float z[4] = {};  // (four chains of additions)
+    if (kb1 * G::KB > wmin) {
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i % 4] = fmaf(O[d][i], 0.0f, z[i % 4]);
+    }
+    const bool spoiled = __any(!((z[0] + z[1]) + (z[2] + z[3]) == 0.0f));
+    if (lane == 0) s_spoiled[wave] = spoiled;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) any |= s_spoiled[w];
+    if (rfl32((uint32_t)any)) {
+      m = kNegInf, l = 0.0f;
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
+      for (int kb = kb0; kb < kb1; kb += KG) {
+        pages(kb);
+        __syncthreads();  // the stage has been read
+        fetch(lds0, kb);
+        load_q(ea, tid2 & 31, (tid2 >> 5) & 1);
+        meet();
+        step(s0, kb + kg, 0, std::true_type{});
+      }
+    }
   }
   if constexpr (KG == 2) {
     // the second group's sums, then its maxima and sums of P, to LDS (every wave has read its last
@@ -659,13 +769,6 @@ void prompt_kernel(const PromptArgs a) {
     }
   }
 
-  // (the row again, from a thread index that the compiler takes for another, and the arguments read
-  // again, so that nothing of what follows is kept in registers through the loop)
-  int tid2 = (int)threadIdx.x;
-  asm volatile("" : "+v"(tid2));
-  auto kernarg = (const __attribute__((address_space(4))) PromptArgs*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(kernarg));
-  const PromptArgs& ea = *(const PromptArgs*)kernarg;
   const int row = R0 + (tid2 & 31), tok = row / ea.G;
   const int head = hk * ea.G + (row - tok * ea.G);
   const int h2 = (tid2 >> 5) & 1;
@@ -673,15 +776,6 @@ void prompt_kernel(const PromptArgs a) {
   float x, y;
   lane_pair<32>(l, x, y);
   l = x + y;
-  bool again = false;
-  if (kb1 * G::KB > wmin) {  // masked blocks were among the unit's
-    float z = 0.0f;
-#pragma unroll
-    for (int d = 0; d < G::ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) z = fmaf(O[d][i], 0.0f, z);
-    again = !(z == 0.0f) && tok < t.s.nq && kg == 0;
-  }
   // partials: unit p of the tile at (slot + p step) of the key head's; 32-bit sums by row set,
   // 32-wide block, run of 8 values and lane, so that a wave moves 1 KiB at a time; then (maximum, sum
   // of P) of each row
@@ -699,7 +793,7 @@ void prompt_kernel(const PromptArgs a) {
     return __builtin_amdgcn_raw_buffer_load_b64(rs, part * stride + ML + (unsigned)r * 8u, 0, kCpolSc1);
   };
 
-  if (kg == 0 && !__any(again)) {
+  if (kg == 0) {
     if (any_bad) l = __builtin_nanf("");
     if (t.parts > 1) {
       if (R0 / ea.G < t.s.nq) {
@@ -733,71 +827,6 @@ void prompt_kernel(const PromptArgs a) {
             *(u32x4*)(o + 32 * d + 16 * i + 8 * h2) =
                 u32x4{(uint32_t)r0[0], (uint32_t)r1[0], (uint32_t)r0[1], (uint32_t)r1[1]};
         }
-    }
-  }
-
-  // Something non-finite among the sums: the wave's rows again, one at a time, over the keys
-  // that each sees (lanes hold HD / 64 adjacent values).
-  constexpr int E = HD / 64;
-  const int redo = __any(again) ? 32 : 0;
-  for (int r = 0; r < redo; ++r) {
-    const int R = R0 + r, i = R / ea.G;
-    if (i >= t.s.nq) break;
-    const int hq = hk * ea.G + (R - i * ea.G);
-    const int k1 = min(kb1 * G::KB, seen(ea, t.s, i));
-    const uint16_t* q = (const uint16_t*)ea.q + (t.s.q0 + i) * ea.qt + hq * ea.qh + lane * E;
-    float qv[E], o[E], mr = kNegInf, lr = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) qv[e] = T::get(q[e]), o[e] = 0.0f;
-    for (int key = kb0 * G::KB; key < k1; ++key) {
-      const int pid = PAGED ? table[key >> ea.kv.page_shift] : 0;
-      const int pc = (unsigned)pid >= (unsigned)ea.kv.num_pages ? 0 : pid;
-      const uint8_t* kp = base_of(kpl, key, pc);
-      const uint8_t* vp = base_of(vpl, key, pc);
-      float kv[E], vv[E], dot = 0.0f;
-      if constexpr (Q8) {
-        const float ks = *(const float*)base_of(kspl, key, pc), vs = *(const float*)base_of(vspl, key, pc);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          kv[e] = (float)((const int8_t*)kp)[lane * E + e] * ks;
-          vv[e] = (float)((const int8_t*)vp)[lane * E + e] * vs;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          kv[e] = T::get(((const uint16_t*)kp)[lane * E + e]);
-          vv[e] = T::get(((const uint16_t*)vp)[lane * E + e]);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) dot = fmaf(qv[e], kv[e], dot);
-#pragma unroll
-      for (int z = 1; z < 64; z <<= 1) dot += __shfl_xor(dot, z);
-      const float s = dot * ea.c;
-      const float mn = fmaxf(mr, s), ms = mn == kNegInf ? 0.0f : mn;
-      const float al = exp2_(mr - ms), p = exp2_(s - ms);
-      mr = mn;
-      lr = lr * al + p;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * al + p * vv[e];
-    }
-    if (any_bad) lr = __builtin_nanf("");
-    if (t.parts > 1) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        __builtin_amdgcn_raw_buffer_store_b32(
-            bitcast<uint32_t>(o[e]), rs,
-            (unsigned)t.part * stride + (unsigned)(rg * 32 * HD * 4) +
-                (unsigned)(((d / 32) * 4 + (d % 32) / 8) * 256 + (r + 32 * ((d % 8) / 4)) * 4 + d % 4) * 4u,
-            0, kCpolSc1);
-      }
-      if (lane == 0) st_ml((unsigned)t.part, rg * 32 + r, mr, lr);
-    } else {
-      uint16_t* out = (uint16_t*)ea.o + (long long)(t.s.q0 + i) * ea.ot + hq * ea.oh + lane * E;
-      const bool none = seen(ea, t.s, i) == 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) out[e] = to_out16(none ? 0.0f : o[e] / lr, T::DT);
     }
   }
   if (t.parts == 1 || ea.join_apart) return;
