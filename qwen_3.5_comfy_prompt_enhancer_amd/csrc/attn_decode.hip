@@ -246,6 +246,13 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 2 : HD == 128 ? 3 : 4) void d
     f32x4 S[2];
     f32x4 ks[2], vs[2];
     if constexpr (Q8) {
+      // a scale that is not finite makes no number of its key's score (an infinite one of a negative score
+      // would leave its key out)
+      uint64_t odd = __ballot(!(fabsf(sc) < __builtin_inff()));
+      if (odd) {
+        odd |= odd >> 32 | odd << 32;
+        if (odd >> lane & 1) sc = lane < 32 ? __builtin_nanf("") : 0.0f;
+      }
       // (a wave's LDS instructions take effect in order)
       lsc[lane] = sc;
       __builtin_amdgcn_wave_barrier();

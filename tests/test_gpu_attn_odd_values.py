@@ -135,6 +135,25 @@ def test_scales_that_are_no_numbers(dt, hd, nq, past):
         R.check(out[~sees][:, h], ref[~sees][:, h], tol[~sees][:, h], f"key head {head}")
 
 
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("n,at", [(1, 0), (45, 44), (3000, 1234), (70000, 69000)])
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+@pytest.mark.parametrize("of_values", [False, True])
+def test_a_decode_step_over_a_scale_that_is_no_number(hd, n, at, bad, of_values):
+    """Whatever the sign of its scores; the other key head is what it is."""
+    from qwen35_amd.kernels import attention as A
+    table, pages = R.pages_of([n], 64, 1, 4, "cuda")
+    c = R.cache(pages, 64, 2, hd, BF, 7, True)
+    ok = [x.clone() for x in R.gathered(c, table, 0, n)]
+    q = torch.randn((1, 32, hd), generator=torch.Generator("cuda").manual_seed(3), device="cuda").to(BF)
+    c[3 if of_values else 2][table[0, at // 64].long(), at % 64, 1] = bad
+    out = torch.empty_like(q)
+    A.attn_decode(q, c[0], c[1], table, _ints(n), out, k_s=c[2], v_s=c[3])
+    assert out[:, 16:].isnan().all()
+    ref, tol = R.attend(q, *ok, hd ** -0.5, torch.ones((1, n), dtype=torch.bool, device="cuda"), BF, 2.0 ** -16)
+    R.check(out[:, :16], ref[:, :16], tol[:, :16])
+
+
 def test_one_value_costs_no_more_than_another_pass():
     """A NaN in the first key's value, which every row sees: about three times the time, not hundreds."""
     from qwen35_amd.kernels import attention as A
