@@ -11,7 +11,8 @@
  *
  * Strides are in elements; the last axis (hd values) is contiguous.  Every 16-bit tensor
  * is 16-byte aligned with strides that are multiples of 8; int8 tensors have strides that
- * are multiples of 16.  hd is 64, 128 or 256; a key head has at most 64 query heads, a call
+ * are multiples of 16.  Strides of tokens are at most 2^26, of heads and pages 2^31 - 16 (of an
+ * int8 cache's scales 2^30 - 8); that of an axis of one is not looked at.  hd is 64, 128 or 256; a key head has at most 64 query heads, a call
  * at most 65536 query heads, 2^24 - 1 tokens and 65536 sequences, a sequence 2^30 keys.  Lengths, page tables, slots and positions are
  * read on the device:
  *   - a slot below 0 or past the cache stores nothing (a padded row); the others of a call

@@ -45,18 +45,22 @@ constexpr int kMaxSeqs = 1 << 16;             // sequences of a call: every work
 constexpr int kMaxGroup = 64;                 // query heads of a key head
 constexpr long long kMaxKeys = 1LL << 30;     // keys of a sequence
 constexpr long long kMaxTokenStride = 1LL << 26;  // eight rows' offset stays in 32 bits
-constexpr long long kMaxPageStride = (1LL << 31) - 16;  // in bytes below 2^32
+constexpr long long kMaxStride = (1LL << 31) - 16;  // of heads and pages: in bytes below 2^32
 
-// One 16-bit (es = 2) or int8 tensor: n of the outer strides.  `write`: rows must not overlap.
+// One 16-bit (es = 2) or int8 tensor: n of the outer strides (that of an axis of one is never used).
+// `write`: rows must not overlap.
 int check_tensor(const char* fn, const char* name, const void* p, int es, int hd, long long n0, long long s0,
                  long long n1, long long s1, bool write) {
   const int mult = es == 1 ? 16 : 8;
   if (!p) return fail(QLIN_ERR_INVALID, "%s: null %s", fn, name);
+  if (n0 <= 1) s0 = 0;
+  if (n1 <= 1) s1 = 0;
   if (!aligned(p, 16) || s0 % mult || s1 % mult || s0 < 0 || s1 < 0)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: %s must be 16-byte aligned with strides that are multiples of %d", fn, name,
                 mult);
-  if (s0 > kMaxTokenStride || s1 > kMaxTokenStride)
-    return fail(QLIN_ERR_UNSUPPORTED, "%s: strides of %s above %lld", fn, name, kMaxTokenStride);
+  if (s0 > kMaxTokenStride || s1 > kMaxStride)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: strides of %s above %lld (rows) or %lld (heads)", fn, name, kMaxTokenStride,
+                kMaxStride);
   if (write && ((n0 > 1 && s0 < hd) || (n1 > 1 && s1 < hd)))
     return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, name);
   return QLIN_OK;
@@ -107,12 +111,14 @@ int check_cache(const char* fn, const qlin_paged_kv* c, int hkv, int hd, int dty
   const int es = q8 ? 1 : 2, mult = q8 ? 16 : 8;
   QA_TRY(check_tensor(fn, "k_cache", c->k, es, hd, c->page, c->k_token, hkv, c->k_head, write));
   QA_TRY(check_tensor(fn, "v_cache", c->v, es, hd, c->page, c->v_token, hkv, c->v_head, write));
-  if (c->k_page % mult || c->v_page % mult || c->k_page < 0 || c->v_page < 0)
-    return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides must be multiples of %d", fn, mult);
-  if (c->k_page > kMaxPageStride || c->v_page > kMaxPageStride)
-    return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides above %lld", fn, kMaxPageStride);
-  if (write && c->num_pages > 1 && (c->k_page < hd || c->v_page < hd))
-    return fail(QLIN_ERR_INVALID, "%s: pages of the cache overlap", fn);
+  if (c->num_pages > 1) {
+    if (c->k_page % mult || c->v_page % mult || c->k_page < 0 || c->v_page < 0)
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides must be multiples of %d", fn, mult);
+    if (c->k_page > kMaxStride || c->v_page > kMaxStride)
+      return fail(QLIN_ERR_UNSUPPORTED, "%s: page strides above %lld", fn, kMaxStride);
+    if (write && (c->k_page < hd || c->v_page < hd))
+      return fail(QLIN_ERR_INVALID, "%s: pages of the cache overlap", fn);
+  }
   if (q8) {
     if (!c->k_s || !c->v_s) return fail(QLIN_ERR_INVALID, "%s: an int8 cache needs k_s and v_s", fn);
     if (!aligned(c->k_s, 4) || !aligned(c->v_s, 4))
@@ -120,9 +126,10 @@ int check_cache(const char* fn, const qlin_paged_kv* c, int hkv, int hd, int dty
     const int64_t st[6] = {c->ks_page, c->ks_token, c->ks_head, c->vs_page, c->vs_token, c->vs_head};
     const int n[3] = {c->num_pages, c->page, hkv};
     for (int i = 0; i < 6; ++i) {
-      if (st[i] < 0 || st[i] > (i % 3 ? kMaxTokenStride : kMaxPageStride / 2))
+      if (n[i % 3] <= 1) continue;
+      if (st[i] < 0 || st[i] > (i % 3 == 1 ? kMaxTokenStride : kMaxStride / 2))
         return fail(QLIN_ERR_UNSUPPORTED, "%s: stride of the scales negative or too large", fn);
-      if (write && n[i % 3] > 1 && st[i] < 1) return fail(QLIN_ERR_INVALID, "%s: scales of the cache overlap", fn);
+      if (write && st[i] < 1) return fail(QLIN_ERR_INVALID, "%s: scales of the cache overlap", fn);
     }
   } else if (c->k_s || c->v_s) {
     return fail(QLIN_ERR_INVALID, "%s: a 16-bit cache has no scales", fn);

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeArgs a) {
   const int heads = a.HQ + a.HKV + (a.v ? a.HKV : 0);
 
   auto kind_of = [&](int h) { return h < a.HQ ? 0 : h < a.HQ + a.HKV ? 1 : 2; };
-  // the token's rows (uniform), and a head's place in them: strides are below 2^27 bytes
+  // the token's rows (uniform), and a head's place in them: strides are below 2^32 bytes
   const uint8_t* qr = (const uint8_t*)a.q + (long long)t * a.qt * 2;
   const uint8_t* kr = (const uint8_t*)a.k + (long long)t * a.kt * 2;
   const uint8_t* vr = (const uint8_t*)a.v + (long long)t * a.vt * 2;

@@ -21,7 +21,8 @@ Cache tensors are [pages, page, kv_heads, hd] (a power of two tokens to a page, 
 1024) with any strides in front of the last axis, so a buffer that is laid out
 [pages, kv_heads, page, hd] passes as its permuted view.  They hold the queries' type, or
 int8 codes with fp32 scales k_s / v_s [pages, page, kv_heads].  16-bit tensors need
-16-byte aligned rows (strides that are multiples of 8; int8: of 16).
+16-byte aligned rows (strides that are multiples of 8; int8: of 16; of tokens at most 2^26
+elements, of heads and pages 2^31 - 16).
 
 Lengths, page tables, slots and positions stay on the device and are never waited for;
 what they may hold is stated in include/qlin_attn.h.  All calls run on the current
