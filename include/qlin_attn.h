@@ -109,7 +109,8 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head,
                      float scale, int causal, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same over the cache: sequence b's keys are the first kv_len[b] tokens of the pages
- * table[b][0 .. max_pages - 1] (its own queries' keys among them). */
+ * table[b][0 .. max_pages - 1] (its own queries' keys among them; of a table of no pages, which may be
+ * NULL, no sequence has any). */
 int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const qlin_paged_kv* cache,
                            const int* table, int64_t table_stride, int max_pages, const int* kv_len,
                            const int* cu_q, void* out, int64_t o_token, int64_t o_head,

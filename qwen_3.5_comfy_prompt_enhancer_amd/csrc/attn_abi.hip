@@ -144,6 +144,7 @@ int shift_of(int page) { return __builtin_ctz((unsigned)page); }
 int check_paged(const char* fn, const qlin_paged_kv* cache, const int* table, int64_t table_stride, int max_pages,
                 const int* kv_len, int hkv, int hd, int dtype, KvSrc& kv) {
   QA_TRY(check_cache(fn, cache, hkv, hd, dtype, false, kv.k, kv.v));
+  if (max_pages == 0) table = kv_len;  // (a table of no pages is never read: no sequence has a key)
   if (!table || !kv_len) return fail(QLIN_ERR_INVALID, "%s: null page table or lengths", fn);
   if (!aligned(table, 4) || !aligned(kv_len, 4))
     return fail(QLIN_ERR_UNSUPPORTED, "%s: table and kv_len must be 4-byte aligned", fn);

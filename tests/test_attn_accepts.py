@@ -60,3 +60,11 @@ def test_strides_of_an_axis_of_one(tmp):
         _accepted(tmp, D.decode(one8, B=1, hkv=1), D.rope(one8, T=1, hkv=1))
     two = D.cache(2, 64, k_head=65)
     _refused(tmp, "multiples of 8", D.decode(two, hkv=2), D.prompt(qt=513), D.rope(ko_token=129))
+
+
+def test_a_table_of_no_pages(tmp):
+    """All sequences are empty; torch gives such a table the address 0."""
+    kv = D.cache(4, 64)
+    _accepted(tmp, D.decode(kv, table=None, max_pages=0), D.paged(kv, table=None, max_pages=0))
+    _refused(tmp, "null page table", D.decode(kv, table=None), D.paged(kv, table=None),
+             D.decode(kv, table=None, max_pages=0, kv_len=None))

@@ -1,5 +1,5 @@
-"""A cache whose heads lie further apart than a token's stride may be, [kv_heads, pages, page, hd]: written by
-qk_norm_rope, read by a chunk and by a decode step."""
+"""Caches at the ends of what the calls accept: heads further apart than a token's stride may be, [kv_heads,
+pages, page, hd], written by qk_norm_rope, read by a chunk and by a decode step; a table of no pages."""
 from __future__ import annotations
 
 import pytest
@@ -42,3 +42,17 @@ def test_heads_of_more_than_a_token_stride(int8):
     ref, tol = R.attend(qr, kk, vv, hd ** -0.5, R.causal(n, n, "cuda"), BF)
     R.check(out, ref, tol, "prompt")
     R.check(one, ref[-1:], tol[-1:], "decode")
+
+
+def test_a_table_of_no_pages_gives_zeros():
+    from qwen35_amd.kernels import attention as A
+    c = R.cache(4, 16, 2, 64, BF, 1)
+    table = torch.empty((3, 0), dtype=torch.int32, device="cuda")
+    kv_len = torch.tensor([0, 5, 0], dtype=torch.int32, device="cuda")
+    q = torch.randn((3, 8, 64), device="cuda").to(BF)
+    for call in (lambda o: A.attn_decode(q, c[0], c[1], table, kv_len, o),
+                 lambda o: A.attn_prompt_paged(q, c[0], c[1], table, kv_len,
+                                               torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda"), o)):
+        out = torch.full_like(q, 7)
+        call(out)
+        assert (out == 0).all()
