@@ -25,6 +25,10 @@
  *     key; elsewhere infinities and NaN go through the formulas;
  *   - row bounds (cu) are clamped to the rows there are, and query bounds that fall count as the
  *     highest before them.
+ * What a call writes shares no byte with what it reads or else writes (q_out that is q and k_out that
+ * is k aside, with the same strides): such calls are refused.  Tensors may lie between each other's
+ * rows, heads or pages; where they do so with strides that are different but about the same length,
+ * over long axes, they are taken to overlap.
  */
 #ifndef QLIN_ATTN_H
 #define QLIN_ATTN_H
@@ -62,9 +66,9 @@ typedef struct qlin_rope {
   int64_t k_token, k_head;
   const void* v;               /* [T][kv_heads][hd], or NULL (no cache) */
   int64_t v_token, v_head;
-  void* q_out;                 /* may be q itself */
+  void* q_out;                 /* may be q itself, with its strides */
   int64_t qo_token, qo_head;
-  void* k_out;                 /* rotated keys, may be k itself; NULL: the cache only */
+  void* k_out;                 /* rotated keys, may be k itself, with its strides; NULL: the cache only */
   int64_t ko_token, ko_head;
   const void* slots;           /* [T] places in the cache: page * page size + token; NULL: no cache */
   int slots_64;                /* 1: int64, 0: int32 */
@@ -98,8 +102,7 @@ int qlin_qk_norm_rope(const qlin_rope* args, const qlin_paged_kv* cache, void* s
  * out = softmax(scale q k^T) v over all keys of the sequence, or where `causal` over the
  * keys j <= i + keys - queries for its query i.  Query head h uses key head
  * h / (q_heads / kv_heads).  A row that sees no key is zero; masked keys have no part in a
- * row whatever they hold.  Rows of no sequence are left as they were.  out must not overlap
- * q, k or v. */
+ * row whatever they hold.  Rows of no sequence are left as they were. */
 int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head,
                      const void* k, int64_t k_token, int64_t k_head,
                      const void* v, int64_t v_token, int64_t v_head,

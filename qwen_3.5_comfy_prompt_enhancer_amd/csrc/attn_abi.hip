@@ -162,6 +162,95 @@ int check_paged(const char* fn, const qlin_paged_kv* cache, const int* table, in
   return QLIN_OK;
 }
 
+// A tensor's bytes: runs of `width` at every sum of indexes times strides (bytes; an axis of one has 0).
+struct Region {
+  const char* name;
+  const char* p;
+  long long width;
+  long long n[3], s[3];
+  long long end() const {
+    long long e = width;
+    for (int i = 0; i < 3; ++i) e += (n[i] - 1) * s[i];
+    return e;
+  }
+};
+
+Region region(const char* name, const void* p, int es, int run, long long n0, long long s0, long long n1, long long s1,
+              long long n2 = 1, long long s2 = 0) {
+  return Region{name, (const char*)p, (long long)es * run, {n0, n1, n2},
+                {n0 > 1 ? s0 * es : 0, n1 > 1 ? s1 * es : 0, n2 > 1 ? s2 * es : 0}};
+}
+
+// Sums c + sum k_i s_i with lo_i <= k_i <= hi_i: whether one lies between -before and after (both
+// excluded).  Axes come from the longest stride to the shortest; of each only the few multiples are tried
+// that the shorter ones can still bring there.  Layouts that take more than `budget` tries (strides of
+// about the same length, over long axes) are taken to overlap.
+struct Sums {
+  struct Axis { long long s, lo, hi; } ax[6];
+  int axes = 0;
+  long long before, after;
+  int budget = 4096;
+
+  void add(long long s, long long lo, long long hi) {
+    if (s == 0 || (lo == 0 && hi == 0)) return;
+    for (int i = 0; i < axes; ++i)
+      if (ax[i].s == s) {
+        ax[i].lo += lo, ax[i].hi += hi;
+        return;
+      }
+    int at = axes++;
+    for (; at > 0 && ax[at - 1].s < s; --at) ax[at] = ax[at - 1];
+    ax[at] = Axis{s, lo, hi};
+  }
+  static long long floor_div(long long a, long long b) { return a / b - (a % b < 0); }
+  bool meet(long long c, int i = 0, bool zero = false) {  // zero: all k 0 so far, which does not count
+    if (i == axes) return !zero && c > -before && c < after;
+    if (--budget < 0) return true;
+    long long least = 0, most = 0;
+    for (int j = i + 1; j < axes; ++j) least += ax[j].lo * ax[j].s, most += ax[j].hi * ax[j].s;
+    const long long k0 = std::max(ax[i].lo, -floor_div(c + most + before - 1, ax[i].s));
+    const long long k1 = std::min(ax[i].hi, floor_div(after - 1 - c - least, ax[i].s));
+    for (long long k = k0; k <= k1; ++k)
+      if (meet(c + k * ax[i].s, i + 1, zero && k == 0)) return true;
+    return false;
+  }
+};
+
+int check_regions(const char* fn, const Region& a, const Region& b) {
+  if (!a.p || !b.p || a.p + a.end() <= b.p || b.p + b.end() <= a.p) return QLIN_OK;
+  Sums d;
+  d.before = a.width, d.after = b.width;
+  for (int i = 0; i < 3; ++i) {
+    d.add(a.s[i], 0, a.n[i] - 1);
+    d.add(b.s[i], -(b.n[i] - 1), 0);
+  }
+  if (d.meet(a.p - b.p)) return fail(QLIN_ERR_INVALID, "%s: %s overlaps %s", fn, a.name, b.name);
+  return QLIN_OK;
+}
+
+// A cache's keys, values and scales.
+struct CacheRegions {
+  Region r[4];
+  int n;
+};
+CacheRegions cache_regions(const qlin_paged_kv* c, int hkv, int hd) {
+  const int es = c->dtype == QLIN_I8 ? 1 : 2;
+  CacheRegions x = {{region("k_cache", c->k, es, hd, c->num_pages, c->k_page, c->page, c->k_token, hkv, c->k_head),
+                     region("v_cache", c->v, es, hd, c->num_pages, c->v_page, c->page, c->v_token, hkv, c->v_head)},
+                    2};
+  if (c->dtype == QLIN_I8) {
+    x.r[2] = region("k_s", c->k_s, 4, 1, c->num_pages, c->ks_page, c->page, c->ks_token, hkv, c->ks_head);
+    x.r[3] = region("v_s", c->v_s, 4, 1, c->num_pages, c->vs_page, c->page, c->vs_token, hkv, c->vs_head);
+    x.n = 4;
+  }
+  return x;
+}
+int check_cache_apart(const char* fn, const Region& a, const qlin_paged_kv* c, int hkv, int hd) {
+  const CacheRegions x = cache_regions(c, hkv, hd);
+  for (int i = 0; i < x.n; ++i) QA_TRY(check_regions(fn, a, x.r[i]));
+  return QLIN_OK;
+}
+
 // The partial sums' place in the workspace, behind its counters and exchange slots.
 int workspace_parts(const char* fn, void* ws, size_t bytes, char** part, size_t* avail) {
   const size_t base = counter_bytes() + poll_bytes();
@@ -292,6 +381,30 @@ int qlin_qk_norm_rope(const qlin_rope* r, const qlin_paged_kv* cache, void* stre
   a.T = r->T, a.HQ = r->q_heads, a.HKV = r->kv_heads, a.hd = r->hd, a.rot = r->rot;
   a.axes = r->axes, a.interleaved = r->interleaved, a.dt = r->dtype;
   for (int i = 0; i < 3; ++i) a.sec[i] = i < r->axes ? r->sections[i] : 0;
+  // What is written, and what it may be: q_out q itself, k_out k itself (each head is read before it is
+  // written, by the same threads).
+  const Region q = region("q", r->q, 2, r->hd, r->T, r->q_token, r->q_heads, r->q_head);
+  const Region k = region("k", r->k, 2, r->hd, r->T, r->k_token, r->kv_heads, r->k_head);
+  const Region v = region("v", a.v, 2, r->hd, r->T, r->v_token, r->kv_heads, r->v_head);
+  const Region qo = region("q_out", r->q_out, 2, r->hd, r->T, r->qo_token, r->q_heads, r->qo_head);
+  const Region ko = region("k_out", r->k_out, 2, r->hd, r->T, r->ko_token, r->kv_heads, r->ko_head);
+  auto same = [](const Region& x, const Region& y) { return x.p == y.p && x.s[0] == y.s[0] && x.s[1] == y.s[1]; };
+  if (!same(qo, q)) QA_TRY(check_regions(fn, qo, q));
+  QA_TRY(check_regions(fn, qo, k));
+  QA_TRY(check_regions(fn, qo, v));
+  if (r->k_out) {
+    if (!same(ko, k)) QA_TRY(check_regions(fn, ko, k));
+    QA_TRY(check_regions(fn, ko, q));
+    QA_TRY(check_regions(fn, ko, v));
+    QA_TRY(check_regions(fn, ko, qo));
+  }
+  if (cache) {
+    const CacheRegions x = cache_regions(cache, r->kv_heads, r->hd);
+    for (int i = 0; i < x.n; ++i) {
+      for (const Region* y : {&q, &k, &v, &qo, &ko}) QA_TRY(check_regions(fn, *y, x.r[i]));
+      for (int j = 0; j < i; ++j) QA_TRY(check_regions(fn, x.r[j], x.r[i]));
+    }
+  }
   return status(fn, launch_rope(a, (hipStream_t)stream));
 }
 
@@ -326,6 +439,12 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void*
   a.cu = cu_q, a.T = T, a.B = B, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
   QA_TRY(plan_prompt(fn, a, hd, Tk, workspace, workspace_bytes));
+  const Region to = region("out", out, 2, hd, T, o_token, q_heads, o_head);
+  QA_TRY(check_regions(fn, to, region("q", q, 2, hd, T, q_token, q_heads, q_head)));
+  if (Tk > 0) {
+    QA_TRY(check_regions(fn, to, region("k", k, 2, hd, Tk, k_token, kv_heads, k_head)));
+    QA_TRY(check_regions(fn, to, region("v", v, 2, hd, Tk, v_token, kv_heads, v_head)));
+  }
   return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
 }
 
@@ -354,6 +473,9 @@ int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const
   a.cu = cu_q, a.T = T, a.B = B, a.HKV = kv_heads, a.G = q_heads / kv_heads;
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
   QA_TRY(plan_prompt(fn, a, hd, (long long)max_pages * cache->page, workspace, workspace_bytes));
+  const Region to = region("out", out, 2, hd, T, o_token, q_heads, o_head);
+  QA_TRY(check_regions(fn, to, region("q", q, 2, hd, T, q_token, q_heads, q_head)));
+  QA_TRY(check_cache_apart(fn, to, cache, kv_heads, hd));
   return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
 }
 
@@ -394,6 +516,9 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   if ((target + B + 2) * hg * slot > (long long)avail || B * hg * kDecodeCounters * 4 > (long long)counter_bytes())
     target = 0;
   QA_TRY(check_grid(fn, (target + B + 2) * hg));
+  const Region to = region("out", out, 2, hd, B, o_seq, q_heads, o_head);
+  QA_TRY(check_regions(fn, to, region("q", q, 2, hd, B, q_seq, q_heads, q_head)));
+  QA_TRY(check_cache_apart(fn, to, cache, kv_heads, hd));
   a.target = (int)target;
   a.few = (int)std::min(std::max(1LL, few / hg), std::max(1LL, target));
   a.units = (int)(target + B + (target ? 2 : 0));  // (two for what the device's estimate rounds)

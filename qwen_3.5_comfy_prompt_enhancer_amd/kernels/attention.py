@@ -24,7 +24,8 @@ int8 codes with fp32 scales k_s / v_s [pages, page, kv_heads].  16-bit tensors n
 16-byte aligned rows (strides that are multiples of 8; int8: of 16; of tokens at most 2^26
 elements, of heads and pages 2^31 - 16).
 
-Lengths, page tables, slots and positions stay on the device and are never waited for;
+What a call writes shares no memory with what it reads (`qk_norm_rope` in place aside): such calls are
+refused.  Lengths, page tables, slots and positions stay on the device and are never waited for;
 what they may hold is stated in include/qlin_attn.h.  All calls run on the current
 stream of their tensors' device and can be captured (see `qlin.capture`).
 """
@@ -260,7 +261,7 @@ def attn_prompt(q, k, v, cu_q, out, cu_k=None, scale=None, causal=True):
     [Tk, kv_heads, hd].  cu_q, cu_k: int32 [B + 1], rising from 0.  `causal`: query i of a
     sequence sees its keys j <= i + keys - queries (the last query sees all).  scale:
     hd ** -0.5 unless given.  out [T, q_heads, hd]; a row that sees no key is zero, rows of
-    no sequence stay as they were.  out must not overlap q, k or v.  Returns out."""
+    no sequence stay as they were.  Returns out."""
     T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must both be [rows, kv_heads, hd]")

@@ -68,3 +68,62 @@ def test_a_table_of_no_pages(tmp):
     _accepted(tmp, D.decode(kv, table=None, max_pages=0), D.paged(kv, table=None, max_pages=0))
     _refused(tmp, "null page table", D.decode(kv, table=None), D.paged(kv, table=None),
              D.decode(kv, table=None, max_pages=0, kv_len=None))
+
+
+def test_outputs_next_to_inputs(tmp):
+    """Columns of one buffer's rows, in any order, and the planes of one cache."""
+    row = 8 * 128 + 2 * 4 * 64            # heads of a query and a gate, keys, values
+    k0 = D.Q + 2 * 8 * 128
+    _accepted(tmp,
+              D.prompt(qt=row, qh=128, k=k0, kt=row, v=k0 + 2 * 256, vt=row, out=D.Q + 2 * 64, ot=row, oh=128),
+              D.prompt(out=D.Q + 9 * 512 * 2), D.prompt(out=D.K - 9 * 512 * 2), D.decode(D.cache(4, 64), out=D.Q + 2048),
+              # q_out and k_out in place, or q_out in the gates' columns
+              D.rope(q_token=row, q_head=128, q_out=D.Q, qo_token=row, qo_head=128, k=k0, k_token=row, k_out=k0,
+                     ko_token=row, v=k0 + 512, v_token=row),
+              D.rope(q_token=row, q_head=128, q_out=D.Q + 128, qo_token=row, qo_head=128, k=k0, k_token=row),
+              # keys and values of a page next to each other, or of a token, or of a head
+              D.rope(D.cache(4, 64, v=D.K + 2 * 64 * 256, k_page=2 * 64 * 256, v_page=2 * 64 * 256)),
+              D.rope(D.cache(4, 64, v=D.K + 2 * 256, k_page=128 * 256, k_token=512, v_page=128 * 256, v_token=512)),
+              D.rope(D.cache(4, 64, v=D.K + 2 * 64, k_page=128 * 256, k_token=512, k_head=128, v_page=128 * 256,
+                             v_token=512, v_head=128)))
+
+
+def test_outputs_that_lie_in_inputs(tmp):
+    kv, kv8 = D.cache(4, 64), D.cache(4, 64, dtype=D.I8)
+    _refused(tmp, "out overlaps q", D.prompt(out=D.Q + 512 * 2), D.prompt(out=D.Q - 2 * 512 * 2 + 16),
+             D.decode(kv, out=D.Q + 1024), D.paged(kv, out=D.Q + 16))
+    _refused(tmp, "out overlaps k", D.prompt(out=D.K), D.prompt(out=D.K + 256), D.paged(kv, out=D.K + (1 << 17)),
+             D.decode(kv8, out=D.K))
+    _refused(tmp, "out overlaps v", D.prompt(out=D.V + 128 * 4), D.decode(kv, out=D.V))
+    _refused(tmp, "out overlaps k_s", D.decode(kv8, out=D.KS + 512))
+    _refused(tmp, "overlaps q", D.rope(q_out=D.Q + 1024), D.rope(q_out=D.Q, qo_token=1024), D.rope(k_out=D.Q))
+    _refused(tmp, "overlaps k", D.rope(q_out=D.K), D.rope(k_out=D.K + 512), D.rope(k_out=D.K, ko_token=512))
+    _refused(tmp, "overlaps v", D.rope(kv, k_out=D.V + (1 << 43)), D.rope(kv, q_out=D.V + (1 << 43) + 64))
+    _refused(tmp, "overlaps q_out", D.rope(k_out=D.OUT + 128))
+    _refused(tmp, "overlaps v_cache", D.rope(D.cache(4, 64, k=D.V)), D.rope(D.cache(4, 64, k=D.V + 256)))
+    _refused(tmp, "overlaps v_s", D.rope(D.cache(4, 64, dtype=D.I8, k_s=D.VS)))
+    _refused(tmp, "overlaps k_cache", D.rope(kv, q=D.K), D.rope(kv, k_out=D.K + 4096))
+
+
+def test_overlaps_are_found_as_by_counting(tmp):
+    """Random layouts of a few rows and heads: refused where some byte belongs to both, and only there."""
+    import random
+    rng = random.Random(5)
+    calls, want = [], []
+    while len(calls) < 400:
+        B, hq, hkv = rng.randint(1, 4), rng.choice([1, 2, 4]), 1
+        row = [64 * rng.randint(1, 9) + rng.choice([0, 0, 8, 24]) for _ in range(2)]
+        head = [64 * rng.randint(1, 9) + rng.choice([0, 0, 8, 40]) for _ in range(2)]
+        if rng.random() < 0.5:
+            row[1], head[1] = row[0], head[0]
+        at = 8 * rng.randint(-300, 300)
+        a, b = ({o + b * r + h * s + e for b in range(B) for h in range(hq) for e in range(64)}
+                for o, r, s in ((0, row[0], head[0]), (at, row[1], head[1])))
+        if at == 0 or len(b) != B * hq * 64:
+            continue
+        calls.append(D.decode(D.cache(hkv, 64), B=B, hq=hq, hkv=hkv, qs=row[0], qh=head[0], out=D.Q + 2 * at, os=row[1],
+                              oh=head[1]))
+        want.append(bool(a & b))
+    assert 40 < sum(want) < 360
+    for call, bad, (status, launches, msg) in zip(calls, want, D.run(tmp, calls)):
+        assert (status < 0 and "out overlaps q" in msg and not launches) if bad else (status == 0 and launches), (call, msg)
