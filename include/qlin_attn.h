@@ -25,7 +25,8 @@
  *     key; elsewhere infinities and NaN go through the formulas;
  *   - row bounds (cu) are clamped to the rows there are, and query bounds that fall count as the
  *     highest before them.
- * What a call writes shares no byte with what it reads or else writes (q_out that is q and k_out that
+ * Rows, heads and pages of what a call writes do not overlap, and it shares no byte with what the call
+ * reads or else writes (q_out that is q and k_out that
  * is k aside, with the same strides): such calls are refused.  Tensors may lie between each other's
  * rows, heads or pages; where they do so with strides that are different but about the same length,
  * over long axes, they are taken to overlap.

@@ -228,6 +228,21 @@ int check_regions(const char* fn, const Region& a, const Region& b) {
   return QLIN_OK;
 }
 
+// Whether runs of one region share bytes.
+int check_region(const char* fn, const Region& a) {
+  Sums d;
+  d.before = d.after = a.width;
+  for (int i = 0; i < 3; ++i)
+    if (a.n[i] > 1) {
+      if (a.s[i] < a.width) return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, a.name);
+      for (int j = 0; j < i; ++j)  // (two axes of one stride: index (0, 1) is (1, 0))
+        if (a.n[j] > 1 && a.s[j] == a.s[i]) return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, a.name);
+      d.add(a.s[i], 1 - a.n[i], a.n[i] - 1);
+    }
+  if (d.meet(0, 0, true)) return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, a.name);
+  return QLIN_OK;
+}
+
 // A cache's keys, values and scales.
 struct CacheRegions {
   Region r[4];
@@ -389,10 +404,12 @@ int qlin_qk_norm_rope(const qlin_rope* r, const qlin_paged_kv* cache, void* stre
   const Region qo = region("q_out", r->q_out, 2, r->hd, r->T, r->qo_token, r->q_heads, r->qo_head);
   const Region ko = region("k_out", r->k_out, 2, r->hd, r->T, r->ko_token, r->kv_heads, r->ko_head);
   auto same = [](const Region& x, const Region& y) { return x.p == y.p && x.s[0] == y.s[0] && x.s[1] == y.s[1]; };
+  QA_TRY(check_region(fn, qo));
   if (!same(qo, q)) QA_TRY(check_regions(fn, qo, q));
   QA_TRY(check_regions(fn, qo, k));
   QA_TRY(check_regions(fn, qo, v));
   if (r->k_out) {
+    QA_TRY(check_region(fn, ko));
     if (!same(ko, k)) QA_TRY(check_regions(fn, ko, k));
     QA_TRY(check_regions(fn, ko, q));
     QA_TRY(check_regions(fn, ko, v));
@@ -401,6 +418,7 @@ int qlin_qk_norm_rope(const qlin_rope* r, const qlin_paged_kv* cache, void* stre
   if (cache) {
     const CacheRegions x = cache_regions(cache, r->kv_heads, r->hd);
     for (int i = 0; i < x.n; ++i) {
+      QA_TRY(check_region(fn, x.r[i]));
       for (const Region* y : {&q, &k, &v, &qo, &ko}) QA_TRY(check_regions(fn, *y, x.r[i]));
       for (int j = 0; j < i; ++j) QA_TRY(check_regions(fn, x.r[j], x.r[i]));
     }
@@ -440,6 +458,7 @@ int qlin_attn_prompt(const void* q, int64_t q_token, int64_t q_head, const void*
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
   QA_TRY(plan_prompt(fn, a, hd, Tk, workspace, workspace_bytes));
   const Region to = region("out", out, 2, hd, T, o_token, q_heads, o_head);
+  QA_TRY(check_region(fn, to));
   QA_TRY(check_regions(fn, to, region("q", q, 2, hd, T, q_token, q_heads, q_head)));
   if (Tk > 0) {
     QA_TRY(check_regions(fn, to, region("k", k, 2, hd, Tk, k_token, kv_heads, k_head)));
@@ -474,6 +493,7 @@ int qlin_attn_prompt_paged(const void* q, int64_t q_token, int64_t q_head, const
   a.causal = causal, a.c = scale * 1.44269504088896340736f;
   QA_TRY(plan_prompt(fn, a, hd, (long long)max_pages * cache->page, workspace, workspace_bytes));
   const Region to = region("out", out, 2, hd, T, o_token, q_heads, o_head);
+  QA_TRY(check_region(fn, to));
   QA_TRY(check_regions(fn, to, region("q", q, 2, hd, T, q_token, q_heads, q_head)));
   QA_TRY(check_cache_apart(fn, to, cache, kv_heads, hd));
   return status(fn, launch_prompt(a, dtype, hd, (hipStream_t)stream));
@@ -517,6 +537,7 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
     target = 0;
   QA_TRY(check_grid(fn, (target + B + 2) * hg));
   const Region to = region("out", out, 2, hd, B, o_seq, q_heads, o_head);
+  QA_TRY(check_region(fn, to));
   QA_TRY(check_regions(fn, to, region("q", q, 2, hd, B, q_seq, q_heads, q_head)));
   QA_TRY(check_cache_apart(fn, to, cache, kv_heads, hd));
   a.target = (int)target;

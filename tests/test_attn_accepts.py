@@ -127,3 +127,32 @@ def test_overlaps_are_found_as_by_counting(tmp):
     assert 40 < sum(want) < 360
     for call, bad, (status, launches, msg) in zip(calls, want, D.run(tmp, calls)):
         assert (status < 0 and "out overlaps q" in msg and not launches) if bad else (status == 0 and launches), (call, msg)
+
+
+def test_outputs_that_overlap_themselves(tmp):
+    """Strides that are each long enough, but lead to the same place in two ways."""
+    _refused(tmp, "rows of out overlap", D.prompt(ot=64, oh=64), D.prompt(ot=64, oh=256), D.prompt(ot=128, oh=192),
+             D.decode(D.cache(4, 64), os=64, oh=64), D.paged(D.cache(4, 64), ot=512, oh=72 * 64 + 8 - 4 * 512))
+    _refused(tmp, "rows of q_out overlap", D.rope(qo_token=64, qo_head=64))
+    _refused(tmp, "rows of k_out overlap", D.rope(ko_token=128, ko_head=192))
+    _refused(tmp, "rows of k_cache overlap", D.rope(D.cache(4, 64, k_page=64 * 128)), D.rope(D.cache(4, 64, k_token=64)))
+    _refused(tmp, "rows of v_s overlap", D.rope(D.cache(4, 64, dtype=D.I8, vs_token=2)))
+    # heads before tokens, tokens before pages, gaps
+    _accepted(tmp, D.prompt(ot=64, oh=9 * 64), D.prompt(ot=192, oh=9 * 192 + 8), D.prompt(T=2, hq=4, ot=192, oh=2 * 192),
+              D.rope(D.cache(4, 64, k_page=64, k_token=8 * 64, k_head=8 * 64 * 64)),
+              D.rope(D.cache(4, 64, dtype=D.I8, vs_page=1, vs_token=8, vs_head=512)), D.prompt(T=2, hq=4, ot=192, oh=128))
+
+
+def test_overlaps_within_are_found_as_by_counting(tmp):
+    import random
+    rng = random.Random(6)
+    calls, want = [], []
+    for _ in range(400):
+        T, hq = rng.randint(1, 6), rng.choice([1, 2, 4, 8])
+        row, head = (64 + 8 * rng.randint(0, 70) for _ in range(2))
+        runs = [t * row + h * head for t in range(T) for h in range(hq)]
+        calls.append(D.prompt(T=T, hq=hq, hkv=1, B=1, ot=row, oh=head))
+        want.append(len({o + e for o in runs for e in range(0, 64, 8)}) < len(runs) * 8)
+    assert 40 < sum(want) < 360
+    for call, bad, (status, launches, msg) in zip(calls, want, D.run(tmp, calls)):
+        assert (status < 0 and "rows of out overlap" in msg and not launches) if bad else (status == 0 and launches), (call, msg)
