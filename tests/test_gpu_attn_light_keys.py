@@ -1,16 +1,5 @@
 """One key far above very many others, with a value of zero as an attention sink has: the output is of the
-others alone, each of whose weights is a small part of the sink's (fp16 has five bits of exponent).
-
-Allowed error, u = half a step, e = 2^-24, A = sum_j p_j |v_j| / sum_j p_j, S = scale max_j |q| . |k_j|:
-
-* the output's rounding u |o| (2^-25 where it is subnormal) and P's u A;
-* 32 bits: a score's products and sums move every p by a factor exp(+-(hd + 4) e S), exponentials and
-  rescaling by 16 e, sums by `ADDS` e for O and for the sum of P each.  ADDS bounds the additions that one
-  value goes through: 32 keys of a product, a unit's blocks a wave (decode 8 of 32, prompts at most 2^15 / 192
-  = 171 at 2^20 keys), the joins of waves and parts (at most 448 + 4);
-* keys in the sink's own block are taken against a reference that puts the sink at 2^8 at least, where a
-  subnormal is off by at most 2^-25: 32 2^-33 of the sink's P, of the largest value there.
-"""
+others alone, each of whose weights is a small part of the sink's (fp16 has five bits of exponent)."""
 from __future__ import annotations
 
 import math
@@ -18,12 +7,12 @@ import math
 import pytest
 import torch
 
+import attn_far as F
 import attn_ref as R
 
 pytestmark = pytest.mark.gpu
 
 BF, FP = torch.bfloat16, torch.float16
-ADDS = 32 + 171 + 452
 
 
 def _inputs(n, hd, at, octaves, dt, seed, rows=1, G=4):
@@ -42,32 +31,14 @@ def _inputs(n, hd, at, octaves, dt, seed, rows=1, G=4):
 
 def _check(out, q, k, v, dt, name):
     """One row [G, hd] against 64 bits."""
-    hd = q.shape[-1]
-    scale, u = hd ** -0.5, R.half_step(dt)
-    qd, kd, vd = q.double(), k[:, 0].double(), v[:, 0].double()
-    s = qd @ kd.t() * scale
-    p = torch.exp(s - s.amax(1, keepdim=True))
-    l = p.sum(1, keepdim=True)
-    o, A = p @ vd / l, p @ vd.abs() / l
-    S = (qd.abs() @ kd.abs().t() * scale).amax(1, keepdim=True)
-    tol = u * o.abs() + A * (u + 2 * (hd + 4) * R.E32 * S + (16 + 2 * ADDS) * R.E32)
-    if dt == FP:
-        tol = tol + 2.0 ** -25 + 32 * 2.0 ** -33 / l * vd.abs().max()
+    o, tol, _ = F.row(q, k[:, 0], v[:, 0], dt)
     assert (o.abs() > 4 * tol).float().mean() > 0.9, f"{name}: the tolerance does not tell a zero"
     R.check(out, o, tol, name)
 
 
 def _paged(k, v, page, seed):
-    n, pages = k.shape[0], -(-k.shape[0] // page)
-    g = torch.Generator(device="cuda").manual_seed(seed)
-    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)[None]
-    cache = []
-    for x in (k, v):
-        c = torch.zeros((pages, page, 1, k.shape[2]), dtype=k.dtype, device="cuda")
-        i = torch.arange(n, device="cuda")
-        c[table[0].long()[i // page], i % page] = x
-        cache.append(c)
-    return cache, table
+    c, table = F.paged(k[:, 0], v[:, 0], page, seed)
+    return c[:2], table
 
 
 def _ints(*x):
