@@ -85,6 +85,15 @@ def _call(name, device, *args):
         C.check(status, name)
 
 
+_INT_MAX = (1 << 31) - 1  # of the ABI's sizes: a ctypes int keeps 32 bits of a larger one
+
+
+def _size(name, n):
+    if n > _INT_MAX:
+        raise ValueError(f"{name}: {n} is more than {_INT_MAX}")
+    return n
+
+
 def _strides(name, t, rows, heads, hd, dtype):
     """Row and head strides of a [rows, heads, hd] tensor of 16-bit values whose last axis is
     contiguous."""
@@ -112,6 +121,8 @@ def _queries(q):
     st = q.stride()
     if st[2] != 1:
         raise ValueError("the last axis of q must be contiguous")
+    if shape[0] > _INT_MAX or shape[1] > _INT_MAX:
+        _size("rows and heads of q", max(shape))
     return *shape, dt, st[0], st[1]
 
 
@@ -142,6 +153,8 @@ def _table(table, kv_len, B):
     if table.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
         raise ValueError("table must be int32 with a contiguous last axis")
     _vector("kv_len", kv_len, B)
+    if shape[1] > _INT_MAX:
+        _size("pages of a table's row", shape[1])
     return st[0], shape[1]
 
 
@@ -157,6 +170,8 @@ def _cache(k, v, k_s, v_s, dtype, hd):
     ks, vs = k.stride(), v.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the last axis of the cache must be contiguous")
+    if shape[0] > _INT_MAX or shape[2] > _INT_MAX:
+        _size("pages and heads of the cache", max(shape))
     if k.dtype == dtype:
         if k_s is not None or v_s is not None:
             raise ValueError("a 16-bit cache has no scales")
@@ -265,13 +280,13 @@ def attn_prompt(q, k, v, cu_q, out, cu_k=None, scale=None, causal=True):
     T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must both be [rows, kv_heads, hd]")
-    Tk, hkv = k.shape[0], k.shape[1]
+    Tk, hkv = _size("rows of k", k.shape[0]), _size("heads of k", k.shape[1])
     kt, kh = _strides("k", k, Tk, hkv, hd, q.dtype)
     vt, vh = _strides("v", v, Tk, hkv, hd, q.dtype)
     ot, oh = _strides("out", out, T, hq, hd, q.dtype)
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q must be [sequences + 1]")
-    B = cu_q.shape[0] - 1
+    B = _size("sequences", cu_q.shape[0] - 1)
     _vector("cu_q", cu_q, B + 1)
     if cu_k is None:
         if Tk != T:
@@ -297,7 +312,7 @@ def attn_prompt_paged(q, k_cache, v_cache, table, kv_len, cu_q, out, k_s=None, v
     ot, oh = _strides("out", out, T, hq, hd, q.dtype)
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q must be [sequences + 1]")
-    B = cu_q.shape[0] - 1
+    B = _size("sequences", cu_q.shape[0] - 1)
     _vector("cu_q", cu_q, B + 1)
     tb, pages = _table(table, kv_len, B)
     C.require_cuda(q, k_cache, v_cache, table, kv_len, cu_q, out, k_s, v_s)

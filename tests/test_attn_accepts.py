@@ -3,6 +3,7 @@ would be launched is recorded, nothing runs."""
 from __future__ import annotations
 
 import pytest
+import torch
 
 import attn_dispatch as D
 
@@ -156,3 +157,26 @@ def test_overlaps_within_are_found_as_by_counting(tmp):
     assert 40 < sum(want) < 360
     for call, bad, (status, launches, msg) in zip(calls, want, D.run(tmp, calls)):
         assert (status < 0 and "rows of out overlap" in msg and not launches) if bad else (status == 0 and launches), (call, msg)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """A ctypes int keeps the low 32 bits of what it is given: 2^32 + 5 rows would be 5."""
+    from qwen35_amd.kernels import attention as A
+    far = (1 << 32) + 5
+
+    def t(*shape, dt=torch.bfloat16):
+        return torch.empty(shape, dtype=dt, device="meta")
+
+    q, k, kv, n, cu = t(2, 8, 64), t(2, 4, 64), t(4, 16, 4, 64), t(2, dt=torch.int32), t(3, dt=torch.int32)
+    table = t(2, 3, dt=torch.int32)
+    for call in (lambda: A.attn_prompt(q, t(far, 4, 64), t(far, 4, 64), cu, q, cu_k=cu),
+                 lambda: A.attn_prompt(t(far, 8, 64), k, k, cu, t(far, 8, 64), cu_k=cu),
+                 lambda: A.attn_prompt(q, k, k, t(far, dt=torch.int32), q),
+                 lambda: A.attn_decode(t(far, 8, 64), kv, kv, table, n, t(far, 8, 64)),
+                 lambda: A.attn_decode(q, t(far, 16, 4, 64), t(far, 16, 4, 64), table, n, q),
+                 lambda: A.attn_decode(q, kv, kv, t(2, far, dt=torch.int32), n, q),
+                 lambda: A.attn_prompt_paged(q, kv, kv, t(2, far, dt=torch.int32), n, cu, q),
+                 lambda: A.qk_norm_rope(t(far, 8, 64), t(far, 4, 64), t(far, dt=torch.int64),
+                                        t(16, dt=torch.float32), t(far, 8, 64), t(far, 4, 64))):
+        with pytest.raises(ValueError, match="is more than"):
+            call()
