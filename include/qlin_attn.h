@@ -12,9 +12,10 @@
  * Strides are in elements; the last axis (hd values) is contiguous.  Every 16-bit tensor
  * is 16-byte aligned with strides that are multiples of 8; int8 tensors have strides that
  * are multiples of 16.  Strides of tokens are at most 2^26, of heads and pages 2^31 - 16 (of an
- * int8 cache's scales 2^30 - 8); that of an axis of one is not looked at.  hd is 64, 128 or 256; a key head has at most 64 query heads, a call
- * at most 65536 query heads, 2^24 - 1 tokens and 65536 sequences, a sequence 2^30 keys.  Lengths, page tables, slots and positions are
- * read on the device:
+ * int8 cache's scales 2^30 - 8); that of an axis of one is not looked at.  hd is 64, 128 or 256;
+ * a key head has at most 64 query heads, a call at most 65536 query heads, 2^24 - 1 tokens and 65536
+ * sequences, a sequence 2^30 keys.  scale is a positive number.  Lengths, page tables, slots and
+ * positions are read on the device:
  *   - a slot below 0 or past the cache stores nothing (a padded row); the others of a call
  *     differ: what a slot given twice holds is of no one token;
  *   - kv_len below 0 counts as 0, above what the table's row holds as that;
@@ -25,11 +26,10 @@
  *     key; elsewhere infinities and NaN go through the formulas;
  *   - row bounds (cu) are clamped to the rows there are, and query bounds that fall count as the
  *     highest before them.
- * Rows, heads and pages of what a call writes do not overlap, and it shares no byte with what the call
- * reads or else writes (q_out that is q and k_out that
- * is k aside, with the same strides): such calls are refused.  Tensors may lie between each other's
- * rows, heads or pages; where they do so with strides that are different but about the same length,
- * over long axes, they are taken to overlap.
+ * Rows, heads and pages of what a call writes do not overlap, and it shares no byte with what the
+ * call reads or else writes (q_out that is q and k_out that is k aside, with the same strides): such
+ * calls are refused.  Tensors may lie between each other's rows, heads or pages; where they do so with
+ * strides that are different but about the same length, over long axes, they are taken to overlap.
  */
 #ifndef QLIN_ATTN_H
 #define QLIN_ATTN_H

@@ -48,7 +48,7 @@ EXTRA = {
     "prefill_w4_f16.hip": _VGPR_FORM,
     "prefill_w4_bf16.hip": _VGPR_FORM,
     "prefill_w4_f32.hip": _VGPR_FORM,
-    # the same for prompt attention's 256 accumulators and 128 query registers per lane
+    # the same for prompt attention's 128 accumulators and 64 query registers per lane (heads of 256 values)
     "attn_prompt_bf16.hip": _VGPR_FORM,
     "attn_prompt_f16.hip": _VGPR_FORM,
 }

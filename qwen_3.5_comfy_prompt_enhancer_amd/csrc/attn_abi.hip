@@ -283,7 +283,8 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   QA_TRY(workspace_parts(fn, ws, ws_bytes, &part, &avail));
   // Units: about as many as run at once (two, three or four workgroups a CU by head size), fewer
   // where their sums are the larger; 8192 tokens, 256 values, 384 / 448 / 512 / 640 units: 315 (not
-  // cut) / 258 / 265 / 283 us.
+  // cut) / 258 / 265 / 283 us; 8192 tokens of 8 heads, 128 values, not cut / 384 / 448 / 512 / 576 / 640:
+  // 196 / 193 / 170 / 181 / 174 / 165, 64 values, not cut / 448 / 512 / 640 / 768: 138 / 115 / 122 / 110 / 112.
   a.rows = kPromptRows;
   long long target = hd == 256 ? 448 : hd == 128 ? 512 : 640;
   // Few tiles (of 16-bit keys) are halved, two groups of waves sharing their keys: 512 tokens 20.8
@@ -320,7 +321,9 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   a.target = (int)target;
   a.tiles = (int)tiles;
   // A second launch joins where parts are many (see prompt_join_kernel): not where sequences of the average
-  // length are too short for a cut (a launch that finds nothing to join costs 3 us), nor for halved
+  // length are too short for a cut (a launch that finds nothing to join costs 3 us), with an eighth for
+  // batches of which only the longest is cut (1100, 950 and 800 tokens, this line / without the eighth: 37.8 /
+  // 47.3 us, 1300, 900 and 600 37.2 / 44.3, three of 950, which are not cut, 41.4 / 38.4), nor for halved
   // tiles of small heads, whose few small parts their last one joins as quickly (1300 tokens, a
   // launch / the last part: 64 values 15.2 / 13.4 us, 128 20.2 / 18.4, 256 31.8 / 32.8).
   const long long average = a.kv.table ? max_keys : max_keys / a.B;

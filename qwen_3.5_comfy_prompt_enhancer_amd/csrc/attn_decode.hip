@@ -21,7 +21,7 @@
 //     that column c of all lanes is an A operand of 16 value columns;
 //   * int8: codes become 16-bit whole numbers (exact); a key's scale multiplies its scores in 32
 //     bits, a value's scale its probability.
-// The running maximum is a column's, hence a lane's own.  P is rounded to 16 bits for its
+// The running maximum (the reference that P is taken against) is a column's, hence a lane's own.  P is rounded to 16 bits for its
 // product (half a step of 2^-8 or 2^-11 of each term; the sum of P is of the unrounded); in fp16 it is
 // taken against a reference that keeps a block's largest P between 2^4 and 2^15, as light keys would
 // else leave fp16's range (fp16_reference).  With int8 values P times scale goes as the sum of two bf16
@@ -29,8 +29,8 @@
 //
 // Waves join through LDS, units of a sequence through memory: the last of 16 units to arrive
 // adds their parts in unit order, the last of those groups adds the groups', so that the result
-// does not depend on the order of arrival and no workgroup reads more than 16 parts (or as many as it
-// takes to keep a sequence's groups within its counters).
+// does not depend on the order of arrival.  A group has 16 parts, or as many as it takes to keep a
+// sequence's groups within its counters, and the last join one sum of each of up to 31 groups.
 #include "attn_dev.h"
 
 namespace qlin {

@@ -80,7 +80,7 @@ struct DecodeArgs {
   float* part;            // unit partials
   unsigned* cnt;          // arrival counters, zero between calls
 };
-// A part: rows x hd sums of 32 bits, then (maximum, sum of P, 0, 0) of each row.
+// A part: rows x hd sums of 32 bits, then (reference of P, sum of P, 0, 0) of each row.
 __host__ __device__ constexpr int decode_slot_floats(int rows, int hd) { return rows * hd + rows * 4; }
 constexpr int kDecodeBlock = 32;     // keys a wave takes at a time
 constexpr int kDecodeChunk = 4;      // blocks of a unit come in multiples of this (one per wave)
@@ -117,7 +117,7 @@ constexpr int kPromptFill = 3000;    // (tile, block) pairs that fill the chip w
 constexpr int kPromptJoinApart = 256;  // row tiles of all key heads up to which a second launch joins
 constexpr int kPromptCounters = 32;  // counters of a (key head, row tile)
 constexpr int kPromptRows = 128;     // rows of a tile: tokens x the query heads of a key head
-// a unit's partial: sums of its rows, then (maximum, sum of P) of each
+// a unit's partial: sums of its rows, then (reference of P, sum of P) of each
 __host__ __device__ constexpr long long prompt_slot_floats(int hd, int rows) { return (long long)rows * (hd + 2); }
 hipError_t launch_prompt(const PromptArgs& a, int dt, int hd, hipStream_t st);
 hipError_t launch_prompt_bf16(const PromptArgs& a, int hd, hipStream_t st);

@@ -25,7 +25,7 @@
 //     2^-8 .. 2^15 on either side (fp16_reference).  P is rounded to the queries' type for its product;
 //     its sum, the maximum and O are 32-bit.
 //
-// What bounds it: the MFMAs (of 256 values, 32 of 32 cycles a block and wave), then the softmax's
+// What bounds it: the MFMAs (of 256 values, 32 products of 32 cycles a block and wave), then the softmax's
 // vector work and LDS.  32 rows a wave, operands read three products ahead and two workgroups a CU (256
 // values; three or four of smaller heads) took 310 us for an 8192-token prompt of 8 heads of 256 values
 // where 64 rows a wave, each operand feeding two MFMAs, took 696: two waves a SIMD hide each other's

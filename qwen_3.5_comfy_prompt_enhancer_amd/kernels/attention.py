@@ -274,8 +274,8 @@ def attn_prompt(q, k, v, cu_q, out, cu_k=None, scale=None, causal=True):
     """Attention of packed prompts: sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1
     of q [T, q_heads, hd], its keys and values rows cu_k[b] .. (default: cu_q) of k, v
     [Tk, kv_heads, hd].  cu_q, cu_k: int32 [B + 1], rising from 0.  `causal`: query i of a
-    sequence sees its keys j <= i + keys - queries (the last query sees all).  scale:
-    hd ** -0.5 unless given.  out [T, q_heads, hd]; a row that sees no key is zero, rows of
+    sequence sees its keys j <= i + keys - queries (the last query sees all).  scale (a
+    positive number): hd ** -0.5 unless given.  out [T, q_heads, hd]; a row that sees no key is zero, rows of
     no sequence stay as they were.  Returns out."""
     T, hq, hd, dt, qt, qh = _queries(q)
     if k.dim() != 3 or k.shape != v.shape:
