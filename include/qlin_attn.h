@@ -23,7 +23,9 @@
  *     output that sees a key of it, and maybe of others of that sequence (no memory outside
  *     the cache is read);
  *   - a scale of an int8 cache that is not finite makes numbers of no output that sees its
- *     key; elsewhere infinities and NaN go through the formulas;
+ *     key; elsewhere infinities and NaN go through the formulas, but that an infinite fp16 value
+ *     whose key weighs less than 2^-17 of its block's heaviest may make no number of its column
+ *     (the weight is an fp16 number too, and may be zero);
  *   - row bounds (cu) are clamped to the rows there are, and query bounds that fall count as the
  *     highest before them.
  * Rows, heads and pages of what a call writes do not overlap, and it shares no byte with what the
