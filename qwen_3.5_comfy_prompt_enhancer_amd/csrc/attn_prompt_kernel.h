@@ -45,8 +45,8 @@
 // A row's masked keys have no part in it whatever they hold.  Scores are replaced before the maximum.  An
 // int8 value's scale that is not finite is taken out, and makes its key's score no number instead.  A 16-bit
 // value that is no number is none times a P of zero either: a unit whose sums come out non-finite after
-// masked blocks is computed again, finite values apart from the others (split), in about twice the time
-// (prompts of 512 / 2048 tokens whose first value is NaN 66 / 170 us, of numbers 22 / 48).
+// masked blocks is computed again, finite values apart from the others (split): prompts of 512 / 2048 tokens
+// whose first value is NaN take 66 / 170 us, of numbers 22 / 48.
 #pragma once
 
 #include "attn_dev.h"
