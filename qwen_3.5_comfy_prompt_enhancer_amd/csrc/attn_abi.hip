@@ -1,42 +1,19 @@
 // extern "C" entry points of the attention operators (declared in include/qlin_attn.h): checks
 // of arguments and launch plans.
 #include <math.h>
-#include <stdarg.h>
-#include <stdio.h>
 #include <stdlib.h>
 
 #include <algorithm>
 
 #include "../../include/qlin_attn.h"
+#include "../../include/qlin_candidates.h"
+#include "abi_check.h"
 #include "attn_internal.h"
 #include "qlin_dev.h"
-#include "qlin_internal.h"
 
 using namespace qlin;
 
 namespace {
-
-int fail(int code, const char* fmt, ...) {
-  char msg[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(msg, sizeof(msg), fmt, ap);
-  va_end(ap);
-  return set_error(code, msg);
-}
-
-int status(const char* fn, hipError_t e) {
-  if (e == hipSuccess) return QLIN_OK;
-  return fail(QLIN_ERR_HIP, "%s: HIP error %d (%s)", fn, (int)e, hipGetErrorString(e));
-}
-
-#define QA_TRY(expr)                \
-  do {                              \
-    const int rc_ = (expr);         \
-    if (rc_ != QLIN_OK) return rc_; \
-  } while (0)
-
-bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 constexpr int kMaxRows = (1 << 24) - 1;       // tokens of a call (rows of a key head stay below 2^31), and its
                                               // workgroups (a launch has less than 2^32 threads)
@@ -162,87 +139,6 @@ int check_paged(const char* fn, const qlin_paged_kv* cache, const int* table, in
   return QLIN_OK;
 }
 
-// A tensor's bytes: runs of `width` at every sum of indexes times strides (bytes; an axis of one has 0).
-struct Region {
-  const char* name;
-  const char* p;
-  long long width;
-  long long n[3], s[3];
-  long long end() const {
-    long long e = width;
-    for (int i = 0; i < 3; ++i) e += (n[i] - 1) * s[i];
-    return e;
-  }
-};
-
-Region region(const char* name, const void* p, int es, int run, long long n0, long long s0, long long n1, long long s1,
-              long long n2 = 1, long long s2 = 0) {
-  return Region{name, (const char*)p, (long long)es * run, {n0, n1, n2},
-                {n0 > 1 ? s0 * es : 0, n1 > 1 ? s1 * es : 0, n2 > 1 ? s2 * es : 0}};
-}
-
-// Sums c + sum k_i s_i with lo_i <= k_i <= hi_i: whether one lies between -before and after (both
-// excluded).  Axes come from the longest stride to the shortest; of each only the few multiples are tried
-// that the shorter ones can still bring there.  Layouts that take more than `budget` tries (strides of
-// about the same length, over long axes) are taken to overlap.
-struct Sums {
-  struct Axis { long long s, lo, hi; } ax[6];
-  int axes = 0;
-  long long before, after;
-  int budget = 4096;
-
-  void add(long long s, long long lo, long long hi) {
-    if (s == 0 || (lo == 0 && hi == 0)) return;
-    for (int i = 0; i < axes; ++i)
-      if (ax[i].s == s) {
-        ax[i].lo += lo, ax[i].hi += hi;
-        return;
-      }
-    int at = axes++;
-    for (; at > 0 && ax[at - 1].s < s; --at) ax[at] = ax[at - 1];
-    ax[at] = Axis{s, lo, hi};
-  }
-  static long long floor_div(long long a, long long b) { return a / b - (a % b < 0); }
-  bool meet(long long c, int i = 0, bool zero = false) {  // zero: all k 0 so far, which does not count
-    if (i == axes) return !zero && c > -before && c < after;
-    if (--budget < 0) return true;
-    long long least = 0, most = 0;
-    for (int j = i + 1; j < axes; ++j) least += ax[j].lo * ax[j].s, most += ax[j].hi * ax[j].s;
-    const long long k0 = std::max(ax[i].lo, -floor_div(c + most + before - 1, ax[i].s));
-    const long long k1 = std::min(ax[i].hi, floor_div(after - 1 - c - least, ax[i].s));
-    for (long long k = k0; k <= k1; ++k)
-      if (meet(c + k * ax[i].s, i + 1, zero && k == 0)) return true;
-    return false;
-  }
-};
-
-int check_regions(const char* fn, const Region& a, const Region& b) {
-  if (!a.p || !b.p || a.p + a.end() <= b.p || b.p + b.end() <= a.p) return QLIN_OK;
-  Sums d;
-  d.before = a.width, d.after = b.width;
-  for (int i = 0; i < 3; ++i) {
-    d.add(a.s[i], 0, a.n[i] - 1);
-    d.add(b.s[i], -(b.n[i] - 1), 0);
-  }
-  if (d.meet(a.p - b.p)) return fail(QLIN_ERR_INVALID, "%s: %s overlaps %s", fn, a.name, b.name);
-  return QLIN_OK;
-}
-
-// Whether runs of one region share bytes.
-int check_region(const char* fn, const Region& a) {
-  Sums d;
-  d.before = d.after = a.width;
-  for (int i = 0; i < 3; ++i)
-    if (a.n[i] > 1) {
-      if (a.s[i] < a.width) return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, a.name);
-      for (int j = 0; j < i; ++j)  // (two axes of one stride: index (0, 1) is (1, 0))
-        if (a.n[j] > 1 && a.s[j] == a.s[i]) return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, a.name);
-      d.add(a.s[i], 1 - a.n[i], a.n[i] - 1);
-    }
-  if (d.meet(0, 0, true)) return fail(QLIN_ERR_INVALID, "%s: rows of %s overlap", fn, a.name);
-  return QLIN_OK;
-}
-
 // A cache's keys, values and scales.
 struct CacheRegions {
   Region r[4];
@@ -263,16 +159,6 @@ CacheRegions cache_regions(const qlin_paged_kv* c, int hkv, int hd) {
 int check_cache_apart(const char* fn, const Region& a, const qlin_paged_kv* c, int hkv, int hd) {
   const CacheRegions x = cache_regions(c, hkv, hd);
   for (int i = 0; i < x.n; ++i) QA_TRY(check_regions(fn, a, x.r[i]));
-  return QLIN_OK;
-}
-
-// The partial sums' place in the workspace, behind its counters and exchange slots.
-int workspace_parts(const char* fn, void* ws, size_t bytes, char** part, size_t* avail) {
-  const size_t base = counter_bytes() + poll_bytes();
-  if (!ws || bytes < base) return fail(QLIN_ERR_WORKSPACE, "%s: workspace missing or too small", fn);
-  if (!aligned(ws, 256)) return fail(QLIN_ERR_INVALID, "%s: workspace must be 256-byte aligned", fn);
-  *part = (char*)ws + base;
-  *avail = bytes - base;
   return QLIN_OK;
 }
 
@@ -335,6 +221,41 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
   a.units = (int)units;
   a.part = (float*)part;
   a.cnt = (unsigned*)ws;
+  return QLIN_OK;
+}
+
+// Row tiles and units of a decode step over shared prefixes.
+int plan_shared(const char* fn, SharedArgs& a, int hd, int page, char* part, size_t avail) {
+  const long long rows = (long long)((a.B + a.G - 1) / a.G) * a.R;  // of a prefix, on average
+  a.tiles = a.R > 16 || rows > 32 ? 4 : rows > 16 ? 2 : 1;
+  a.spt = 16 * a.tiles / a.R;
+  long long few = 256, total = 512;
+  if (const char* e = getenv("QLIN_SHARED_UNITS")) {  // for tuning runs
+    if (atoi(e) > 0) few = total = atoi(e);
+  }
+  const long long tiles = a.B / a.spt + a.G;  // units of a prefix that is not cut
+  const long long keys = std::max(1, a.pre.max_pages) * (long long)page, own = std::max(1, a.own.max_pages) * (long long)page;
+  const long long bound = tiles * ((keys + 4 * kSharedBlock - 1) / (4 * kSharedBlock)) +
+                          a.B * ((own + 4 * kSharedBlock - 1) / (4 * kSharedBlock));
+  long long target = std::min(std::max(1LL, total / a.HKV), bound);
+  // every unit leaves its rows' sums: at most target + tiles of prefixes, target + B own ones (and two more
+  // for what the device's estimate rounds); fewer where that is more than the workspace holds
+  const long long row = (long long)hd * 4 + 8, unit = (long long)(a.spt + 1) * a.R;
+  const long long fixed = ((tiles + 2) * a.spt + a.B + 2) * a.R;
+  target = std::min(target, ((long long)avail / row / a.HKV - fixed) / unit);
+  if (target < 1)
+    return fail(QLIN_ERR_UNSUPPORTED, "%s: %d sequences of %d query heads are more than the workspace holds sums of", fn,
+                a.B, a.HKV * a.R);
+  a.target = (int)target;
+  a.few = (int)std::min(std::max(1LL, few / a.HKV), target);
+  a.own_rows = (target + tiles + 2) * a.spt * a.R;
+  a.rows = a.own_rows + (target + a.B + 2) * a.R;
+  const long long units = target + tiles + a.B + 2;
+  QA_TRY(check_grid(fn, units * a.HKV));
+  QA_TRY(check_grid(fn, (long long)a.B * a.HKV * a.R));
+  a.units = (int)units;
+  a.part = (float*)part;
+  a.ml = (float*)(part + (long long)a.HKV * a.rows * hd * 4);
   return QLIN_OK;
 }
 
@@ -549,6 +470,45 @@ int qlin_attn_decode(const void* q, int64_t q_seq, int64_t q_head, const qlin_pa
   a.part = (float*)part;
   a.cnt = (unsigned*)workspace;
   return status(fn, launch_decode(a, dtype, hd, (hipStream_t)stream));
+}
+
+int qlin_attn_decode_shared(const void* q, int64_t q_seq, int64_t q_head, const qlin_paged_kv* cache,
+                            const int* prefix_table, int64_t prefix_table_stride, int max_prefix_pages,
+                            const int* prefix_len, const int* cu_seq, int G, const int* table, int64_t table_stride,
+                            int max_pages, const int* kv_len, void* out, int64_t o_seq, int64_t o_head, int B,
+                            int q_heads, int kv_heads, int hd, int dtype, float scale, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const char* fn = "qlin_attn_decode_shared";
+  set_error(QLIN_OK, "");
+  if (B < 0 || G < 0) return fail(QLIN_ERR_INVALID, "%s: negative size", fn);
+  QA_TRY(check_heads(fn, q_heads, kv_heads, hd, dtype));
+  QA_TRY(check_scale(fn, scale));
+  if (B == 0 || G == 0) return QLIN_OK;
+  QA_TRY(check_seqs(fn, B));
+  if (G > kMaxSeqs) return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d groups", fn, kMaxSeqs);
+  if (!cu_seq) return fail(QLIN_ERR_INVALID, "%s: null sequence bounds", fn);
+  if (!aligned(cu_seq, 4)) return fail(QLIN_ERR_UNSUPPORTED, "%s: sequence bounds must be 4-byte aligned", fn);
+  QA_TRY(check_tensor(fn, "q", q, 2, hd, B, q_seq, q_heads, q_head, false));
+  QA_TRY(check_tensor(fn, "out", out, 2, hd, B, o_seq, q_heads, o_head, true));
+  QA_TRY(check_apart(fn, q, out));
+  SharedArgs a = {};
+  QA_TRY(check_paged(fn, cache, prefix_table, prefix_table_stride, max_prefix_pages, prefix_len, kv_heads, hd, dtype,
+                     a.pre));
+  QA_TRY(check_paged(fn, cache, table, table_stride, max_pages, kv_len, kv_heads, hd, dtype, a.own));
+  const Region to = region("out", out, 2, hd, B, o_seq, q_heads, o_head);
+  QA_TRY(check_region(fn, to));
+  QA_TRY(check_regions(fn, to, region("q", q, 2, hd, B, q_seq, q_heads, q_head)));
+  QA_TRY(check_cache_apart(fn, to, cache, kv_heads, hd));
+  char* part;
+  size_t avail;
+  QA_TRY(workspace_parts(fn, workspace, workspace_bytes, &part, &avail));
+  a.q = q, a.qb = q_seq, a.qh = q_head;
+  a.o = out, a.ob = o_seq, a.oh = o_head;
+  a.cu = cu_seq, a.G = G, a.B = B, a.HKV = kv_heads, a.R = q_heads / kv_heads;
+  a.c = scale * 1.44269504088896340736f;
+  QA_TRY(plan_shared(fn, a, hd, cache->page, part, avail));
+  return status(fn, dtype == QLIN_BF16 ? launch_shared_bf16(a, hd, (hipStream_t)stream)
+                                       : launch_shared_f16(a, hd, (hipStream_t)stream));
 }
 
 }  // extern "C"

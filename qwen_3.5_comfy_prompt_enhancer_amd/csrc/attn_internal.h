@@ -89,6 +89,30 @@ constexpr int kDecodeGroup = 16;     // units joined at a time
 constexpr int kDecodeCounters = 32;  // counters of a (sequence, key head, group)
 hipError_t launch_decode(const DecodeArgs& a, int dt, int hd, hipStream_t st);
 
+// Attention of one token per sequence, of groups that share a prefix (attn_shared*.hip).
+struct SharedArgs {
+  const void* q;
+  long long qb, qh;
+  void* o;
+  long long ob, oh;
+  KvSrc pre, own;         // one cache; pre: a group's table row and length, own: a sequence's
+  const int* cu;          // [G + 1] sequences of each group
+  int G, B, HKV, R;       // R: query heads of a key head
+  int tiles;              // 16-row tiles of a prefix's unit: 1, 2 or 4
+  int spt;                // sequences of a prefix's unit
+  float c;                // scale * log2(e)
+  int target, few;        // units of a key head that long and short work is cut into
+  int units;              // units per key head: the grid's bound
+  long long own_rows;     // rows of parts of a key head in front of the own ones
+  long long rows;         // rows of parts of a key head
+  float* part;            // [key head][row][hd] sums
+  float* ml;              // [key head][row][2] reference and sum of P
+};
+constexpr int kSharedBlock = 32;     // keys a wave takes at a time
+constexpr int kSharedLong = 32;      // blocks of a unit up to which fewer units are better
+hipError_t launch_shared_bf16(const SharedArgs& a, int hd, hipStream_t st);
+hipError_t launch_shared_f16(const SharedArgs& a, int hd, hipStream_t st);
+
 // Attention of packed prompts over packed keys or a paged cache (attn_prompt*.hip).
 struct PromptArgs {
   const void* q;

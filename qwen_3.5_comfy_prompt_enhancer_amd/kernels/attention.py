@@ -8,7 +8,9 @@ and write a paged cache, which several sequences share and a page table orders:
                        three axes, keys and values into the cache;
 * `attn_prompt`        attention of packed prompts over their own keys;
 * `attn_prompt_paged`  attention of the next chunk of prompts over the cache;
-* `attn_decode`        attention of one new token of each sequence over the cache.
+* `attn_decode`        attention of one new token of each sequence over the cache;
+* `attn_decode_shared` the same for groups of sequences that share a prefix, whose keys are
+                       read once for the group.
 
 A step of an attention layer, from proj3's rows to the output projection's producer:
 
@@ -38,7 +40,7 @@ import torch
 
 from . import qlin as C
 
-__all__ = ["qk_norm_rope", "attn_prompt", "attn_prompt_paged", "attn_decode"]
+__all__ = ["qk_norm_rope", "attn_prompt", "attn_prompt_paged", "attn_decode", "attn_decode_shared"]
 
 QLIN_I8 = 4
 
@@ -59,7 +61,10 @@ _SIGS = {
                                _P, _S, _P],
     "qlin_attn_decode": [_P, _L, _L, _B, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I, _I, _I, _F, _P, _S, _P],
 }
-EXPORTS = tuple(_SIGS)
+EXPORTS = tuple(_SIGS)  # of include/qlin_attn.h
+# include/qlin_candidates.h
+_SIGS["qlin_attn_decode_shared"] = [_P, _L, _L, _B, _P, _L, _I, _P, _P, _I, _P, _L, _I, _P, _P, _L, _L, _I, _I, _I,
+                                    _I, _I, _F, _P, _S, _P]
 
 _DT = {torch.bfloat16: C.QLIN_BF16, torch.float16: C.QLIN_F16}
 _WDT = {**_DT, torch.float32: C.QLIN_F32}
@@ -144,15 +149,15 @@ def _weight(name, w, hd):
     return dt
 
 
-def _table(table, kv_len, B):
+def _table(table, kv_len, B, name="table", lengths="kv_len"):
     """Stride and width of a page table [B, pages]; checks the lengths too."""
     shape = table.shape
     if len(shape) != 2 or shape[0] != B:
-        raise ValueError(f"table must be [{B}, pages]")
+        raise ValueError(f"{name} must be [{B}, pages]")
     st = table.stride()
     if table.dtype != torch.int32 or (shape[1] > 1 and st[1] != 1):
-        raise ValueError("table must be int32 with a contiguous last axis")
-    _vector("kv_len", kv_len, B)
+        raise ValueError(f"{name} must be int32 with a contiguous last axis")
+    _vector(lengths, kv_len, B)
     if shape[1] > _INT_MAX:
         _size("pages of a table's row", shape[1])
     return st[0], shape[1]
@@ -337,4 +342,32 @@ def attn_decode(q, k_cache, v_cache, table, kv_len, out, k_s=None, v_s=None, sca
     _call("qlin_attn_decode", out.get_device(), q.data_ptr(), qb, qh, cache, table.data_ptr(), tb, pages,
           kv_len.data_ptr(), out.data_ptr(), ob, oh, B, hq, hkv, hd, dt, hd ** -0.5 if scale is None else scale, ws,
           nws, stream)
+    return out
+
+
+def attn_decode_shared(q, k_cache, v_cache, prefix_table, prefix_len, cu_seq, table, kv_len, out, k_s=None, v_s=None,
+                       scale=None):
+    """`attn_decode` for sequences in groups that share a prefix (the candidates of one prompt,
+    prompts behind one instruction): q and out [B, q_heads, hd].  Group g's sequences are rows
+    cu_seq[g] .. cu_seq[g + 1] - 1; each sees the first prefix_len[g] tokens of pages
+    prefix_table[g, 0], prefix_table[g, 1], ..., whose keys are read once for the group, and
+    then its own first kv_len[b] tokens (the new one among them) of pages table[b, 0], ...
+    A prefix may end anywhere in its last page.  prefix_table: int32 [groups, pages],
+    prefix_len: int32 [groups], cu_seq: int32 [groups + 1], rising from 0; table and kv_len as
+    attn_decode's.  A sequence without keys gives zeros; rows behind the last group stay as
+    they were.  scale: hd ** -0.5 unless given.  Returns out."""
+    B, hq, hd, dt, qb, qh = _queries(q)
+    cache, hkv = _cache(k_cache, v_cache, k_s, v_s, q.dtype, hd)
+    ob, oh = _strides("out", out, B, hq, hd, q.dtype)
+    if cu_seq.dim() != 1 or cu_seq.shape[0] < 1:
+        raise ValueError("cu_seq must be [groups + 1]")
+    G = _size("groups", cu_seq.shape[0] - 1)
+    _vector("cu_seq", cu_seq, G + 1)
+    pb, ppages = _table(prefix_table, prefix_len, G, "prefix_table", "prefix_len")
+    tb, pages = _table(table, kv_len, B)
+    C.require_cuda(q, k_cache, v_cache, prefix_table, prefix_len, cu_seq, table, kv_len, out, k_s, v_s)
+    ws, nws, stream = C.scratch(out)
+    _call("qlin_attn_decode_shared", out.get_device(), q.data_ptr(), qb, qh, cache, prefix_table.data_ptr(), pb, ppages,
+          prefix_len.data_ptr(), cu_seq.data_ptr(), G, table.data_ptr(), tb, pages, kv_len.data_ptr(), out.data_ptr(),
+          ob, oh, B, hq, hkv, hd, dt, hd ** -0.5 if scale is None else scale, ws, nws, stream)
     return out
