@@ -1,6 +1,7 @@
 // extern "C" entry points of what lies between the vocabulary head and the next token (declared in
 // include/qlin_candidates.h): checks of arguments and launch plans.
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -161,12 +162,15 @@ int qlin_sample(const void* logits, int dtype, int64_t logits_row, int B, int V,
   a.tokens = tokens, a.tokens64 = tokens_64, a.logp = logprobs;
   // a workgroup for each tile of a row, fewer where their lists would be more than one can join or than
   // the workspace holds
-  const long long tiles = ((long long)V + kSampleTile - 1) / kSampleTile, list = 8LL * (a.k + 1);
-  const long long chunks = std::min({tiles, (long long)kSampleKeys / a.k, (long long)avail / list / B, kMaxGrid / B});
+  const long long tiles = ((long long)V + kSampleTile - 1) / kSampleTile, keys = sample_list(a.k), list = 8 * (keys + 1);
+  long long chunks = std::min({tiles, std::max(8LL, 1024LL / B), (long long)kSampleKeys / keys, (long long)avail / list / B, kMaxGrid / B});
+  if (const char* e = getenv("QLIN_SAMPLE_CHUNKS")) {  // for tuning runs
+    if (atoi(e) > 0) chunks = std::min(chunks, (long long)atoi(e));
+  }
   if (chunks < 1) return fail(QLIN_ERR_WORKSPACE, "%s: workspace too small for %d rows", fn, B);
   a.chunks = (int)chunks;
   a.keys = (uint64_t*)part;
-  a.stats = (uint64_t*)part + (long long)B * chunks * a.k;
+  a.stats = (uint64_t*)part + (long long)B * chunks * keys;
   a.cnt = (unsigned*)workspace;
   return status(fn, launch_sample(a, (hipStream_t)stream));
 }

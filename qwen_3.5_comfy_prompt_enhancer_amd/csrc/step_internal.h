@@ -53,13 +53,15 @@ struct SampleArgs {
   int tokens64;
   float* logp;            // or nullptr
   int chunks;             // workgroups of a row
-  uint64_t* keys;         // [B][chunks][k] largest of each chunk
+  uint64_t* keys;         // [B][sample_list(k)][chunks] the largest of each chunk among them
   uint64_t* stats;        // [B][chunks] maximum and sum
   unsigned* cnt;          // arrivals of each row, zero between calls
 };
 constexpr int kSampleTile = 8192;   // logits that a workgroup looks at in one go
 constexpr int kSampleMost = 128;    // largest k
-constexpr int kSampleKeys = 4096;   // chunks x k at most
+constexpr int kSampleKeys = 6144;   // keys of a row's chunks at most
+// keys that a chunk leaves room for
+__host__ __device__ constexpr int sample_list(int k) { return k + k / 2 + 4; }
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st);
 
 }  // namespace qlin

@@ -204,3 +204,31 @@ def test_graph_and_streams():
                 outs.append(sampling.sample(xc, uc, t))
     torch.cuda.synchronize()
     assert all(torch.equal(o.cpu(), eager[0]) for o in outs)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("k", [1, 20, 128])
+def test_many_of_equal_value(dt, k):
+    """Masks of the type's lowest value, rows of a few distinct values, and ties at the k-th place."""
+    V = 8192 * 4 + 77
+    g = torch.Generator().manual_seed(k)
+    low = torch.finfo(dt).min
+    x = torch.full((5, V), low, dtype=dt)
+    x[0, torch.randperm(V, generator=g)[:k // 2 + 1]] = 1.0           # the others come from the masked ones
+    x[1] = torch.randint(0, 3, (V,), generator=g).to(dt)
+    x[2] = torch.randint(0, 300, (V,), generator=g).to(dt)
+    x[3, 9000:] = -2.5
+    x[4] = (torch.arange(V) % 8 == 5).to(dt)                          # one place of each thread's eight
+    for u in (0.1, 0.9):
+        check(x, torch.full((5,), u), top_k=k, temperature=1e9 if dt == F32 else 2.0)
+
+
+def test_most_in_few_threads():
+    """A tile whose largest lie in 100 threads' places, all different: more than reach the list as a rule."""
+    V = 8192 + 100
+    i = torch.arange(V)
+    x = torch.where(i % 2048 < 800, 50 + (i * 2654435761 % 4096).float() / 128, -i.float() / 4096)[None].expand(3, V).contiguous()
+    x[1, 8192:] = 200.0
+    for k in (50, 128):
+        for u in (0.001, 0.77, 0.9999):
+            check(x, torch.full((3,), u), top_k=k, temperature=20.0)
