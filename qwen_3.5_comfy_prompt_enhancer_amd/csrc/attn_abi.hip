@@ -227,7 +227,7 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
 // Row tiles and units of a decode step over shared prefixes.
 int plan_shared(const char* fn, SharedArgs& a, int hd, int page, char* part, size_t avail) {
   const long long rows = (long long)((a.B + a.G - 1) / a.G) * a.R;  // of a prefix, on average
-  a.tiles = a.R > 16 || rows > 32 ? 4 : rows > 16 ? 2 : 1;
+  a.tiles = a.R > 16 || rows > 32 ? 8 : rows > 16 ? 2 : 1;
   a.spt = 16 * a.tiles / a.R;
   long long few = 256, total = 512;
   if (const char* e = getenv("QLIN_SHARED_UNITS")) {  // for tuning runs

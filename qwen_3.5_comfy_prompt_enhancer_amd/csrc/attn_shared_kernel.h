@@ -29,7 +29,7 @@
 // the prefix's first, so that results do not depend on the order in which units end.
 #pragma once
 
-#include "attn_dev.h"
+#include "attn_prompt_kernel.h"
 
 namespace qlin {
 
@@ -40,34 +40,51 @@ constexpr int kWaves = 4;
 
 __device__ __forceinline__ int blocks_of(int len) { return (len + kSharedBlock - 1) / kSharedBlock; }
 
-// Groups g0 + lane (none behind the last): first sequence, sequences, keys of the prefix.  Bounds are
-// clamped to the sequences there are and taken as rising; `start`: the highest bound so far, for
-// calls with rising g0.
+// Bounds and prefix length of group g0 + lane (none behind the last), and keys of sequence b0 + lane, as they are.
+struct Lens {
+  int c0, c1, len;
+};
+__device__ __forceinline__ Lens load_group(const SharedArgs& a, int g0) {
+  const int g = g0 + ((int)threadIdx.x & 63);
+  Lens r = {0, 0, 0};
+  if (g < a.G) {
+    r.c0 = a.cu[g];
+    r.c1 = a.cu[g + 1];
+    r.len = kv_length(a.pre, g);
+  }
+  return r;
+}
+__device__ __forceinline__ int load_own(const SharedArgs& a, int b0) {
+  const int b = b0 + ((int)threadIdx.x & 63);
+  return b < a.B ? kv_length(a.own, b) : 0;
+}
+
+// Groups g0 + lane: first sequence, sequences, keys of the prefix.  Bounds are clamped to the sequences there
+// are and taken as rising; `start`: the highest bound so far, for calls with rising g0.
 struct Group {
   int b0, n, len;
 };
-__device__ __forceinline__ Group group_of(const SharedArgs& a, int g0, int& start) {
-  const int g = g0 + ((int)threadIdx.x & 63);
-  Group r = {0, 0, 0};
-  int c0 = 0, c1 = 0;
-  if (g < a.G) {
-    c0 = min(max(a.cu[g], 0), a.B);
-    c1 = min(max(a.cu[g + 1], 0), a.B);
-    r.len = kv_length(a.pre, g);
-  }
+__device__ __forceinline__ Group group_of(const SharedArgs& a, const Lens& l, int& start) {
+  const int c0 = min(max(l.c0, 0), a.B), c1 = min(max(l.c1, 0), a.B);
+  Group r;
   r.b0 = max(wave_scan_max(c0), start);
   r.n = max(0, c1 - r.b0);
+  r.len = l.len;
   start = lane_value(max(wave_scan_max(max(c0, c1)), start), 63);
   return r;
 }
 
 // What all workgroups make of the lengths: blocks of a unit, and the sequences of some group
-// (lo .. hi - 1).
+// (lo .. hi - 1).  The first 64 groups' and sequences' lengths are read once, together.
 struct Plan {
   int chunk, lo, hi;
+  Lens groups;
+  int own;
 };
-__device__ __forceinline__ int own_length(const SharedArgs& a, const Plan& p, int b) {
-  return b >= p.lo && b < p.hi ? kv_length(a.own, b) : 0;
+__device__ __forceinline__ Lens groups_at(const SharedArgs& a, const Plan& p, int g0) { return g0 ? load_group(a, g0) : p.groups; }
+__device__ __forceinline__ int own_at(const SharedArgs& a, const Plan& p, int b0) {
+  const int n = b0 ? load_own(a, b0) : p.own, b = b0 + ((int)threadIdx.x & 63);
+  return b >= p.lo && b < p.hi ? n : 0;
 }
 __device__ __forceinline__ int tiles_of(const SharedArgs& a, const Group& g) {
   return g.len > 0 ? (g.n + a.spt - 1) / a.spt : 0;
@@ -76,17 +93,18 @@ __device__ __forceinline__ int parts_of(const Plan& p, int len) { return (blocks
 
 __device__ __forceinline__ Plan make_plan(const SharedArgs& a) {
 #pragma clang fp contract(off)  // (both launches have to make the same of them)
-  const int lane = (int)threadIdx.x & 63;
   Plan p;
-  p.lo = min(max(a.cu[0], 0), a.B);
+  p.groups = load_group(a, 0);
+  p.own = load_own(a, 0);
+  p.lo = min(max(lane_value(p.groups.c0, 0), 0), a.B);
   int start = 0;
   float total = 0.0f;  // (an estimate where it is large; the same for all workgroups)
   for (int g0 = 0; g0 < a.G; g0 += 64) {
-    const Group g = group_of(a, g0, start);
+    const Group g = group_of(a, groups_at(a, p, g0), start);
     total += (float)tiles_of(a, g) * (float)blocks_of(g.len);
   }
   p.hi = max(start, p.lo);
-  for (int b0 = p.lo; b0 < p.hi; b0 += 64) total += (float)blocks_of(own_length(a, p, b0 + lane));
+  for (int b0 = 0; b0 < p.hi; b0 += 64) total += (float)blocks_of(own_at(a, p, b0));
   total = lane_value(wave_scan(total), 63);
   const float few = ceilf(total / (float)a.few), most = ceilf(total / (float)a.target);
   p.chunk = max((int)fminf(few <= (float)kSharedLong ? few : fmaxf((float)kSharedLong, most), 1e8f), 1);
@@ -113,10 +131,9 @@ __device__ __forceinline__ void part_tile(int i, int parts, int tiles, int& part
 }
 
 __device__ __forceinline__ bool find_unit(const SharedArgs& a, const Plan& p, int u, Unit& r) {
-  const int lane = (int)threadIdx.x & 63;
   int base = 0, start = 0;
   for (int g0 = 0; g0 < a.G; g0 += 64) {
-    const Group g = group_of(a, g0, start);
+    const Group g = group_of(a, groups_at(a, p, g0), start);
     const int tiles = tiles_of(a, g), parts = parts_of(p, g.len);
     const int end = wave_scan(tiles * parts), sum = lane_value(end, 63);
     if (u < base + sum) {
@@ -137,8 +154,8 @@ __device__ __forceinline__ bool find_unit(const SharedArgs& a, const Plan& p, in
     base += sum;
   }
   int own = 0;
-  for (int b0 = p.lo; b0 < p.hi; b0 += 64) {
-    const int len = own_length(a, p, b0 + lane);
+  for (int b0 = 0; b0 < p.hi; b0 += 64) {
+    const int len = own_at(a, p, b0);
     const int parts = parts_of(p, len);
     const int end = wave_scan(parts), sum = lane_value(end, 63);
     if (u < base + own + sum) {
@@ -183,10 +200,15 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
   return T::pack_exact((float)(int8_t)(w0 >> (8 * c)), (float)(int8_t)(w1 >> (8 * c)));
 }
 
+// The first row of a unit's part.
+__device__ __forceinline__ long long part_row(const SharedArgs& a, const Unit& U, int hk) {
+  return (long long)hk * a.rows + (U.prefix ? (long long)U.slot * (a.spt * a.R) : a.own_rows + (long long)U.slot * a.R);
+}
+
 // Dynamic LDS: the queries of NT tiles as operands; behind the loop the waves' sums of a tile.
 template <int HD>
 constexpr int shared_lds(int nt) {
-  const int q = nt * (HD / 32) * 1024 + kWaves * 256, join = kWaves * 16 * HD * 4 + kWaves * 128;
+  const int q = nt * (HD / 32) * 1024 + kWaves * 256, join = kWaves * 16 * (HD + 4) * 4 + kWaves * 128;
   return q > join ? q : join;
 }
 
@@ -205,15 +227,17 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
   const int rows = U.n * a.R;
 
   // queries to LDS, as operands: step s of tile t at ((t STEPS + s) 64 + lane) 16 bytes, column j = row
-  // 16 t + j, the same hd order as a key's loads
-  for (int x = tid; x < NT * STEPS * 64; x += kThreads) {
-    const int l = x & 63, s = (x >> 6) % STEPS, row = (x >> 6) / STEPS * 16 + (l & 15);
+  // 16 t + j, the same hd order as a key's loads.  (Loaded in front of the first block, written behind its loads.)
+  constexpr int QL = (NT * STEPS + kWaves - 1) / kWaves;
+  u32x4 qr[QL];
+#pragma unroll
+  for (int i = 0; i < QL; ++i) {
+    const int x = i * kThreads + tid, l = x & 63, s = (x >> 6) % STEPS, row = (x >> 6) / STEPS * 16 + (l & 15);
     const int d = Q8 ? 64 * (s / 2) + 16 * (l >> 4) + 8 * (s % 2) : 32 * s + 8 * (l >> 4);
     const int seq = row / a.R;
-    u32x4 v = {0, 0, 0, 0};
+    qr[i] = u32x4{0, 0, 0, 0};
     if (row < rows)
-      v = ld_global<u32x4>((const uint16_t*)a.q + (U.b0 + seq) * a.qb + (hk * a.R + (row - seq * a.R)) * a.qh + d);
-    *(u32x4*)(lds + x * 4) = v;
+      qr[i] = ld_global<u32x4>((const uint16_t*)a.q + (U.b0 + seq) * a.qb + (hk * a.R + (row - seq * a.R)) * a.qh + d);
   }
   const f32x4* lq = (const f32x4*)lds + lane;
 
@@ -297,7 +321,11 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
     load_v(blk, pid);
     pages(blk + kWaves, pin);
   }
-  __syncthreads();  // (the queries)
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < QL; ++i)
+    if (i * kThreads + tid < NT * STEPS * 64) *(u32x4*)(lds + (i * kThreads + tid) * 4) = qr[i];
+  __syncthreads();
   float* lsc = lds + NT * STEPS * 256 + wave * 64;
   for (; blk < blk1; blk += kWaves) {
     const bool more = blk + kWaves < blk1;
@@ -449,9 +477,10 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
   }
 
   // waves join in LDS, tile by tile: wave w's sums at w 16 HD, references and sums of P behind all
-  float* mlw = lds + kWaves * 16 * HD;
-  const long long row0 = (long long)hk * a.rows + (U.prefix ? (long long)U.slot * (a.spt * a.R)
-                                                            : a.own_rows + (long long)U.slot * a.R);
+  // (rows HD + 4 apart: the 16 of a tile start in different banks; HD apart the stores took 3 us more)
+  constexpr int ST = HD + 4;
+  float* mlw = lds + kWaves * 16 * ST;
+  const long long row0 = part_row(a, U, hk);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int n = min(16, rows - 16 * t);
@@ -462,7 +491,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
     for (int c = 0; c < VC; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float* dst = lds + (wave * 16 + j) * HD + c * 16 * VW + VW * (4 * g + i);
+        float* dst = lds + (wave * 16 + j) * ST + c * 16 * VW + VW * (4 * g + i);
 #pragma unroll
         for (int x = 0; x < VW; x += 4)
           *(f32x4*)(dst + x) = f32x4{O[t][c * VW + x][i], O[t][c * VW + x + 1][i], O[t][c * VW + x + 2][i], O[t][c * VW + x + 3][i]};
@@ -483,7 +512,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float e = exp2_(mlw[(w * 16 + r) * 2] - Ms);
-        const f32x4 x = *(const f32x4*)(lds + w * 16 * HD + f * 4);
+        const f32x4 x = *(const f32x4*)(lds + (w * 16 + r) * ST + (f % (HD / 4)) * 4);
         o += x * e;
         sum += mlw[(w * 16 + r) * 2 + 1] * e;
       }
@@ -497,40 +526,389 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
   }
 }
 
-// Workgroups that a CU holds by registers.
-constexpr int shared_occupancy(int hd, int nt) {
-  return hd == 256 ? (nt == 1 ? 2 : 1) : hd == 128 ? (nt == 1 ? 3 : nt == 2 ? 2 : 1) : (nt <= 2 ? 3 : 2);
+// One unit of many rows: a tile of 128, 32 to a wave, over keys that land in LDS for all four waves (as
+// prompt_kernel's: a ring of two blocks by 16-byte LDS DMA, 32x32x16 MFMAs with Q and O in registers, a lane
+// half a row).
+template <typename T, int HD, bool Q8>
+__device__ __forceinline__ void wide_unit(const SharedArgs& a, const Unit& U, int hk, uint32_t lds0) {
+  using G = PGeo<HD>;
+  using TV = std::conditional_t<Q8, Bf16, T>;  // type of P and V in their product
+  constexpr int PN = Q8 ? 2 : 1;               // P x scale as two bf16 numbers
+  constexpr int ES = Q8 ? 1 : 2;
+  const int tid = (int)threadIdx.x;
+  const int wave = (int)rfl32((uint32_t)tid >> 6), lane = tid & 63;
+  const int col = lane & 31, h = lane >> 5;
+  const KvSrc& kv = U.prefix ? a.pre : a.own;
+  const int rows = U.n * a.R, R0 = wave * 32, row = R0 + col;
+  const int kb0 = U.blk0, kb1 = U.blk1, nk = U.len;
+  u32x4 Q[G::NS];
+  {
+    const int seq = row / a.R;
+    const uint16_t* q = (const uint16_t*)a.q + (U.b0 + min(seq, U.n - 1)) * a.qb + (hk * a.R + (row - seq * a.R)) * a.qh + 8 * h;
+#pragma unroll
+    for (int s = 0; s < G::NS; ++s) Q[s] = ld_global<u32x4>(q + 16 * s);
+  }
+  f32x16 O[G::ND];
+  float m = kNegInf, l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
+
+  const int* table = kv.table + U.src * kv.table_stride;
+  // whether a page of the unit's keys lies outside the cache: looked at by every wave (each fetches a quarter
+  // of the keys that all of them use)
+  bool any_bad = false;
+  {
+    const int e1 = (min(kb1 * G::KB, nk) - 1) >> kv.page_shift;
+    for (int e = (kb0 * G::KB) >> kv.page_shift; e <= e1; e += 64)
+      any_bad |= (unsigned)table[min(e + lane, e1)] >= (unsigned)kv.num_pages;
+    any_bad = __any(any_bad);
+  }
+  // this wave's 8 keys of a block: the first one's place (keys behind the last are the last)
+  auto key8_of = [&](int kb) { return min(min(kb, kb1 - 1) * G::KB + 8 * wave, (nk - 1) & ~7); };
+  // (a scalar load: a vector one's wait would also wait for the copies in flight)
+  auto page_of = [&](int kb) {
+    return ((const __attribute__((address_space(4))) int*)table)[key8_of(kb) >> kv.page_shift];
+  };
+  struct Place {
+    const uint8_t* p;
+    uint32_t sp, st;
+  };
+  const Place kpl = {(const uint8_t*)kv.k.p + hk * kv.k.sh * ES, (uint32_t)kv.k.sp * ES, (uint32_t)kv.k.st * ES};
+  const Place vpl = {(const uint8_t*)kv.v.p + hk * kv.v.sh * ES, (uint32_t)kv.v.sp * ES, (uint32_t)kv.v.st * ES};
+  const Place kspl = {(const uint8_t*)(kv.k.s + hk * kv.k.ssh), (uint32_t)kv.k.ssp * 4u, (uint32_t)kv.k.sst * 4u};
+  const Place vspl = {(const uint8_t*)(kv.v.s + hk * kv.v.ssh), (uint32_t)kv.v.ssp * 4u, (uint32_t)kv.v.sst * 4u};
+  const uint32_t pmask = (1u << kv.page_shift) - 1u;
+  auto base_of = [&](const Place& x, int key, int pid) {
+    return x.p + ((uint64_t)(uint32_t)pid * x.sp + (uint64_t)((uint32_t)key & pmask) * x.st);
+  };
+  // copies of this wave's 8 keys of block kb; 16-bit: to their swizzled places in a stage
+  auto issue = [&](uint32_t stage, int kb, int pid) __attribute__((always_inline)) {
+    // (from a value that the compiler takes for a new one each time: kept through the loop, the copies'
+    // offsets would push operands out of the registers)
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int r_in = lane / G::LPR, p16 = lane % G::LPR;
+    const int key8 = key8_of(kb);
+    pid = (unsigned)pid >= (unsigned)kv.num_pages ? 0 : pid;
+    const int rmax = nk - 1 - key8;
+    const uint8_t* kp = rfl_p(base_of(kpl, key8, pid));
+    const uint8_t* vp = rfl_p(base_of(vpl, key8, pid));
+    if constexpr (!Q8) {
+      const uint32_t at = stage + (uint32_t)(8 * wave * G::ROWB);
+#pragma unroll
+      for (int i = 0; i < G::NI; ++i) {
+        const int r = G::RPI * i + r_in, krow = 8 * wave + r;
+        const int ck = p16 ^ G::swk(krow);
+        const int cv = (((p16 >> 2) ^ G::swv(krow)) << 2) | (p16 & 3);
+        const uint32_t rc = (uint32_t)min(r, rmax);
+        dma16(kp, rc * kpl.st + (uint32_t)ck * 16u, at + (uint32_t)(G::RPI * i * G::ROWB));
+        dma16(vp, rc * vpl.st + (uint32_t)cv * 16u, at + (uint32_t)(G::HALF + G::RPI * i * G::ROWB));
+      }
+    } else {
+      // codes of row r at 8 wave HD + r HD (keys, then values), scales of keys and values behind
+      constexpr int L8 = HD / 16, R8 = 64 / L8;  // lanes of a row, rows of a copy
+      const uint32_t at = stage + (uint32_t)(8 * wave * HD);
+      if (R8 <= 8 || lane < 8 * L8) {
+#pragma unroll
+        for (int i = 0; i < (R8 < 8 ? 8 / R8 : 1); ++i) {
+          const uint32_t rc = (uint32_t)min(R8 * i + lane / L8, rmax);
+          const uint32_t c = (uint32_t)(lane % L8) * 16u;
+          dma16(kp, rc * kpl.st + c, at + (uint32_t)(R8 * i * HD));
+          dma16(vp, rc * vpl.st + c, at + (uint32_t)(G::KB * HD + R8 * i * HD));
+        }
+      }
+      if (lane < 8) {
+        const uint32_t r = (uint32_t)min(lane, rmax);
+        const uint32_t sc = stage + (uint32_t)(G::STAGE / 2 + 64 * wave);
+        dma4(rfl_p(base_of(kspl, key8, pid)), r * kspl.st, sc);
+        dma4(rfl_p(base_of(vspl, key8, pid)), r * vspl.st, sc + 32u);
+      }
+    }
+  };
+  // int8: this wave's codes of a block as 16-bit whole numbers, to their places in the tile
+  auto widen = [&](uint32_t codes) __attribute__((always_inline)) {
+    constexpr int CH = HD / 16;  // 16-byte chunks of a row of codes
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    // this wave's scales: keys', then values'
+    const uint32_t scales = codes + (uint32_t)(G::STAGE / 2 + 64 * wave + 4 * (lane & 15));
+    const uint64_t odd = __ballot(!(fabsf(lds_ld<float>(scales)) < __builtin_inff()));
+#pragma unroll
+    for (int i = 0; i < 8 * CH / 64 || i == 0; ++i) {
+      const int x = i * 64 + lane, r = x / CH, c16 = x % CH, krow = 8 * wave + r;
+      if (8 * CH < 64 && x >= 8 * CH) break;
+      const uint32_t from = codes + (uint32_t)(krow * HD + c16 * 16);
+      const u32x4 kc = lds_ld<u32x4>(from), vc = lds_ld<u32x4>(from + G::KB * HD);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        u32x4 ko, vo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t wk = kc[2 * y + e / 2], wv = vc[2 * y + e / 2];
+          const int b = 16 * (e % 2);
+          ko[e] = T::pack_exact((float)(int8_t)(wk >> b), (float)(int8_t)(wk >> (b + 8)));
+          vo[e] = TV::pack_exact((float)(int8_t)(wv >> b), (float)(int8_t)(wv >> (b + 8)));
+        }
+        const int c = 2 * c16 + y;
+        const uint32_t to = lds0 + (uint32_t)(krow * G::ROWB);
+        lds_st(to + (uint32_t)((c ^ G::swk(krow)) << 4), ko);
+        lds_st(to + (uint32_t)(G::HALF + (((((c >> 2) ^ G::swv(krow)) << 2) | (c & 3)) << 4)), vo);
+      }
+    }
+    // a scale that is not finite makes no number of its key's score; as a value's it is taken out
+    if (odd && ((odd | odd >> 8) >> (lane & 7) & 1)) lds_st(scales, lane & 8 ? 0.0f : __builtin_nanf(""));
+  };
+  // 16-bit keys: values behind the last key, which hold it again and may be infinite, as zeros (this wave's 8)
+  auto clear = [&](uint32_t stage, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < G::NI; ++i) {
+      const int r = 8 * wave + G::RPI * i + lane / G::LPR;
+      if (kb * G::KB + r >= nk) lds_st(stage + (uint32_t)(G::HALF + r * G::ROWB + (lane % G::LPR) * 16), u32x4{0, 0, 0, 0});
+    }
+  };
+
+  // LDS places of this lane's operands: step s of K at ka ^ 32 s (the swizzle reaches 256 bytes), 32-wide block d of
+  // V at va ^ 64 (d % 4), two transposing reads of 4 keys each
+  const int s16 = lane & 15;
+  const uint32_t ka = lds0 + (uint32_t)(col * G::ROWB + ((h ^ G::swk(col)) << 4));
+  const uint32_t va = lds0 + (uint32_t)(G::HALF + (4 * h + (s16 >> 2)) * G::ROWB + (G::swv(s16 >> 2) << 6) +
+                                        ((lane >> 4) & 1) * 32 + (s16 & 3) * 8);
+  auto step = [&](auto stage_c, int kb, uint32_t scales) __attribute__((always_inline)) {
+    constexpr uint32_t stage = decltype(stage_c)::value;
+    if (R0 >= rows) return;
+    // operands are read kAhead products ahead
+    auto k_at = [&](int s) {
+      return lds_ld<u32x4>((ka ^ (uint32_t)((s & 7) << 5)) + stage + (s >= 8 ? 256u : 0u));
+    };
+    f32x16 S = {};
+    {
+      u32x4 k[kAhead];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) k[s] = k_at(s);
+#pragma unroll
+      for (int s = 0; s < G::NS; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+        S = T::mma32(k[s % kAhead], Q[s], S);
+        if (s + kAhead < G::NS) k[s % kAhead] = k_at(s + kAhead);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (Q8) {
+      // scales of keys 8 i + 4 h ..: this lane's four runs of scores
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 ks = lds_ld<f32x4>(scales + (uint32_t)(64 * i + 16 * h));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[4 * i + e] *= ks[e];
+      }
+    }
+    if (kb * G::KB + G::KB > nk) {
+      const int rel = nk - kb * G::KB - 4 * h;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 >= rel) S[i] = kNegInf;
+    }
+    float mx = fmaxf(fmaxf(S[0], S[1]), S[2]);
+#pragma unroll
+    for (int i = 3; i < 15; i += 2) mx = fmaxf(fmaxf(mx, S[i]), S[i + 1]);
+    mx = fmaxf(mx, S[15]);
+    float x, y;
+    lane_pair<32>(mx, x, y);
+    mx = fmaxf(x, y) * a.c;
+    // (sums are rescaled only when a row's maximum has grown by more than 2^8, in fp16 when a block's largest P would
+    // leave 2^-8 .. 2^15 on either side)
+    constexpr bool NARROW = TV::DT == DT_F16;
+    if (NARROW ? __any(off_window(mx - m, -8.0f, 15.0f)) : __any(mx > m + 8.0f)) {
+      float mn = fmaxf(m, mx);
+      if constexpr (NARROW) {
+        lane_pair<32>(l, x, y);
+        mn = fp16_reference(m, mx, x + y, -8.0f, 8.0f, 15.0f);
+      }
+      const float al = exp2_(m - (mn == kNegInf ? 0.0f : mn));
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[d][i] *= al;
+    }
+    const float ms = m == kNegInf ? 0.0f : m;
+    u32x4 P[PN][2];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = exp2_(fmaf(S[8 * k + e], a.c, -ms));
+        sum += p[e];
+      }
+      f32x4 vs[2];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vs[i] = lds_ld<f32x4>(scales + (uint32_t)(64 * (2 * k + i) + 32 + 16 * h));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float p0 = p[2 * e], p1 = p[2 * e + 1];
+        if constexpr (Q8) {
+          p0 *= vs[e / 2][2 * (e % 2)];
+          p1 *= vs[e / 2][2 * (e % 2) + 1];
+        }
+        const uint32_t w = TV::pack(p0, p1);
+        P[0][k][e] = w;
+        if constexpr (PN == 2) P[1][k][e] = TV::pack(p0 - bitcast<float>(w << 16), p1 - bitcast<float>(w & 0xFFFF0000u));
+      }
+    }
+    l += sum;
+    auto v_at = [&](int x) {  // operand of block x / 2, keys 16 (x % 2) ..
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      u32x2 v[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        const int d = x / 2, k = x % 2;
+        const uint32_t at = (va ^ (uint32_t)((d & 3) << 6)) + stage +
+                            (uint32_t)((d >> 2) * 256 + (16 * k + 8 * z) * G::ROWB);
+        v[z] = bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
+      }
+      return u32x4{v[0].x, v[0].y, v[1].x, v[1].y};
+    };
+    u32x4 v[kAhead];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) v[x] = v_at(x);
+#pragma unroll
+    for (int x = 0; x < 2 * G::ND; ++x) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < PN; ++n) O[x / 2] = TV::mma32(v[x % kAhead], P[n][x % 2], O[x / 2]);
+      if (x + kAhead < 2 * G::ND) v[x % kAhead] = v_at(x + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // this wave's copies have landed and its LDS accesses are done, and so for all waves
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto lds_done = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int pid = page_of(kb0);
+  if constexpr (!Q8) {
+    constexpr std::integral_constant<uint32_t, 0> s0;
+    constexpr std::integral_constant<uint32_t, (uint32_t)G::STAGE> s1;
+    issue(lds0, kb0, pid);
+    pid = page_of(kb0 + 1);
+    auto turn = [&](auto stage_c, int kb) __attribute__((always_inline)) {
+      constexpr uint32_t stage = decltype(stage_c)::value;
+      meet();
+      if (kb * G::KB + G::KB > nk) {
+        clear(lds0 + stage, kb);
+        lds_done();
+      }
+      issue(lds0 + (stage ? 0u : (uint32_t)G::STAGE), kb + 1, pid);
+      pid = page_of(kb + 2);
+      step(stage_c, kb, 0);
+    };
+    for (int kb = kb0;;) {
+      turn(s0, kb);
+      if (++kb >= kb1) break;
+      turn(s1, kb);
+      if (++kb >= kb1) break;
+    }
+  } else {
+    // codes of block kb + 1 land while block kb is widened and used
+    const uint32_t c0 = lds0 + G::STAGE;
+    constexpr uint32_t CODES = G::STAGE / 2 + G::SCALES;
+    constexpr std::integral_constant<uint32_t, 0> s0;
+    uint32_t codes = c0;
+    issue(codes, kb0, pid);
+    pid = page_of(kb0 + 1);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      meet();  // the tile has been read, this block's codes and scales are there
+      const uint32_t next = codes == c0 ? c0 + CODES : c0;
+      issue(next, kb + 1, pid);
+      pid = page_of(kb + 2);
+      widen(codes);
+      lds_done();  // the tile is written
+      step(s0, kb, codes + G::STAGE / 2);
+      codes = next;
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
+  __builtin_amdgcn_sched_barrier(0);
+
+  if (row >= rows) return;
+  float x, y;
+  lane_pair<32>(l, x, y);
+  l = any_bad ? __builtin_nanf("") : x + y;
+  const long long at = part_row(a, U, hk) + row;
+  float* o = a.part + at * HD + 4 * h;
+#pragma unroll
+  for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *(f32x4*)(o + 32 * d + 8 * i) = f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
+  if (h == 0) {
+    a.ml[at * 2] = m;
+    a.ml[at * 2 + 1] = l;
+  }
 }
 
-// NT: tiles of a prefix's unit, NO: of an own one.
-template <typename T, int HD, bool Q8, int NT, int NO>
+// Workgroups that a CU holds by registers.
+constexpr int shared_occupancy(int hd, int nt) {
+  return hd == 256 ? (nt == 2 ? 1 : 2) : hd == 128 ? (nt == 2 ? 2 : 3) : 3;
+}
+
+// NT: tiles of a prefix's unit (0: the wide form, for own keys too where a key head has more than 16 query heads).
+template <typename T, int HD, bool Q8, int NT>
 __global__ __launch_bounds__(kThreads, shared_occupancy(HD, NT)) void shared_kernel(const SharedArgs a) {
-  extern __shared__ __attribute__((aligned(16))) float lds[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int hk = (int)blockIdx.x % a.HKV, unit = (int)blockIdx.x / a.HKV;
   const Plan p = make_plan(a);
   Unit U;
   if (!find_unit(a, p, unit, U)) return;
   for (int* x : {&U.prefix, &U.src, &U.len, &U.b0, &U.n, &U.blk0, &U.blk1, &U.slot}) *x = (int)rfl32((uint32_t)*x);
-  if (U.prefix) run_unit<T, HD, Q8, NT>(a, U, hk, lds);
-  else run_unit<T, HD, Q8, NO>(a, U, hk, lds);
+  if constexpr (NT == 0) {
+    if (U.prefix || a.R > 16) {
+      wide_unit<T, HD, Q8>(a, U, hk, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+      return;
+    }
+  } else if (U.prefix) {
+    run_unit<T, HD, Q8, NT>(a, U, hk, (float*)lds);
+    return;
+  }
+  run_unit<T, HD, Q8, 1>(a, U, hk, (float*)lds);
 }
 
-// A row (sequence, query head) a workgroup: its parts, the prefix's first, in turn over 1024 / HD
-// slices of HD / 4 threads, whose sums meet in LDS.
-template <typename T, int HD>
+// Joins the parts of a sequence's rows of one key head: a workgroup takes ROWS of them, in 1024 / (HD ROWS) slices of
+// ROWS HD / 4 threads, which take parts in turn, the prefix's first; slices meet in LDS.  Few rows take one of them a
+// workgroup, many rows as many as there are threads for (each workgroup finds its parts from the lengths again).
+template <typename T, int HD, int ROWS>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a) {
-  constexpr int LPR = HD / 4, SL = kThreads / LPR, N = 8;
-  __shared__ __attribute__((aligned(16))) float so[SL * HD];
-  __shared__ float sm[SL * 2];
+  constexpr int LPR = HD / 4, SL = kThreads / (LPR * ROWS), N = 8;
+  __shared__ __attribute__((aligned(16))) float so[SL > 1 ? SL * ROWS * HD : 4];
+  __shared__ float sm[SL * ROWS * 2];
   const int tid = (int)threadIdx.x, lane = tid & 63;
-  const int hq = (int)blockIdx.x % (a.HKV * a.R), b = (int)blockIdx.x / (a.HKV * a.R);
-  const int hk = hq / a.R, head = hq - hk * a.R;
+  const int runs = (a.R + ROWS - 1) / ROWS;
+  const int u = (int)blockIdx.x / runs, b = u / a.HKV, hk = u - b * a.HKV;
+  const int s = tid / (LPR * ROWS), rr = tid / LPR % ROWS, f = tid % LPR;
+  const int head = ((int)blockIdx.x - u * runs) * ROWS + rr;
   const Plan p = make_plan(a);
   if (b < p.lo || b >= p.hi) return;  // a row of no group
   // parts of the prefix: slots pslot, pslot + 1, ..., row prow of each
   int base = 0, start = 0, pslot = 0, np = 0, prow = 0;
   for (int g0 = 0; g0 < a.G; g0 += 64) {
-    const Group g = group_of(a, g0, start);
+    const Group g = group_of(a, groups_at(a, p, g0), start);
     const int tiles = tiles_of(a, g), parts = parts_of(p, g.len);
     const int end = wave_scan(tiles * parts);
     const uint64_t mine = __ballot(b >= g.b0 && b < g.b0 + g.n);
@@ -539,14 +917,14 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
       const int nt = lane_value(tiles, at), in = b - lane_value(g.b0, at);
       np = nt ? lane_value(parts, at) : 0;
       pslot = base + lane_value(end, at) - nt * np + in / a.spt * np;
-      prow = in % a.spt * a.R + head;
+      prow = in % a.spt * a.R;
       break;
     }
     base += lane_value(end, 63);
   }
   int oslot = 0, no = 0;
-  for (int b0 = p.lo; b0 < p.hi; b0 += 64) {
-    const int parts = parts_of(p, own_length(a, p, b0 + lane));
+  for (int b0 = 0; b0 < p.hi; b0 += 64) {
+    const int parts = parts_of(p, own_at(a, p, b0));
     const int end = wave_scan(parts);
     if (b < b0 + 64) {
       no = lane_value(parts, b - b0);
@@ -555,12 +933,12 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
     }
     oslot += lane_value(end, 63);
   }
+  const int hrow = min(head, a.R - 1);  // (rows behind the last are the last again, and not stored)
   const long long first = (long long)hk * a.rows;
-  const long long pre0 = first + (long long)pslot * (a.spt * a.R) + prow;
-  const long long own0 = first + a.own_rows + (long long)oslot * a.R + head;
+  const long long pre0 = first + (long long)pslot * (a.spt * a.R) + prow + hrow;
+  const long long own0 = first + a.own_rows + (long long)oslot * a.R + hrow;
   const int n = np + no;
   auto row_of = [&](int i) { return i < np ? pre0 + (long long)i * (a.spt * a.R) : own0 + (long long)(i - np) * a.R; };
-  const int s = tid / LPR, f = tid % LPR;
   f32x4 o = {0, 0, 0, 0};
   float M = kNegInf, ls = 0.0f;
   for (int i0 = s; i0 < n; i0 += SL * N) {
@@ -587,45 +965,54 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
       M = mn;
     }
   }
-  *(f32x4*)(so + s * HD + f * 4) = o;
-  if (f == 0) sm[s * 2] = M, sm[s * 2 + 1] = ls;
-  __syncthreads();
-  if (tid >= LPR) return;
-  f32x4 r = {0, 0, 0, 0};
-  float top = kNegInf, sum = 0.0f;
+  if constexpr (SL > 1) {
+    *(f32x4*)(so + tid * 4) = o;
+    if (f == 0) sm[tid / LPR * 2] = M, sm[tid / LPR * 2 + 1] = ls;
+    __syncthreads();
+    if (s > 0) return;
+    float top = kNegInf, sum = 0.0f;
+    o = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < SL; ++i) top = fmaxf(top, sm[i * 2]);
-  const float ts = top == kNegInf ? 0.0f : top;
+    for (int i = 0; i < SL; ++i) top = fmaxf(top, sm[(i * ROWS + rr) * 2]);
+    const float ts = top == kNegInf ? 0.0f : top;
 #pragma unroll
-  for (int i = 0; i < SL; ++i) {
-    const float e = exp2_(sm[i * 2] - ts);
-    r += *(const f32x4*)(so + i * HD + tid * 4) * e;
-    sum += sm[i * 2 + 1] * e;
+    for (int i = 0; i < SL; ++i) {
+      const float e = exp2_(sm[(i * ROWS + rr) * 2] - ts);
+      o += *(const f32x4*)(so + (i * ROWS * LPR + tid) * 4) * e;
+      sum += sm[(i * ROWS + rr) * 2 + 1] * e;
+    }
+    ls = sum;
   }
-  const float inv = n == 0 ? 0.0f : 1.0f / sum;  // a sequence without keys: zeros
-  *(u32x2*)((uint16_t*)a.o + b * a.ob + hq * a.oh + tid * 4) =
-      u32x2{T::pack(r[0] * inv, r[1] * inv), T::pack(r[2] * inv, r[3] * inv)};
+  if (head >= a.R) return;
+  const float inv = n == 0 ? 0.0f : 1.0f / ls;  // a sequence without keys: zeros
+  *(u32x2*)((uint16_t*)a.o + b * a.ob + (hk * a.R + head) * a.oh + f * 4) =
+      u32x2{T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv)};
 }
 
-template <typename T, int HD, bool Q8, int NT, int NO>
+template <typename T, int HD, bool Q8, int NT>
 hipError_t launch_nt(const SharedArgs& a, hipStream_t st) {
-  auto kern = shared_kernel<T, HD, Q8, NT, NO>;
-  constexpr size_t lds = shared_lds<HD>(NT > NO ? NT : NO);
+  auto kern = shared_kernel<T, HD, Q8, NT>;
+  constexpr int wide = NT == 0 ? prompt_lds<HD, Q8, 1>() : 0, thin = shared_lds<HD>(NT == 0 ? 1 : NT);
+  constexpr size_t lds = wide > thin ? wide : thin;
   static std::atomic<uint64_t> done{0};
   hipError_t e = allow_lds((const void*)kern, lds, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.units * a.HKV)), dim3(kThreads), lds, st, a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL((shared_join_kernel<T, HD>), dim3((unsigned)(a.B * a.HKV * a.R)), dim3(kThreads), 0, st, a);
+  constexpr int MANY = 1024 / HD;
+  if ((long long)a.B * a.HKV * a.R >= kSharedManyRows && a.R >= MANY)
+    hipLaunchKernelGGL((shared_join_kernel<T, HD, MANY>), dim3((unsigned)(a.B * a.HKV * ((a.R + MANY - 1) / MANY))),
+                       dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((shared_join_kernel<T, HD, 1>), dim3((unsigned)(a.B * a.HKV * a.R)), dim3(kThreads), 0, st, a);
   return hipGetLastError();
 }
 
 template <typename T, int HD, bool Q8>
 hipError_t launch_q(const SharedArgs& a, hipStream_t st) {
-  if (a.R > 16) return launch_nt<T, HD, Q8, 4, 4>(a, st);
-  if (a.tiles == 1) return launch_nt<T, HD, Q8, 1, 1>(a, st);
-  if (a.tiles == 2) return launch_nt<T, HD, Q8, 2, 1>(a, st);
-  return launch_nt<T, HD, Q8, 4, 1>(a, st);
+  if (a.tiles == 1) return launch_nt<T, HD, Q8, 1>(a, st);
+  if (a.tiles == 2) return launch_nt<T, HD, Q8, 2>(a, st);
+  return launch_nt<T, HD, Q8, 0>(a, st);
 }
 
 template <typename T, int HD>
