@@ -227,14 +227,25 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
 // Row tiles and units of a decode step over shared prefixes.
 int plan_shared(const char* fn, SharedArgs& a, int hd, int page, char* part, size_t avail) {
   const long long rows = (long long)((a.B + a.G - 1) / a.G) * a.R;  // of a prefix, on average
-  a.tiles = a.R > 16 || rows > 32 ? 8 : rows > 16 ? 2 : 1;
+  // 17 to 32 rows take one unit of two tiles, or two of one, which read the keys twice (the second time from the L2) but
+  // come two to a CU (of 256 values) and more even: 8 sequences of 4 query heads to a key head, one / two tiles: of 256
+  // values behind 8000 tokens 17.8 / 20.0 us, 64000 40 / 48, 100003 65 / 55; of 128 behind 2000 10.7 / 11.7, 32000 21.8 /
+  // 21.4, six prompts of up to 6000 35 / 31.  int8 keys are cheaper read than two tiles are kept in registers.
+  const long long keys = std::max(1, a.pre.max_pages) * (long long)page, own = std::max(1, a.own.max_pages) * (long long)page;
+  const bool q8 = a.own.k.s != nullptr;
+  const long long bytes = (long long)a.G * keys * a.HKV * hd * 4;
+  const bool two = rows > 16 && !q8 && bytes > (hd == 256 ? 160LL << 20 : 24LL << 20);
+  a.tiles = a.R > 16 || rows > 32 ? 8 : two ? 2 : 1;
   a.spt = 16 * a.tiles / a.R;
-  long long few = 256, total = 512;
+  // One workgroup a CU as long as that makes units of at most `brief` blocks: more of them read no faster and leave more
+  // sums to join (8 sequences behind 32000 tokens of 256 values, 256 / 512 units: 25 / 31 us).  Where vector work bounds
+  // a wide unit (int8 keys, 64 values), three (64 sequences behind 16384 int8 keys of 256 values 54 -> 43 us).
+  long long few = a.tiles == 8 && (q8 || hd == 64) ? 768 : 256, total = two && hd == 256 ? 256 : std::max(512LL, few);
+  a.brief = q8 ? 24 : 32;
   if (const char* e = getenv("QLIN_SHARED_UNITS")) {  // for tuning runs
     if (atoi(e) > 0) few = total = atoi(e);
   }
   const long long tiles = a.B / a.spt + a.G;  // units of a prefix that is not cut
-  const long long keys = std::max(1, a.pre.max_pages) * (long long)page, own = std::max(1, a.own.max_pages) * (long long)page;
   const long long bound = tiles * ((keys + 4 * kSharedBlock - 1) / (4 * kSharedBlock)) +
                           a.B * ((own + 4 * kSharedBlock - 1) / (4 * kSharedBlock));
   long long target = std::min(std::max(1LL, total / a.HKV), bound);

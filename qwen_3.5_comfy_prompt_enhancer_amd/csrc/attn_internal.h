@@ -102,6 +102,7 @@ struct SharedArgs {
   int spt;                // sequences of a prefix's unit
   float c;                // scale * log2(e)
   int target, few;        // units of a key head that long and short work is cut into
+  int brief;              // blocks of a unit up to which work is short
   int units;              // units per key head: the grid's bound
   long long own_rows;     // rows of parts of a key head in front of the own ones
   long long rows;         // rows of parts of a key head
@@ -109,8 +110,9 @@ struct SharedArgs {
   float* ml;              // [key head][row][2] reference and sum of P
 };
 constexpr int kSharedBlock = 32;     // keys a wave takes at a time
-constexpr int kSharedLong = 32;      // blocks of a unit up to which fewer units are better
 constexpr int kSharedManyRows = 1024;  // rows of a call from which a workgroup joins several
+constexpr int kSharedFewRows = 256;    // rows of a call up to which a join may take 512 threads,
+constexpr int kSharedManyKeys = 4096;  // for prefixes (by their table) of more keys
 hipError_t launch_shared_bf16(const SharedArgs& a, int hd, hipStream_t st);
 hipError_t launch_shared_f16(const SharedArgs& a, int hd, hipStream_t st);
 

@@ -107,7 +107,7 @@ __device__ __forceinline__ Plan make_plan(const SharedArgs& a) {
   for (int b0 = 0; b0 < p.hi; b0 += 64) total += (float)blocks_of(own_at(a, p, b0));
   total = lane_value(wave_scan(total), 63);
   const float few = ceilf(total / (float)a.few), most = ceilf(total / (float)a.target);
-  p.chunk = max((int)fminf(few <= (float)kSharedLong ? few : fmaxf((float)kSharedLong, most), 1e8f), 1);
+  p.chunk = max((int)fminf(few <= (float)a.brief ? few : fmaxf((float)a.brief, most), 1e8f), 1);
   p.chunk = (p.chunk + kWaves - 1) / kWaves * kWaves;
   return p;
 }
@@ -192,7 +192,15 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // Dwords of codes that the compiler must not take apart before they are used (it would carry
 // single bytes, a register each, around the loop).
-__device__ __forceinline__ void opaque(uint32_t& a, uint32_t& b) { asm volatile("" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void opaque(uint32_t& a) { asm volatile("" : "+v"(a)); }
+__device__ __forceinline__ void opaque(u32x2& a) { asm volatile("" : "+v"(a)); }
+__device__ __forceinline__ void opaque(u32x4& a) { asm volatile("" : "+v"(a)); }
+
+// int8 keys: a query is the sum of three int8 digits, q = m / 127 (d0 + d1 / 254 + d2 / 254^2) with the row's
+// largest m, off by at most half of m / 127 / 254^2 (2^-24 m, and a step of 32 bits of each product on the way).  The
+// products with codes are then whole numbers of the matrix units, added up exactly, and no code is widened (as bf16
+// numbers a block's keys took 192 vector instructions: MEASURED).
+constexpr int DIGITS = 3;
 
 // Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
 template <typename T>
@@ -207,8 +215,8 @@ __device__ __forceinline__ long long part_row(const SharedArgs& a, const Unit& U
 
 // Dynamic LDS: the queries of NT tiles as operands; behind the loop the waves' sums of a tile.
 template <int HD>
-constexpr int shared_lds(int nt) {
-  const int q = nt * (HD / 32) * 1024 + kWaves * 256, join = kWaves * 16 * (HD + 4) * 4 + kWaves * 128;
+constexpr int shared_lds(int nt, bool q8) {
+  const int q = nt * (q8 ? DIGITS * (HD / 64) : HD / 32) * 1024 + nt * 64 + kWaves * 256, join = kWaves * 16 * (HD + 4) * 4 + kWaves * 128;
   return q > join ? q : join;
 }
 
@@ -226,21 +234,25 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
   const KvSrc& kv = U.prefix ? a.pre : a.own;
   const int rows = U.n * a.R;
 
-  // queries to LDS, as operands: step s of tile t at ((t STEPS + s) 64 + lane) 16 bytes, column j = row
-  // 16 t + j, the same hd order as a key's loads.  (Loaded in front of the first block, written behind its loads.)
+  // queries, column j = row 16 t + j: loaded in front of the first block, written to LDS as operands behind its loads
   constexpr int QL = (NT * STEPS + kWaves - 1) / kWaves;
   u32x4 qr[QL];
+  auto q_at = [&](int i, int& row, int& s, int& l) {
+    const int x = i * kThreads + tid;
+    l = x & 63, s = (x >> 6) % STEPS, row = (x >> 6) / STEPS * 16 + (l & 15);
+    return x < NT * STEPS * 64;
+  };
 #pragma unroll
   for (int i = 0; i < QL; ++i) {
-    const int x = i * kThreads + tid, l = x & 63, s = (x >> 6) % STEPS, row = (x >> 6) / STEPS * 16 + (l & 15);
+    int row, s, l;
+    const bool some = q_at(i, row, s, l);
     const int d = Q8 ? 64 * (s / 2) + 16 * (l >> 4) + 8 * (s % 2) : 32 * s + 8 * (l >> 4);
     const int seq = row / a.R;
     qr[i] = u32x4{0, 0, 0, 0};
-    if (row < rows)
+    if (some && row < rows)
       qr[i] = ld_global<u32x4>((const uint16_t*)a.q + (U.b0 + seq) * a.qb + (hk * a.R + (row - seq * a.R)) * a.qh + d);
   }
   const f32x4* lq = (const f32x4*)lds + lane;
-
   f32x4 O[NT][VC * VW];
   float m[NT], l[NT];
 #pragma unroll
@@ -322,11 +334,59 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
     pages(blk + kWaves, pin);
   }
   __builtin_amdgcn_sched_barrier(0);
+  constexpr int QF = Q8 ? NT * DIGITS * KL * 256 : NT * STEPS * 256;  // floats of the operands
+  float qscale[NT];
+  if constexpr (!Q8) {
+    // step s of tile t at ((t STEPS + s) 64 + lane) 16 bytes
 #pragma unroll
-  for (int i = 0; i < QL; ++i)
-    if (i * kThreads + tid < NT * STEPS * 64) *(u32x4*)(lds + (i * kThreads + tid) * 4) = qr[i];
+    for (int i = 0; i < QL; ++i)
+      if (i * kThreads + tid < NT * STEPS * 64) *(u32x4*)(lds + (i * kThreads + tid) * 4) = qr[i];
+  } else {
+    // digits (see query_digits): number n of 64 values i of tile t at (((t DIGITS + n) KL + i) 64 + lane) 16 bytes
+    constexpr uint32_t LEAST = 0x04000000u;  // (2^-119: 127 over it is a number)
+    uint32_t* most = (uint32_t*)(lds + QF);  // the rows' largest, as bits
+    if (tid < NT * 16) most[tid] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      int row, s, l;
+      if (!q_at(i, row, s, l)) continue;
+      uint32_t top = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, bitcast<uint32_t>(T::get((uint16_t)(qr[i][e / 2] >> (16 * (e % 2))))) & 0x7FFFFFFFu);
+      atomicMax(most + row, top);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      int row, s, l;
+      if (!q_at(i, row, s, l)) continue;
+      const float inv = 127.0f / bitcast<float>(max(most[row], LEAST));
+      uint32_t w[DIGITS][2] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float r = T::get((uint16_t)(qr[i][e / 2] >> (16 * (e % 2)))) * inv;
+#pragma unroll
+        for (int n = 0; n < DIGITS; ++n) {
+          const float d = fminf(fmaxf(rintf(r), -127.0f), 127.0f);
+          r = (r - d) * 254.0f;
+          w[n][e / 4] |= ((uint32_t)(int)d & 0xFFu) << (8 * (e % 4));
+        }
+      }
+      const int t = row / 16;
+#pragma unroll
+      for (int n = 0; n < DIGITS; ++n)
+        *(u32x2*)((uint32_t*)lds + (((t * DIGITS + n) * KL + s / 2) * 64 + l) * 4 + 2 * (s % 2)) = u32x2{w[n][0], w[n][1]};
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint32_t top = most[16 * t + j];
+      // (a query that is not finite makes numbers of no score)
+      qscale[t] = top < 0x7F800000u ? bitcast<float>(max(top, LEAST)) / 127.0f * a.c : __builtin_nanf("");
+    }
+  }
   __syncthreads();
-  float* lsc = lds + NT * STEPS * 256 + wave * 64;
+  float* lsc = lds + QF + NT * 16 + wave * 64;
   for (; blk < blk1; blk += kWaves) {
     const bool more = blk + kWaves < blk1;
     f32x4 S[NT][2];
@@ -349,32 +409,37 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
       }
       __builtin_amdgcn_wave_barrier();
     }
+    if constexpr (Q8) {
+      // the codes as they are, times each digit of the queries: whole numbers
+      const u32x4* lw = (const u32x4*)lds + lane;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) S[t][0] = S[t][1] = f32x4{0, 0, 0, 0};
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      u32x4 qv[NT];
+        for (int t = 0; t < NT; ++t) {
+          i32x4 D[DIGITS];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) qv[t] = bitcast<u32x4>(lq[(t * STEPS + s) * 64]);
+          for (int n = 0; n < DIGITS; ++n) {
+            D[n] = i32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 kop;
-        if constexpr (Q8) {
-          const u32x4 r = kr[h][s / 2];
-          const uint32_t w0 = s % 2 ? r.z : r.x, w1 = s % 2 ? r.w : r.y;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w = e < 2 ? w0 : w1;
-            const int c = 2 * (e % 2);
-            asm volatile("" : "+v"(w));
-            kop[e] = T::pack_exact((float)(int8_t)(w >> (8 * c)), (float)(int8_t)(w >> (8 * c + 8)));
+            for (int i = 0; i < KL; ++i)
+              D[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bitcast<i32x4>(kr[h][i]), bitcast<i32x4>(lw[((t * DIGITS + n) * KL + i) * 64]), D[n], 0, 0, 0);
           }
-        } else {
-          kop = kr[h][s];
-        }
-        if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) S[t][h] = T::mma16(kop, qv[t], S[t][h]);
+          for (int e = 0; e < 4; ++e)
+            S[t][h][e] = fmaf(fmaf((float)D[2][e], 1.0f / 254.0f, (float)D[1][e]), 1.0f / 254.0f, (float)D[0][e]) * ks[h][e];
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) S[t][0] = S[t][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        u32x4 qv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) qv[t] = bitcast<u32x4>(lq[(t * STEPS + s) * 64]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) S[t][h] = T::mma16(kr[h][s], qv[t], S[t][h]);
       }
     }
     if (more) load_k(blk + kWaves, pin);
@@ -397,7 +462,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * h + i] = (Q8 ? S[t][h][i] * ks[h][i] : S[t][h][i]) * a.c;
+        for (int i = 0; i < 4; ++i) x[4 * h + i] = S[t][h][i] * (Q8 ? qscale[t] : a.c);
       if (last) {
 #pragma unroll
         for (int s = 0; s < 8; ++s)
@@ -440,32 +505,45 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
         for (int c = 0; c < VC * VW; ++c) O[t][c] *= al;
       }
     }
+    if constexpr (Q8) {
 #pragma unroll
-    for (int c = 0; c < VC; ++c)
+      for (int r = 0; r < 8; ++r)
 #pragma unroll
-      for (int x = 0; x < VW; ++x) {
-        u32x4 vop;
+        for (int c = 0; c < VC; ++c) opaque(vr[r][c]);
+    }
+    // value column y of the lane's VC VW: its 8 keys
+    auto v_op = [&](int y) {
+      const int c = y / VW, x = y % VW;
+      u32x4 vop;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t w0, w1;
-          constexpr int PER = 4 / ES;  // columns of a dword
-          if constexpr (VB == 4) {
-            w0 = vr[2 * e][c];
-            w1 = vr[2 * e + 1][c];
-          } else {
-            w0 = vr[2 * e][c][x / PER];
-            w1 = vr[2 * e + 1][c][x / PER];
-          }
-          if constexpr (Q8) opaque(w0, w1);
-          vop[e] = Q8 ? codes2<TV>(w0, w1, x % PER) : perm(w1, w0, x % 2 ? 0x07060302u : 0x05040100u);
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w0, w1;
+        constexpr int PER = 4 / ES;  // columns of a dword
+        if constexpr (VB == 4) {
+          w0 = vr[2 * e][c];
+          w1 = vr[2 * e + 1][c];
+        } else {
+          w0 = vr[2 * e][c][x / PER];
+          w1 = vr[2 * e + 1][c][x / PER];
         }
-        // (left to itself the compiler widens every column first, and spills)
-        if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int n = 0; n < (Q8 ? 2 : 1); ++n) O[t][c * VW + x] = TV::mma16(vop, pop[t][n], O[t][c * VW + x]);
+        vop[e] = Q8 ? codes2<TV>(w0, w1, x % PER) : perm(w1, w0, x % 2 ? 0x07060302u : 0x05040100u);
       }
+      return vop;
+    };
+    u32x4 vop;
+    if constexpr (Q8) vop = v_op(0);
+#pragma unroll
+    for (int y = 0; y < VC * VW; ++y) {
+      const u32x4 now = Q8 ? vop : v_op(y);
+      if constexpr (Q8) {
+        if (y + 1 < VC * VW) vop = v_op(y + 1);
+        __builtin_amdgcn_sched_barrier(0);  // (left to itself the compiler widens every column first, and spills)
+      }
+#pragma unroll
+      for (int n = 0; n < (Q8 ? 2 : 1); ++n)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) O[t][y] = TV::mma16(now, pop[t][n], O[t][y]);
+    }
     if (more) {
       load_v(blk + kWaves, pin);
       pages(blk + 2 * kWaves, pin);
@@ -893,12 +971,12 @@ __global__ __launch_bounds__(kThreads, shared_occupancy(HD, NT)) void shared_ker
 // Joins the parts of a sequence's rows of one key head: a workgroup takes ROWS of them, in 1024 / (HD ROWS) slices of
 // ROWS HD / 4 threads, which take parts in turn, the prefix's first; slices meet in LDS.  Few rows take one of them a
 // workgroup, many rows as many as there are threads for (each workgroup finds its parts from the lengths again).
-template <typename T, int HD, int ROWS>
-__global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs a) {
-  constexpr int LPR = HD / 4, SL = kThreads / (LPR * ROWS), N = 8;
+template <typename T, int HD, int ROWS, int THREADS>
+__global__ __launch_bounds__(THREADS) void shared_join_kernel(const SharedArgs a) {
+  constexpr int LPR = HD / 4, SL = THREADS / (LPR * ROWS), N = 8;
   __shared__ __attribute__((aligned(16))) float so[SL > 1 ? SL * ROWS * HD : 4];
   __shared__ float sm[SL * ROWS * 2];
-  const int tid = (int)threadIdx.x, lane = tid & 63;
+  const int tid = (int)threadIdx.x;
   const int runs = (a.R + ROWS - 1) / ROWS;
   const int u = (int)blockIdx.x / runs, b = u / a.HKV, hk = u - b * a.HKV;
   const int s = tid / (LPR * ROWS), rr = tid / LPR % ROWS, f = tid % LPR;
@@ -992,26 +1070,32 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(const SharedArgs 
 template <typename T, int HD, bool Q8, int NT>
 hipError_t launch_nt(const SharedArgs& a, hipStream_t st) {
   auto kern = shared_kernel<T, HD, Q8, NT>;
-  constexpr int wide = NT == 0 ? prompt_lds<HD, Q8, 1>() : 0, thin = shared_lds<HD>(NT == 0 ? 1 : NT);
+  constexpr int wide = NT == 0 ? prompt_lds<HD, Q8, 1>() : 0, thin = shared_lds<HD>(NT == 0 ? 1 : NT, Q8);
   constexpr size_t lds = wide > thin ? wide : thin;
   static std::atomic<uint64_t> done{0};
   hipError_t e = allow_lds((const void*)kern, lds, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.units * a.HKV)), dim3(kThreads), lds, st, a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
+  // (64 rows of 65 parts with 256 / 512 / 1024 threads: 6.1 / 5.3 / 6.6 us, of few parts 4.3 / 5.1 / 5.9; 576 rows of 45
+  // 6.7 / 7.6 / 12.6; 2048 rows of 17 one by one 13.6, eight to a workgroup 8.5)
   constexpr int MANY = 1024 / HD;
-  if ((long long)a.B * a.HKV * a.R >= kSharedManyRows && a.R >= MANY)
-    hipLaunchKernelGGL((shared_join_kernel<T, HD, MANY>), dim3((unsigned)(a.B * a.HKV * ((a.R + MANY - 1) / MANY))),
-                       dim3(kThreads), 0, st, a);
+  const long long rows = (long long)a.B * a.HKV * a.R;
+  if (rows >= kSharedManyRows && a.R >= MANY)
+    hipLaunchKernelGGL((shared_join_kernel<T, HD, MANY, 256>), dim3((unsigned)(a.B * a.HKV * ((a.R + MANY - 1) / MANY))),
+                       dim3(256), 0, st, a);
+  else if (HD < 256 || rows > kSharedFewRows || a.pre.max_pages <= (kSharedManyKeys >> a.pre.page_shift))
+    hipLaunchKernelGGL((shared_join_kernel<T, HD, 1, 256>), dim3((unsigned)rows), dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((shared_join_kernel<T, HD, 1>), dim3((unsigned)(a.B * a.HKV * a.R)), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((shared_join_kernel<T, HD, 1, 512>), dim3((unsigned)rows), dim3(512), 0, st, a);
   return hipGetLastError();
 }
 
 template <typename T, int HD, bool Q8>
 hipError_t launch_q(const SharedArgs& a, hipStream_t st) {
   if (a.tiles == 1) return launch_nt<T, HD, Q8, 1>(a, st);
-  if (a.tiles == 2) return launch_nt<T, HD, Q8, 2>(a, st);
+  if constexpr (!Q8)
+    if (a.tiles == 2) return launch_nt<T, HD, Q8, 2>(a, st);
   return launch_nt<T, HD, Q8, 0>(a, st);
 }
 
