@@ -51,6 +51,8 @@ EXTRA = {
     # the same for prompt attention's 128 accumulators and 64 query registers per lane (heads of 256 values)
     "attn_prompt_bf16.hip": _VGPR_FORM,
     "attn_prompt_f16.hip": _VGPR_FORM,
+    "attn_shared_wide_bf16.hip": _VGPR_FORM,
+    "attn_shared_wide_f16.hip": _VGPR_FORM,
 }
 
 

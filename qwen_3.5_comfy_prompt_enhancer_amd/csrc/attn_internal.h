@@ -115,6 +115,8 @@ constexpr int kSharedFewRows = 256;    // rows of a call up to which a join may 
 constexpr int kSharedManyKeys = 4096;  // for prefixes (by their table) of more keys
 hipError_t launch_shared_bf16(const SharedArgs& a, int hd, hipStream_t st);
 hipError_t launch_shared_f16(const SharedArgs& a, int hd, hipStream_t st);
+hipError_t launch_shared_wide_bf16(const SharedArgs& a, int hd, hipStream_t st);
+hipError_t launch_shared_wide_f16(const SharedArgs& a, int hd, hipStream_t st);
 
 // Attention of packed prompts over packed keys or a paged cache (attn_prompt*.hip).
 struct PromptArgs {

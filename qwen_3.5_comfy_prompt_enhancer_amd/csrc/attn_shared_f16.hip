@@ -3,6 +3,8 @@
 
 namespace qlin {
 
-hipError_t launch_shared_f16(const SharedArgs& a, int hd, hipStream_t st) { return launch_shared_t<F16>(a, hd, st); }
+hipError_t launch_shared_f16(const SharedArgs& a, int hd, hipStream_t st) {
+  return a.tiles == 8 ? launch_shared_wide_f16(a, hd, st) : launch_shared_t<F16, false>(a, hd, st);
+}
 
 }  // namespace qlin

@@ -740,6 +740,8 @@ __device__ __forceinline__ void wide_unit(const SharedArgs& a, const Unit& U, in
   };
   // 16-bit keys: values behind the last key, which hold it again and may be infinite, as zeros (this wave's 8)
   auto clear = [&](uint32_t stage, int kb) __attribute__((always_inline)) {
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
 #pragma unroll
     for (int i = 0; i < G::NI; ++i) {
       const int r = 8 * wave + G::RPI * i + lane / G::LPR;
@@ -783,7 +785,9 @@ __device__ __forceinline__ void wide_unit(const SharedArgs& a, const Unit& U, in
       }
     }
     if (kb * G::KB + G::KB > nk) {
-      const int rel = nk - kb * G::KB - 4 * h;
+      int lane = (int)threadIdx.x & 63;
+      asm volatile("" : "+v"(lane));
+      const int rel = nk - kb * G::KB - 4 * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (8 * (i / 4) + i % 4 >= rel) S[i] = kNegInf;
@@ -925,18 +929,22 @@ __device__ __forceinline__ void wide_unit(const SharedArgs& a, const Unit& U, in
   __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no copy may outlive the workgroup
   __builtin_amdgcn_sched_barrier(0);
 
-  if (row >= rows) return;
+  // (the lane's row anew, instead of in a register through the loop)
+  int last = (int)threadIdx.x;
+  asm volatile("" : "+v"(last));
+  const int mine = R0 + (last & 31), half = (last >> 5) & 1;
+  if (mine >= rows) return;
   float x, y;
   lane_pair<32>(l, x, y);
   l = any_bad ? __builtin_nanf("") : x + y;
-  const long long at = part_row(a, U, hk) + row;
-  float* o = a.part + at * HD + 4 * h;
+  const long long at = part_row(a, U, hk) + mine;
+  float* o = a.part + at * HD + 4 * half;
 #pragma unroll
   for (int d = 0; d < G::ND; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       *(f32x4*)(o + 32 * d + 8 * i) = f32x4{O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
-  if (h == 0) {
+  if (half == 0) {
     a.ml[at * 2] = m;
     a.ml[at * 2 + 1] = l;
   }
@@ -1091,26 +1099,25 @@ hipError_t launch_nt(const SharedArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <typename T, int HD, bool Q8>
-hipError_t launch_q(const SharedArgs& a, hipStream_t st) {
-  if (a.tiles == 1) return launch_nt<T, HD, Q8, 1>(a, st);
-  if constexpr (!Q8)
-    if (a.tiles == 2) return launch_nt<T, HD, Q8, 2>(a, st);
-  return launch_nt<T, HD, Q8, 0>(a, st);
-}
-
-template <typename T, int HD>
-hipError_t launch_hd(const SharedArgs& a, hipStream_t st) {
-  return a.own.k.s ? launch_q<T, HD, true>(a, st) : launch_q<T, HD, false>(a, st);
-}
-
 }  // namespace
 
-template <typename T>
+// WIDE: the form of many rows (in files of their own, as it is compiled with other flags)
+template <typename T, int HD, bool WIDE>
+hipError_t launch_shared_hd(const SharedArgs& a, hipStream_t st) {
+  const bool q8 = a.own.k.s != nullptr;
+  if constexpr (WIDE) {
+    return q8 ? launch_nt<T, HD, true, 0>(a, st) : launch_nt<T, HD, false, 0>(a, st);
+  } else {
+    if (a.tiles == 2 && !q8) return launch_nt<T, HD, false, 2>(a, st);
+    return q8 ? launch_nt<T, HD, true, 1>(a, st) : launch_nt<T, HD, false, 1>(a, st);
+  }
+}
+
+template <typename T, bool WIDE>
 hipError_t launch_shared_t(const SharedArgs& a, int hd, hipStream_t st) {
-  if (hd == 256) return launch_hd<T, 256>(a, st);
-  if (hd == 128) return launch_hd<T, 128>(a, st);
-  return launch_hd<T, 64>(a, st);
+  if (hd == 256) return launch_shared_hd<T, 256, WIDE>(a, st);
+  if (hd == 128) return launch_shared_hd<T, 128, WIDE>(a, st);
+  return launch_shared_hd<T, 64, WIDE>(a, st);
 }
 
 }  // namespace qlin

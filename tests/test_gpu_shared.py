@@ -277,3 +277,53 @@ def test_cache_past_4_gib():
     c.cache = (k, v, None, None)
     c.run(prefix_table=far(c.ptable), table=far(c.table))
     R.check(c.out, ref, tol)
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("n", [3, 20])
+def test_odd_queries(dt, int8, n):
+    """A query that is no number, infinite, zero or tiny concerns its own head of its own sequence alone."""
+    c = S.Batch([(n, 300)], [40 + i for i in range(n)], 8, 2, 128, dt, seed=79, int8=int8, page=16)
+    c.q[0, 3, 7] = float("nan")
+    c.q[1, 5, 0] = float("inf")
+    c.q[2, 0] = 0.0
+    c.q[2, 1] *= 2.0 ** -14
+    c.run()
+    ref, tol = c.expected()
+    odd = torch.zeros((n, 8), dtype=torch.bool, device="cuda")
+    odd[0, 3] = odd[1, 5] = True
+    assert bool(c.out[odd].isnan().all())
+    R.check(c.out[~odd], ref[~odd], tol[~odd])
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (32, 1)])
+def test_odd_scales(hq, hkv):
+    """An int8 cache's scales that are not finite: a key's makes no number of what sees it, whatever its score's
+    sign, and places behind the end may hold anything."""
+    c = S.Batch([(4, 100), (3, 40)], [5, 20, 33, 1, 7, 0, 9], hq, hkv, 128, BF, seed=83, page=16, int8=True)
+    _, _, ks, vs = c.cache
+    ref, tol = c.expected()
+    ks[c.ptable[0, 6].long(), 4:] = float("inf")      # behind the first prefix's end
+    vs[c.table[1, 1].long(), 4:] = float("nan")       # behind the second sequence's
+    ks[c.table[4, 0].long(), 3] = float("-inf")       # a key of the fifth sequence
+    c.run()
+    some = [0, 1, 2, 3, 5, 6]
+    R.check(c.out[some], ref[some], tol[some])
+    assert bool(c.out[4].isnan().all())
+
+
+def test_infinite_values_behind_the_end():
+    """Wide tiles zero the values behind the last key, which hold it again: an infinite last value stays in its own
+    column (and makes that column infinite)."""
+    for n in (2, 40):
+        c = S.Batch([(n, 77)], [0] * n, 4, 1, 128, BF, seed=89, page=16)
+        _, v, _, _ = c.cache
+        v[c.ptable[0, 4].long(), 12, 0, 5] = float("inf")     # the 77th key's
+        ref, tol = c.expected()
+        c.run()
+        assert bool((c.out[..., 5] == float("inf")).all())
+        rest = [i for i in range(128) if i != 5]
+        v[c.ptable[0, 4].long(), 12, 0, 5] = 0.0
+        ref, tol = c.expected()
+        R.check(c.out[..., rest], ref[..., rest], tol[..., rest])
