@@ -98,7 +98,7 @@ struct SharedArgs {
   KvSrc pre, own;         // one cache; pre: a group's table row and length, own: a sequence's
   const int* cu;          // [G + 1] sequences of each group
   int G, B, HKV, R;       // R: query heads of a key head
-  int tiles;              // 16-row tiles of a prefix's unit: 1, 2, 4, or 8 in the wide form
+  int tiles;              // 16-row tiles of a prefix's unit: 1, 2, or 8 in the wide form
   int spt;                // sequences of a prefix's unit
   float c;                // scale * log2(e)
   int target, few;        // units of a key head that long and short work is cut into

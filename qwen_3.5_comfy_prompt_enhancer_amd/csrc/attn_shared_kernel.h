@@ -1,32 +1,38 @@
 // Attention of one new token per sequence, of groups of sequences that share a prefix: the kernel
-// template, included by attn_shared_bf16.hip and attn_shared_f16.hip.
+// templates, included by attn_shared_{bf16,f16}.hip and, for many rows, attn_shared_wide_{bf16,f16}.hip.
 //
 //   o[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max)
 //   over the prefix's keys of the sequence's group and the sequence's own keys
 //
-// Bound by the bytes of the cache as long as a group's rows are few: a prefix's keys are read once
-// for all rows (sequences x query heads) of a key head, up to 16 NT of them in a workgroup; groups of
-// more rows take further workgroups over the same keys, and from a few hundred rows on the matrix
-// units bound it.
+// Bound by the bytes of the cache where prefixes are long and a group's rows (sequences x query heads of a key
+// head) few: a prefix's keys are read once for all rows of a tile, further tiles over the same keys meet them in
+// the L2.  8 sequences behind 100003 tokens of two key heads of 256 values: 54 us (4.0 TB/s), int8 45 us, bound by
+// the vector instructions that widen values.  Where little is read, latency bounds it: 4 candidates of a prompt of
+// 180 tokens 12.0 us, of which 2 go to finding a workgroup's unit, 3.6 to its first loads, 5 to the second launch.
 //
-// Work units are runs of 32-key blocks, of a prefix for a tile of whole sequences (NT columns of 16
-// rows), or of one sequence's own keys; every workgroup finds its unit from the lengths on the device.
-// The four waves of a workgroup take blocks in turn.  A block runs without LDS for its keys:
-//   * scores: S^T = K Q^T on 16x16x32 MFMAs, K rows straight from memory as the A operand (16
-//     keys; a lane loads 16 bytes of one key), rows as the columns of B, read from LDS;
-//   * P^T leaves the score layout as the B operand of O^T = V^T P^T without crossing lanes: lane group
-//     g holds keys 4g .. 4g+3 and 16 + 4g .. 16 + 4g+3 of the block, and V's rows are loaded in that order;
-//   * V: a lane loads 8 keys' next hd/16 values; byte permutes pair the keys of a column, once for all
-//     tiles of rows;
-//   * int8: codes become 16-bit whole numbers (exact), once for all tiles; a key's scale multiplies its
-//     scores in 32 bits, a value's its probability.
+// Work units are runs of 32-key blocks, of a prefix for a tile of whole sequences, or of one sequence's own keys;
+// lengths are on the device alone, so every workgroup makes the same plan from them and finds its unit in it.
+// Units come in two forms:
+//   * thin (run_unit): one or two tiles of 16 rows.  The four waves of a workgroup take blocks in turn, whose keys
+//     never pass through LDS:
+//     - scores: S^T = K Q^T on 16x16x32 MFMAs, K rows straight from memory as the A operand (16 keys; a lane loads
+//       16 bytes of one key), rows as the columns of B, read from LDS;
+//     - P^T leaves the score layout as the B operand of O^T = V^T P^T without crossing lanes: lane group g holds
+//       keys 4g .. 4g+3 and 16 + 4g .. 16 + 4g+3 of the block, and V's rows are loaded in that order;
+//     - V: a lane loads 8 keys' next hd/16 values; byte permutes pair the keys of a column, once for all tiles;
+//     - int8 keys stay whole numbers and meet the queries' digits (see DIGITS); values become 16-bit whole numbers
+//       (exact), a key's scale multiplies its scores in 32 bits, a value's its probability.
+//   * wide (wide_unit): 128 rows, 32 of each wave, over keys that land in LDS for all four.  64 sequences behind
+//     16384 tokens, 32 query heads of 128 values to 4 key heads: 58 us, in tiles of 32 rows 91.
 // The running maximum (the reference that P is taken against) is a column's, hence a lane's own.  P is
 // rounded to 16 bits for its product (half a step of each term; the sum of P is of the unrounded), in fp16
 // against a reference that follows the scores (fp16_reference); with int8 values P times scale goes as
 // the sum of two bf16 numbers.  Sums, maxima and O are of 32 bits.
 //
 // Each unit leaves its rows' 32-bit sums; a second launch joins a row's parts in the order of its keys,
-// the prefix's first, so that results do not depend on the order in which units end.
+// the prefix's first, so that results do not depend on the order in which units end.  (The last unit of a sequence
+// joining its parts took 12.9 us for the call of 12.0 above, and 21 instead of 12.2 behind 2000 tokens: one workgroup
+// reads for a whole tile what the second launch reads with one for each row.)
 #pragma once
 
 #include "attn_prompt_kernel.h"
@@ -199,7 +205,7 @@ __device__ __forceinline__ void opaque(u32x4& a) { asm volatile("" : "+v"(a)); }
 // int8 keys: a query is the sum of three int8 digits, q = m / 127 (d0 + d1 / 254 + d2 / 254^2) with the row's
 // largest m, off by at most half of m / 127 / 254^2 (2^-24 m, and a step of 32 bits of each product on the way).  The
 // products with codes are then whole numbers of the matrix units, added up exactly, and no code is widened (as bf16
-// numbers a block's keys took 192 vector instructions: MEASURED).
+// numbers: 54 us behind 100003 keys of 256 values, 45 so).
 constexpr int DIGITS = 3;
 
 // Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.

@@ -1,9 +1,7 @@
 // extern "C" entry points of what lies between the vocabulary head and the next token (declared in
 // include/qlin_candidates.h): checks of arguments and launch plans.
-#include <math.h>
-#include <stdlib.h>
-
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/qlin_candidates.h"
 #include "abi_check.h"
@@ -30,10 +28,9 @@ int check_rows(const char* fn, const char* name, const void* p, int es, long lon
   return QLIN_OK;
 }
 
-int check_float(const char* fn, const char* name, const void* p, int dt) {
+int check_float(const char* fn, const char* name, int dt) {
   if (dt != QLIN_F32 && dt != QLIN_BF16 && dt != QLIN_F16)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: %s of dtype %d (need bf16, fp16 or fp32)", fn, name, dt);
-  (void)p;
   return QLIN_OK;
 }
 
@@ -63,8 +60,8 @@ int qlin_logits_process(const qlin_logits* r, void* stream) {
   set_error(QLIN_OK, "");
   if (!r) return fail(QLIN_ERR_INVALID, "%s: null arguments", fn);
   QA_TRY(check_sizes(fn, r->B, r->V));
-  QA_TRY(check_float(fn, "logits", r->logits, r->dtype));
-  QA_TRY(check_float(fn, "out", r->out, r->out_dtype));
+  QA_TRY(check_float(fn, "logits", r->dtype));
+  QA_TRY(check_float(fn, "out", r->out_dtype));
   if (r->history < 0 || r->biases < 0) return fail(QLIN_ERR_INVALID, "%s: negative size", fn);
   if (r->history > kMaxTokens || r->biases > kMaxTokens)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: more than %d tokens of a row's history or biases", fn, kMaxTokens);
@@ -127,7 +124,7 @@ int qlin_sample(const void* logits, int dtype, int64_t logits_row, int B, int V,
   const char* fn = "qlin_sample";
   set_error(QLIN_OK, "");
   QA_TRY(check_sizes(fn, B, V));
-  QA_TRY(check_float(fn, "logits", logits, dtype));
+  QA_TRY(check_float(fn, "logits", dtype));
   if (top_k < 1 || top_k > kSampleMost)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: top_k %d (need 1 to %d)", fn, top_k, kSampleMost);
   QA_TRY(check_value(fn, "temperature", temperature, temperature_all, 0.0f, kAny));
@@ -163,15 +160,13 @@ int qlin_sample(const void* logits, int dtype, int64_t logits_row, int B, int V,
   // a workgroup for each tile of a row, fewer where their lists would be more than one can join or than
   // the workspace holds
   const long long tiles = ((long long)V + kSampleTile - 1) / kSampleTile, keys = sample_list(a.k), list = 8 * (keys + 1);
-  long long chunks = std::min({tiles, std::max(8LL, 1024LL / B), (long long)kSampleKeys / keys, (long long)avail / list / B, kMaxGrid / B});
-  if (const char* e = getenv("QLIN_SAMPLE_CHUNKS")) {  // for tuning runs
-    if (atoi(e) > 0) chunks = std::min(chunks, (long long)atoi(e));
-  }
+  const long long chunks = std::min({tiles, std::max(8LL, 1024LL / B), (long long)kSampleKeys / keys,
+                                     (long long)avail / list / B, kMaxGrid / B});
   if (chunks < 1) return fail(QLIN_ERR_WORKSPACE, "%s: workspace too small for %d rows", fn, B);
   a.chunks = (int)chunks;
   a.keys = (uint64_t*)part;
   a.stats = (uint64_t*)part + (long long)B * chunks * keys;
-  a.cnt = (unsigned*)workspace;
+  a.cnt = (unsigned*)workspace;  // (kMaxRows of them are a quarter of the counters there are)
   return status(fn, launch_sample(a, (hipStream_t)stream));
 }
 

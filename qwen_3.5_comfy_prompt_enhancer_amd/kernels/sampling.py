@@ -28,7 +28,7 @@ import struct
 import torch
 
 from . import qlin as C
-from .attention import _call, _size, _vector
+from .attention import _INT_MAX, _call, _size, _vector
 from .attention import _SIGS as _ALL
 
 __all__ = ["logits_process", "sample"]
@@ -65,14 +65,24 @@ def _rows(name, t, B=None, n=None, dtypes=None):
 
 
 def _logit_rows(name, t):
-    dt = _FLOATS.get(t.dtype)
+    """Type code, row stride, rows and tokens."""
+    dt, shape = _FLOATS.get(t.dtype), t.shape
     if dt is None:
         raise ValueError(f"{name} must be bfloat16, float16 or float32")
-    return dt, _rows(name, t)
+    if len(shape) != 2:
+        raise ValueError(f"{name} must be [rows, tokens], not {list(shape)}")
+    st = t.stride()
+    if shape[1] > 1 and st[1] != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous")
+    if shape[0] > _INT_MAX or shape[1] > _INT_MAX:
+        _size(f"rows and tokens of {name}", max(shape))
+    return dt, st[0], shape[0], shape[1]
 
 
 def _value(name, x, B):
     """(address, number) of a float or a float32 tensor [B]."""
+    if type(x) is float:
+        return 0, x
     if isinstance(x, torch.Tensor):
         _vector(name, x, B, (torch.float32,))
         return x.data_ptr(), 0.0
@@ -80,7 +90,7 @@ def _value(name, x, B):
 
 
 def _tensor(x):
-    return x if isinstance(x, torch.Tensor) else None
+    return None if type(x) is float or not isinstance(x, torch.Tensor) else x
 
 
 def logits_process(logits, out, tokens=None, lens=None, prompt_lens=None, repetition=1.0, presence=0.0, frequency=0.0,
@@ -97,13 +107,11 @@ def logits_process(logits, out, tokens=None, lens=None, prompt_lens=None, repeti
     [B, (V + 31) // 32] (token i is bit i % 32 of word i // 32) or bool [B, V]; others become -inf.
     An expanded row (stride 0) is one for all.  Ids outside the vocabulary, as padding
     has, count for nothing.  Returns out."""
-    xdt, xs = _logit_rows("logits", logits)
-    B, V = logits.shape
+    xdt, xs, B, V = _logit_rows("logits", logits)
     odt = _FLOATS.get(out.dtype)
     if odt is None:
         raise ValueError("out must be bfloat16, float16 or float32")
     os = _rows("out", out, B, V)
-    _size("rows and tokens of logits", max(B, V))
     rep, pres, freq = (_value(n, x, B) for n, x in (("repetition", repetition), ("presence", presence),
                                                     ("frequency", frequency)))
     tp = ts = t64 = L = lp = pp = 0
@@ -151,9 +159,7 @@ def sample(logits, u, tokens, logprobs=None, temperature=1.0, top_k=20, top_p=1.
     the token's log probability among all of the row's logits, as they are (at temperature 1).
     Logits of -inf and NaN are never drawn; a row of nothing else gives -1 (and -inf).  Returns
     tokens."""
-    xdt, xs = _logit_rows("logits", logits)
-    B, V = logits.shape
-    _size("rows and tokens of logits", max(B, V))
+    xdt, xs, B, V = _logit_rows("logits", logits)
     _vector("u", u, B, (torch.float32,))
     _vector("tokens", tokens, B, _INTS)
     lp = 0
