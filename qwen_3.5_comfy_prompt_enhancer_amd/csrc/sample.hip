@@ -7,12 +7,12 @@
 //   log p = (x - max) - log sum_j exp(x_j - max) over the row
 //
 // Bound by HBM for many rows, by latency for few: a row is read once, by several workgroups, each of which takes
-// a part of it, 32 logits of a thread at a time, for the maximum and the sum of exponentials of each thread.  The k-th
+// a part of it, 32 or 64 logits of a thread, for the maximum and the sum of exponentials of each thread.  The k-th
 // largest of its 256 threads' maxima (to 20 bits, rounded down) is a bound that the part's k largest do not fall
-// below, and in practice little more than k logits reach; the threads whose maximum does look for them again (in
-// the cache) and leave them in LDS.  64 rows of 248320 fp32 logits take 29 us for k = 50 (2.2 TB/s; the sum of
-// exponentials, the search and the join each wait for the one before), one row 13 us.  (Lists kept in registers as
-// tiles come took 104 and 27.)  Where many of equal value reach it (a mask of the type's lowest value), the
+// below, and in practice little more than k logits reach; the threads whose maximum does leave theirs in LDS, from
+// their registers (longer parts are read again; for all parts that took 29 us where this takes 25).  64 rows of 248320
+// fp32 logits take 25 us for k = 50 (2.5 TB/s; 8 us of a workgroup's time go to reading and summing, 5 to the search, 7
+// of the row's last one to the join), one row 11.4.  (Lists kept in registers as tiles come took 104 and 27.)  Where many of equal value reach it (a mask of the type's lowest value), the
 // bound goes on with their index.  The last workgroup of a row to arrive does the same with all parts' candidates,
 // puts what reaches the bound in order by counting, for each, the larger ones, and draws.  Weights and their sums are
 // of 64 bits (k numbers: a draw next to a border then falls as the formula says), the row's sum of exponentials of 32.
@@ -80,26 +80,29 @@ __device__ __forceinline__ void share_tops(Lds& L, uint32_t mine, uint32_t (&o)[
   for (int e = 0; e < 4; ++e) o[e] = L.top[(tid & 63) + 64 * e];
 }
 
+__device__ __forceinline__ void add(Lds& L, uint64_t key, uint64_t low) {
+  if (key < low) return;
+  const int at = atomicAdd(&L.n, 1);
+  if (at < kCandidates) L.cand[at] = key;
+}
+
 // The k largest of a workgroup's keys (order, ~index), which differ, and maybe a few more, to L.cand: how many.
-// top: the largest order of this thread's keys; scan(f) calls f(key) for each of them (0: none).
-template <typename Scan>
-__device__ __forceinline__ int gather(Lds& L, int k, uint32_t top, Scan scan) {
+// top: the largest order of this thread's keys; scan(f) calls f(key) for each of them (0: none); quick(order) adds
+// those from that order on to L.cand.
+template <typename Quick, typename Scan>
+__device__ __forceinline__ int gather(Lds& L, int k, uint32_t top, Quick quick, Scan scan) {
   const int tid = (int)threadIdx.x;
   uint32_t o[4];
   share_tops(L, top, o);
   const uint32_t rough = max(bound_of(o, k, 0x1000u), kLowest);
   auto collect = [&](uint64_t low, bool some) {
-    if (some)
-      scan([&](uint64_t key) {
-        if (key >= low) {
-          const int at = atomicAdd(&L.n, 1);
-          if (at < kCandidates) L.cand[at] = key;
-        }
-      });
+    if (some) scan([&](uint64_t key) { add(L, key, low); });
     __syncthreads();
     return L.n;
   };
-  int n = collect((uint64_t)rough << 32, top >= rough);
+  if (top >= rough) quick(rough);
+  __syncthreads();
+  int n = L.n;
   if (n <= kCandidates) return n;
   // Many of (nearly) equal value: the k-th largest of the threads' largest keys, order and index.
   uint64_t most = 0ull;
@@ -207,10 +210,11 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Lds& L, int b, f
   }
 }
 
-// SHORT: rows of up to 2048 logits, which come one by one, so that all threads have some; else runs of eight.
-template <int DT, bool SHORT>
-__global__ __launch_bounds__(kThreads, 6) void sample_kernel(const SampleArgs a) {
-  constexpr int IT = SHORT ? 1 : kSampleTile / kThreads / 8, N = IT * 8;
+// SHORT: rows of up to 2048 logits, which come one by one, so that all threads have some; else IT runs of eight of a
+// thread at a time.
+template <int DT, bool SHORT, int IT>
+__global__ __launch_bounds__(kThreads, IT > 4 ? 4 : 6) void sample_kernel(const SampleArgs a) {
+  constexpr int N = IT * 8;
   __shared__ Lds L;
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int b = (int)blockIdx.x / a.chunks, chunk = (int)blockIdx.x - b * a.chunks;
@@ -251,9 +255,9 @@ __global__ __launch_bounds__(kThreads, 6) void sample_kernel(const SampleArgs a)
     }
   };
   constexpr int STEP = N * kThreads;
-  float m = -kInf, s = 0.0f;
+  float m = -kInf, s = 0.0f, v[N];
   for (int i0 = 0; i0 < n; i0 += STEP) {
-    float v[N], top = m;
+    float top = m;
     some(i0, [&](int e, float y, int) {
       v[e] = fmaxf(y, -kInf);  // (no number as -inf)
       top = fmaxf(top, v[e]);
@@ -271,13 +275,33 @@ __global__ __launch_bounds__(kThreads, 6) void sample_kernel(const SampleArgs a)
     }
     m = top;
   }
-  int have = gather(L, a.k, order_of(m), [&](auto f) {
+  auto scan = [&](auto f) {
     for (int i0 = 0; i0 < n; i0 += STEP)
       some(i0, [&](int, float y, int i) {
         const uint32_t o = order_of(fmaxf(y, -kInf));
         f(o ? (uint64_t)o << 32 | (uint32_t)~(v0 + i) : 0ull);
       });
-  });
+  };
+  // (a part of one step is still in registers: counted first, so that a thread takes its places at once)
+  auto quick = [&](uint32_t from) {
+    if (n > STEP) {
+      scan([&](uint64_t key) { add(L, key, (uint64_t)from << 32); });
+      return;
+    }
+    const float low = value_of(from);
+    int c = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) c += v[e] >= low;
+    int at = atomicAdd(&L.n, c);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (v[e] >= low) {
+        const int i = SHORT ? e * kThreads + tid : (e / 8 * kThreads + tid) * 8 + e % 8;
+        if (at < kCandidates) L.cand[at] = (uint64_t)order_of(v[e]) << 32 | (uint32_t)~(v0 + i);
+        ++at;
+      }
+  };
+  int have = gather(L, a.k, order_of(m), quick, scan);
   // the row's maximum and sum
   auto join_all = [&]() {
     const float M = wave_max(m);
@@ -331,29 +355,28 @@ __global__ __launch_bounds__(kThreads, 6) void sample_kernel(const SampleArgs a)
   }
   __syncthreads();
   if (!L.last) return;
-  // all candidates: eight of a thread are kept at hand
+  // all candidates, in registers: up to 24 of a thread
+  constexpr int RUN = 8, RUNS = kSampleKeys / kThreads / RUN;
+  static_assert(RUNS * RUN * kThreads == kSampleKeys, "a row's keys");
   const int all = a.chunks * cap;
-  uint64_t key[8];
-  auto load = [&](int i0) __attribute__((always_inline)) {
+  uint64_t key[RUNS][RUN];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      key[e] = __hip_atomic_load(keys + min(i0 + e * kThreads, all - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int r = 0; r < RUNS; ++r) {
+    if (r * RUN * kThreads >= all) break;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) key[e] = i0 + e * kThreads < all ? key[e] : 0ull;
-  };
-  load(tid);
-  auto scan = [&](auto f) {
-    for (int i0 = tid;;) {
+    for (int e = 0; e < RUN; ++e)
+      key[r][e] = __hip_atomic_load(keys + min((r * RUN + e) * kThreads + tid, all - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  auto all_keys = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f(key[e]);
-      if (all <= 8 * kThreads) break;
-      i0 = i0 + 8 * kThreads < all ? i0 + 8 * kThreads : tid;
-      load(i0);
-      if (i0 == tid) break;
+    for (int r = 0; r < RUNS; ++r) {
+      if (r * RUN * kThreads >= all) break;
+#pragma unroll
+      for (int e = 0; e < RUN; ++e) f((r * RUN + e) * kThreads + tid < all ? key[r][e] : 0ull);
     }
   };
   uint32_t top = 0u;
-  scan([&](uint64_t key) { top = max(top, (uint32_t)(key >> 32)); });
+  all_keys([&](uint64_t key) { top = max(top, (uint32_t)(key >> 32)); });
   m = -kInf, s = 0.0f;
   for (int i = tid; i < a.chunks; i += kThreads) {
     const uint64_t v = __hip_atomic_load(stats + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -362,7 +385,8 @@ __global__ __launch_bounds__(kThreads, 6) void sample_kernel(const SampleArgs a)
     m = mn;
   }
   join_all();
-  const int found = gather(L, a.k, top, scan);
+  auto reach = [&](uint32_t from) { all_keys([&](uint64_t key) { add(L, key, (uint64_t)from << 32); }); };
+  const int found = gather(L, a.k, top, reach, all_keys);
   sort_list(L, found, a.k);
   if (wave == 0) draw(a, L, b, m, s, temp, top_p, min_p, u);
 }
@@ -372,8 +396,9 @@ __global__ __launch_bounds__(kThreads, 6) void sample_kernel(const SampleArgs a)
 template <int DT>
 static void launch(const SampleArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(a.B * a.chunks)), block(kThreads);
-  if (a.V <= 8 * kThreads) hipLaunchKernelGGL((sample_kernel<DT, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((sample_kernel<DT, false>), grid, block, 0, st, a);
+  if (a.V <= 8 * kThreads) hipLaunchKernelGGL((sample_kernel<DT, true, 1>), grid, block, 0, st, a);
+  else if (a.V <= (long long)kSampleTile * a.chunks) hipLaunchKernelGGL((sample_kernel<DT, false, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((sample_kernel<DT, false, 8>), grid, block, 0, st, a);
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {

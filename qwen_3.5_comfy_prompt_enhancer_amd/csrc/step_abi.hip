@@ -157,11 +157,14 @@ int qlin_sample(const void* logits, int dtype, int64_t logits_row, int B, int V,
   a.top_p = RowValue{top_p, top_p_all};
   a.min_p = RowValue{min_p, min_p_all};
   a.tokens = tokens, a.tokens64 = tokens_64, a.logp = logprobs;
-  // a workgroup for each tile of a row, fewer where their lists would be more than one can join or than
-  // the workspace holds
-  const long long tiles = ((long long)V + kSampleTile - 1) / kSampleTile, keys = sample_list(a.k), list = 8 * (keys + 1);
-  const long long chunks = std::min({tiles, std::max(8LL, 1024LL / B), (long long)kSampleKeys / keys,
-                                     (long long)avail / list / B, kMaxGrid / B});
+  // A workgroup for each part of a row that a workgroup keeps in registers, fewer where their lists would be more than
+  // one can join or than the workspace holds.  Long parts where they fill the chip: fewer lists, and all workgroups at
+  // once (248320 fp32 logits, parts of 8192 / 16384: one row 11.4 / 13, 16 rows 20.2 / 18.9 us, 64 33.7 / 26.4; 64 rows of
+  // 100003 19.0 / 19.4, 8 13.4 / 15.1).
+  const long long tiles = ((long long)V + kSampleTile - 1) / kSampleTile, half = (tiles + 1) / 2;
+  const long long keys = sample_list(a.k), list = 8 * (keys + 1);
+  const long long parts = half > 8 && half * B >= 256 ? half : tiles;
+  const long long chunks = std::min({parts, (long long)kSampleKeys / keys, (long long)avail / list / B, kMaxGrid / B});
   if (chunks < 1) return fail(QLIN_ERR_WORKSPACE, "%s: workspace too small for %d rows", fn, B);
   a.chunks = (int)chunks;
   a.keys = (uint64_t*)part;

@@ -57,7 +57,7 @@ struct SampleArgs {
   uint64_t* stats;        // [B][chunks] maximum and sum
   unsigned* cnt;          // arrivals of each row, zero between calls
 };
-constexpr int kSampleTile = 8192;   // logits that a workgroup looks at in one go
+constexpr int kSampleTile = 8192;   // logits that a workgroup keeps in registers (or twice as many)
 constexpr int kSampleMost = 128;    // largest k
 constexpr int kSampleKeys = 6144;   // keys of a row's chunks at most
 // keys that a chunk leaves room for

@@ -73,7 +73,8 @@ def test_shared_overlaps(tmp):
 
 @pytest.mark.parametrize("B,V,k,chunks", [(1, 1, 1, 1), (1, 8192, 20, 1), (1, 8193, 20, 2), (1, 248320, 20, 31), (64, 248320, 50, 16),
                                           (1, 248320, 128, 31), (1, 1 << 30, 128, 31), (4096, 50021, 128, 7),
-                                          (1 << 16, 8193, 128, 2), (1 << 16, 1 << 20, 1, 8)])
+                                          (1 << 16, 8193, 128, 2), (1 << 16, 1 << 20, 1, 64),
+                                          (8, 248320, 50, 31), (17, 248320, 50, 16), (256, 131072, 20, 16)])
 def test_sample_grids(tmp, B, V, k, chunks):
     (name, grid), = _run(tmp, sample(B, V, k), 1)
     assert "sample_kernel" in name and grid == B * chunks < 1 << 24

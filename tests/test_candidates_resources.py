@@ -6,7 +6,7 @@ from test_kernel_resources import _find
 
 
 @pytest.mark.parametrize("kernel,forms", [("13shared_kernelI", 30), ("18shared_join_kernelI", 16), ("13logits_kernelI", 45),
-                                          ("13sample_kernelI", 6)])
+                                          ("13sample_kernelI", 9)])
 def test_values_stay_in_registers(kernel, forms):
     """No vector register is spilled and no array lies in scratch."""
     found = _find(kernel)

@@ -232,3 +232,11 @@ def test_most_in_few_threads():
     for k in (50, 128):
         for u in (0.001, 0.77, 0.9999):
             check(x, torch.full((3,), u), top_k=k, temperature=20.0)
+
+
+@pytest.mark.parametrize("dt", [BF, F16, F32])
+@pytest.mark.parametrize("B,V,k", [(16, 262145, 128), (24, 248320, 40), (40, 131073, 5), (20, 300001, 100)])
+def test_long_parts(B, V, k, dt):
+    """Many rows of long vocabularies: parts of up to 16384 logits, or longer ones that are read twice."""
+    x, u = rows(B, V, B + k, dt)
+    check(x, u, top_k=k, temperature=0.9, top_p=0.95)
