@@ -12,10 +12,11 @@
 // below, and in practice little more than k logits reach; the threads whose maximum does leave theirs in LDS, from
 // their registers (longer parts are read again; for all parts that took 29 us where this takes 25).  64 rows of 248320
 // fp32 logits take 25 us for k = 50 (2.5 TB/s; 8 us of a workgroup's time go to reading and summing, 5 to the search, 7
-// of the row's last one to the join), one row 11.4.  (Lists kept in registers as tiles come took 104 and 27.)  Where many of equal value reach it (a mask of the type's lowest value), the
-// bound goes on with their index.  The last workgroup of a row to arrive does the same with all parts' candidates,
-// puts what reaches the bound in order by counting, for each, the larger ones, and draws.  Weights and their sums are
-// of 64 bits (k numbers: a draw next to a border then falls as the formula says), the row's sum of exponentials of 32.
+// of the row's last one to the join), one row 11.4.  (Lists kept in registers as tiles come took 104 and 27.)  Where
+// many of equal value reach it (a mask of the type's lowest value), the bound goes on with their index.  The last
+// workgroup of a row to arrive does the same with all parts' candidates, puts what reaches the bound in order by
+// counting, for each, the larger ones, and draws.  Weights and their sums are of 64 bits (k numbers: a draw next to a
+// border then falls as the formula says), the row's sum of exponentials of 32.
 #include "attn_dev.h"
 #include "step_dev.h"
 

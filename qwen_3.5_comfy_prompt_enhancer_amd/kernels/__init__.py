@@ -5,6 +5,7 @@ activation producers of its kernels/norm.py; `fused` runs a producer and a linea
 one call; `linear` holds the A16 (fp16-activation) weight-only core; `chain` whole
 decode steps in one launch; `layout` the unpack / dequant checks and load-time
 layout producers; `attention` an attention layer's steps between its projections and its
-output projection, over a paged cache; `qlin` loads libqlin.so; `common` holds GROUP.
+output projection, over a paged cache; `sampling` penalties, masks and draws on the
+vocabulary head's rows; `qlin` loads libqlin.so; `common` holds GROUP.
 """
 from .common import GROUP  # noqa: F401
