@@ -14,7 +14,7 @@
 // that fall into its run, a word for each token: how often it came behind the prompt (bits 0 .. 18), the last
 // place among the biases (19 .. 30) and whether the prompt holds it (31); two words where histories or biases
 // are too long for that.  Each run reads the whole history, so many rows (and long histories) take longer
-// runs in larger workgroups: 64 rows of 248320 16-bit logits to 32 bits with histories of 8192 tokens 33 us, without
+// runs in larger workgroups: 64 rows of 248320 16-bit logits to 32 bits with histories of 8192 tokens 32 us, without
 // any 22 (4.3 TB/s).  Larger runs yet (16384, 1024 threads: 37) leave a CU two workgroups that wait for each other's barriers.
 #include "attn_dev.h"
 #include "step_dev.h"
@@ -28,6 +28,10 @@ constexpr int kPlace = 19;
 constexpr long long kManyLogits = 3 << 20;
 constexpr int kLongHistory = 2048;
 constexpr uint32_t kPlaces = 0xFFFu;
+
+// A token's word: a thread looks at eight words by 16-byte reads; in plain order a read of threads 8 .. 15 meets
+// one of 0 .. 7 in the same banks (3.5 M cycles of conflicts in the 32 us above, 0.01 M so; the call 1.2 us less).
+__device__ __forceinline__ uint32_t word_of(uint32_t i) { return i ^ (i >> 4 & 4u); }
 
 // WORDS: of LDS for a token: 1 (all in one), 2 (a count, and a place), or 0 (no history, no biases).
 template <int XDT, int ODT, int WORDS, int THREADS, int IT>
@@ -96,8 +100,8 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
       for (int e = 0; e < N; ++e) {
         const int i = i0 + e * THREADS;
         if (i >= len || id[e] >= (uint32_t)n) continue;
-        if (i < prompt) atomicOr(lds + id[e], kInPrompt);
-        else atomicAdd(lds + id[e], 1u);
+        if (i < prompt) atomicOr(lds + word_of(id[e]), kInPrompt);
+        else atomicAdd(lds + word_of(id[e]), 1u);
       }
       i0 += THREADS * N;
       if (i0 < len) load(i0);
@@ -106,11 +110,12 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
       if (bid < (uint32_t)n) {
         const uint32_t mine = (uint32_t)i + 1u;
         if constexpr (WORDS == 2) {
-          atomicMax(lds + RUN + bid, mine);
+          atomicMax(lds + RUN + word_of(bid), mine);
         } else {
-          uint32_t old = lds[bid];
+          uint32_t* word = lds + word_of(bid);
+          uint32_t old = *word;
           while ((old >> kPlace & kPlaces) < mine) {
-            const uint32_t was = atomicCAS(lds + bid, old, (old & ~(kPlaces << kPlace)) | mine << kPlace);
+            const uint32_t was = atomicCAS(word, old, (old & ~(kPlaces << kPlace)) | mine << kPlace);
             if (was == old) break;
             old = was;
           }
@@ -136,9 +141,9 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
     if (at) y = y + a.bias[b * a.bs + (at - 1u)];
     return y;
   };
-  auto value = [&](float y, int i, bool ok) {
-    if constexpr (WORDS == 1) y = adjusted(y, lds[i], lds[i] >> kPlace & kPlaces);
-    if constexpr (WORDS == 2) y = adjusted(y, lds[i], lds[RUN + i]);
+  auto value = [&](float y, uint32_t w, uint32_t at, bool ok) {
+    if constexpr (WORDS == 1) y = adjusted(y, w, w >> kPlace & kPlaces);
+    if constexpr (WORDS == 2) y = adjusted(y, w, at);
     return ok ? y : -__builtin_inff();
   };
 #pragma unroll
@@ -147,16 +152,24 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const LogitsArgs a) {
     if (i >= n) continue;
     if (i + 8 <= n) {
       float y[8];
+      u32x4 w[2] = {}, at[2] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t from = word_of((uint32_t)i + 4u * h);
+        if constexpr (WORDS > 0) w[h] = *(const u32x4*)(lds + from);
+        if constexpr (WORDS == 2) at[h] = *(const u32x4*)(lds + RUN + from);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool ok = !mask || (a.mask_bytes ? (allowed[it] >> (8 * e)) & 0xFFu : (allowed[it] >> e) & 1u);
-        y[e] = value(r[it].get(e), i + e, ok);
+        y[e] = value(r[it].get(e), w[e / 4][e % 4], at[e / 4][e % 4], ok);
       }
       store8<ODT>(o, i, y);
     } else {
       for (int e = 0; i + e < n; ++e) {
         const bool ok = !mask || (a.mask_bytes ? mask[i + e] != 0 : mask[i / 8] >> e & 1);
-        store1<ODT>(o, i + e, value(load1<XDT>(x, i + e), i + e, ok));
+        const uint32_t from = word_of((uint32_t)(i + e));
+        store1<ODT>(o, i + e, value(load1<XDT>(x, i + e), WORDS > 0 ? lds[from] : 0u, WORDS == 2 ? lds[RUN + from] : 0u, ok));
       }
     }
   }
