@@ -47,7 +47,7 @@ def test_forms(tmp, B, hq, hkv, hd, i8, ppages, form, dt):
     and more than 16 query heads to a key head, the wide form."""
     kv = D.cache(hkv, hd, pages=4096, dtype=D.I8 if i8 else dt)
     got = _run(tmp, shared(kv, B, 1, hq, hkv, hd, ppages, dt=dt), 2)
-    assert f"13shared_kernelI" in got[0][0] and f"Li{hd}ELb{i8}ELi{form}E" in got[0][0], got
+    assert "13shared_kernelI" in got[0][0] and f"Li{hd}ELb{i8}ELi{form}E" in got[0][0], got
     assert "shared_join" in got[1][0]
 
 
