@@ -80,11 +80,12 @@ int qlin_logits_process(const qlin_logits* args, void* stream);
  * 0 <= u < 1.  Of the row's top_k (1 .. 128) largest logits x_0 >= x_1 >= ..., equal ones by their index, with
  * weights w_i = exp((x_i - x_0) / temperature), those are kept that have less than top_p of the weights' sum
  * in front of them and weigh at least min_p (x_0 always), and the first is drawn with which the sum of the
- * kept exceeds u times theirs.  Temperature 0: the largest (a vector's negative numbers count as 0).  Sums and
- * weights are of 64 bits.  logprobs [B] (or NULL): x - log sum exp of the row's logits, at the token.
+ * kept exceeds u times theirs.  Temperature 0: the largest, of equal ones the lowest index, whatever u is (a
+ * vector's negative numbers and NaN count as 0).  Sums and weights are of 64 bits.  logprobs [B] (or NULL):
+ * x - log sum exp of the row's logits, at the token.
  * A logit of -inf or NaN is never drawn and has no part in a sum; a row of nothing else gives token -1 and -inf.
- * Infinite logits share the row among themselves.  A number of each row is a vector [B], or NULL and one
- * number for all.  What the call writes shares no byte with what it reads. */
+ * Infinite logits share the row among themselves, at temperature 0 too.  A number of each row is a vector [B],
+ * or NULL and one number for all.  What the call writes shares no byte with what it reads. */
 int qlin_sample(const void* logits, int dtype, int64_t logits_row, int B, int V, int top_k, const float* u,
                 const float* temperature, float temperature_all, const float* top_p, float top_p_all,
                 const float* min_p, float min_p_all, void* tokens, int tokens_64, float* logprobs,

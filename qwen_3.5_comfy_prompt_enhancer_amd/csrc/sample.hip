@@ -3,7 +3,7 @@
 //
 //   x_0 >= x_1 >= ... the row's k largest (of equal ones the lowest index first)
 //   w_i = exp((x_i - x_0) / T), kept while w_0 + ... + w_{i-1} < top_p (w_0 + ... + w_{k-1}) and w_i >= min_p
-//   token: the first i with w_0 + ... + w_i > u (sum of the kept)
+//   token: the first i with w_0 + ... + w_i > u (sum of the kept); of T = 0 the first
 //   log p = (x - max) - log sum_j exp(x_j - max) over the row
 //
 // Bound by HBM for many rows, by latency for few: a row is read once, by several workgroups, each of which takes
@@ -197,7 +197,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Lds& L, int b, f
   auto first = [](uint64_t even, uint64_t odd) {
     return min(even ? 2 * __builtin_ctzll(even) : 128, odd ? 2 * __builtin_ctzll(odd) + 1 : 128);
   };
-  const int n = max(1, first(cut0, cut1));
+  // (temperature 0: the first alone, as its equals weigh 1 too; infinite ones share the row at any temperature)
+  const int n = T == 0.0 && x0 < (double)kInf ? 1 : max(1, first(cut0, cut1));
   const double goal = (double)u * (n % 2 ? lane64(mid, (n - 1) / 2) : lane64(c1, (n - 1) / 2));
   const int at = min(first(__ballot(mid > goal), __ballot(c1 > goal)), n - 1);
   if (lane) return;

@@ -155,10 +155,10 @@ def sample(logits, u, tokens, logprobs=None, temperature=1.0, top_k=20, top_p=1.
     Of the row's top_k largest logits (1 to 128; equal ones by their index) with the weights
     exp((x - max) / temperature), those are kept that have less than top_p of the weights' sum in
     front of them and weigh at least min_p of the largest; the first is drawn with which the sum of
-    the kept exceeds u times theirs.  temperature 0 takes the largest.  logprobs (float32 [B]):
-    the token's log probability among all of the row's logits, as they are (at temperature 1).
-    Logits of -inf and NaN are never drawn; a row of nothing else gives -1 (and -inf).  Returns
-    tokens."""
+    the kept exceeds u times theirs.  temperature 0 takes the largest, of equal ones the lowest index,
+    whatever u is (only infinite logits share the row there too).  logprobs (float32 [B]): the
+    token's log probability among all of the row's logits, as they are (at temperature 1).  Logits of
+    -inf and NaN are never drawn; a row of nothing else gives -1 (and -inf).  Returns tokens."""
     xdt, xs, B, V = _logit_rows("logits", logits)
     _vector("u", u, B, (torch.float32,))
     _vector("tokens", tokens, B, _INTS)
