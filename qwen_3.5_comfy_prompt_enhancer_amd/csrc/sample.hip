@@ -186,7 +186,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Lds& L, int b, f
     const uint64_t key = i < a.k ? L.list[i] : 0ull;
     const double x = (double)value_of((uint32_t)(key >> 32));
     there[e] = key != 0ull;
-    w[e] = !key ? 0.0 : x == x0 ? 1.0 : exp((x - x0) / T);
+    // (beside an infinite one nothing weighs: in front of the quotient, which is no number where T is infinite too)
+    w[e] = !key ? 0.0 : x == x0 ? 1.0 : x0 == (double)kInf ? 0.0 : exp((x - x0) / T);
   }
   const double c1 = scan64(w[0] + w[1]);
   const double prev = __shfl_up(c1, 1, 64), from = lane ? prev : 0.0, mid = from + w[0];

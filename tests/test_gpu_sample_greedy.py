@@ -65,3 +65,16 @@ def test_log_probability_of_a_tie():
     for u in U:
         tok, lp = run(x, u, temperature=0.0)
         assert int(tok) == 77 and abs(float(lp) + math.log(2)) <= 2.0 ** -23
+
+
+def test_infinite_temperature():
+    """Infinitely hot rows: all of the k largest weigh the same; where some are infinite only those do, as at any
+    temperature."""
+    x = -torch.arange(9000.0)[None].repeat(4, 1)
+    x[1, [70, 8500]] = math.inf
+    x[2, [3, 4, 8999]] = math.inf
+    x[3, 1:] = -math.inf
+    t = torch.full((4,), math.inf, device="cuda")
+    for u, want in ((0.0, [0, 70, 3, 0]), (0.3, [3, 70, 3, 0]), (0.6, [6, 8500, 4, 0]), (0.99, [9, 8500, 8999, 0])):
+        tok, _ = run(x, u, top_k=10, temperature=t)
+        assert tok.tolist() == want, (u, tok.tolist())
