@@ -85,7 +85,7 @@ def _value(name, x, B):
         return 0, x
     if isinstance(x, torch.Tensor):
         _vector(name, x, B, (torch.float32,))
-        return x.data_ptr(), 0.0
+        return x.data_ptr(), 1.0  # (a vector of no rows has no address: the number, one that all arguments may be, is checked)
     return 0, float(x)
 
 
@@ -142,8 +142,7 @@ def logits_process(logits, out, tokens=None, lens=None, prompt_lens=None, repeti
                    bias_ids, bias, mask)
     dev = out.get_device()
     args = _LOGITS.pack(logits.data_ptr(), xs, out.data_ptr(), os, tp, ts, lp, pp, rep[0], pres[0], freq[0], ip, ist, bp,
-                        bst, mp, mst, t64, by_bytes, B, V, L, nb, xdt, odt, rep[1] if not rep[0] else 1.0, pres[1],
-                        freq[1])
+                        bst, mp, mst, t64, by_bytes, B, V, L, nb, xdt, odt, rep[1], pres[1], freq[1])
     _call("qlin_logits_process", dev, args, C.current_stream(dev))
     return out
 
