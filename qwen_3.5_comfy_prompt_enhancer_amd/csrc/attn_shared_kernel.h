@@ -20,7 +20,7 @@
 //     - P^T leaves the score layout as the B operand of O^T = V^T P^T without crossing lanes: lane group g holds
 //       keys 4g .. 4g+3 and 16 + 4g .. 16 + 4g+3 of the block, and V's rows are loaded in that order;
 //     - V: a lane loads 8 keys' next hd/16 values; byte permutes pair the keys of a column, once for all tiles;
-//     - int8 keys stay whole numbers and meet the queries' digits (see DIGITS); values become 16-bit whole numbers
+//     - int8 keys stay whole numbers and meet the queries' digits where those hold them (see DIGITS); values become 16-bit whole numbers
 //       (exact), a key's scale multiplies its scores in 32 bits, a value's its probability.
 //   * wide (wide_unit): 128 rows, 32 of each wave, over keys that land in LDS for all four.  64 sequences behind
 //     16384 tokens, 32 query heads of 128 values to 4 key heads: 58 us, in tiles of 32 rows 91.
@@ -202,11 +202,16 @@ __device__ __forceinline__ void opaque(uint32_t& a) { asm volatile("" : "+v"(a))
 __device__ __forceinline__ void opaque(u32x2& a) { asm volatile("" : "+v"(a)); }
 __device__ __forceinline__ void opaque(u32x4& a) { asm volatile("" : "+v"(a)); }
 
-// int8 keys: a query is the sum of three int8 digits, q = m / 127 (d0 + d1 / 254 + d2 / 254^2) with the row's
-// largest m, off by at most half of m / 127 / 254^2 (2^-24 m, and a step of 32 bits of each product on the way).  The
-// products with codes are then whole numbers of the matrix units, added up exactly, and no code is widened (as bf16
-// numbers: 54 us behind 100003 keys of 256 values, 45 so).
+// int8 keys: a query is the sum of three int8 digits, q = 2^(E - 5) (d0 + d1 / 2^8 + d2 / 2^16) where the row's largest
+// value lies from 2^E to 2^(E + 1).  The products with codes are then whole numbers of the matrix units, added up
+// exactly, and no code is widened (8 sequences behind 100003 keys of 256 values: 41.4 us, as 16-bit numbers 44.8).
+// That holds a bf16 value exactly down to 2^(E - 14), an fp16 one to 2^(E - 11), where most rows have nothing or little
+// below; of smaller values it leaves out up to half of 2^(E - 21).  What a row's digits leave out, summed over its
+// values, times the largest code and a key's scale, bounds how far off a score is.  A block where a key's score could be
+// off by more than 2^-16 (in powers of two: as much as P loses as two bf16 numbers) takes its codes as 16-bit numbers and
+// the queries as they are: rows of very different values, whose large ones may meet codes of zero.
 constexpr int DIGITS = 3;
+constexpr float kLeftOut = 0x1p-16f;
 
 // Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
 template <typename T>
@@ -219,10 +224,11 @@ __device__ __forceinline__ long long part_row(const SharedArgs& a, const Unit& U
   return (long long)hk * a.rows + (U.prefix ? (long long)U.slot * (a.spt * a.R) : a.own_rows + (long long)U.slot * a.R);
 }
 
-// Dynamic LDS: the queries of NT tiles as operands; behind the loop the waves' sums of a tile.
+// Dynamic LDS: the queries of NT tiles as operands (int8 keys: digits, and as they are); behind the loop the waves' sums of
+// a tile.
 template <int HD>
 constexpr int shared_lds(int nt, bool q8) {
-  const int q = nt * (q8 ? DIGITS * (HD / 64) : HD / 32) * 1024 + nt * 64 + kWaves * 256, join = kWaves * 16 * (HD + 4) * 4 + kWaves * 128;
+  const int q = nt * ((q8 ? DIGITS * (HD / 64) : 0) + HD / 32) * 1024 + nt * 128 + kWaves * 256, join = kWaves * 16 * (HD + 4) * 4 + kWaves * 128;
   return q > join ? q : join;
 }
 
@@ -258,7 +264,6 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
     if (some && row < rows)
       qr[i] = ld_global<u32x4>((const uint16_t*)a.q + (U.b0 + seq) * a.qb + (hk * a.R + (row - seq * a.R)) * a.qh + d);
   }
-  const f32x4* lq = (const f32x4*)lds + lane;
   f32x4 O[NT][VC * VW];
   float m[NT], l[NT];
 #pragma unroll
@@ -340,18 +345,19 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
     pages(blk + kWaves, pin);
   }
   __builtin_amdgcn_sched_barrier(0);
-  constexpr int QF = Q8 ? NT * DIGITS * KL * 256 : NT * STEPS * 256;  // floats of the operands
-  float qscale[NT];
-  if constexpr (!Q8) {
-    // step s of tile t at ((t STEPS + s) 64 + lane) 16 bytes
+  constexpr int DF = Q8 ? NT * DIGITS * KL * 256 : 0;  // floats of the digits,
+  constexpr int QF = DF + NT * STEPS * 256;            // and of the operands
+  float qscale[NT], left_out = 0.0f;
+  // step s of tile t at ((t STEPS + s) 64 + lane) 16 bytes behind the digits
 #pragma unroll
-    for (int i = 0; i < QL; ++i)
-      if (i * kThreads + tid < NT * STEPS * 64) *(u32x4*)(lds + (i * kThreads + tid) * 4) = qr[i];
-  } else {
-    // digits (see query_digits): number n of 64 values i of tile t at (((t DIGITS + n) KL + i) 64 + lane) 16 bytes
-    constexpr uint32_t LEAST = 0x04000000u;  // (2^-119: 127 over it is a number)
+  for (int i = 0; i < QL; ++i)
+    if (i * kThreads + tid < NT * STEPS * 64) *(u32x4*)(lds + DF + (i * kThreads + tid) * 4) = qr[i];
+  if constexpr (Q8) {
+    // digit n of 64 values i of tile t at (((t DIGITS + n) KL + i) 64 + lane) 16 bytes
+    constexpr uint32_t LEAST = 21;  // (exponent of 2^-106: 2^21 over it is a number)
     uint32_t* most = (uint32_t*)(lds + QF);  // the rows' largest, as bits
-    if (tid < NT * 16) most[tid] = 0u;
+    uint32_t* lost = most + NT * 16;         // what their digits leave out, in 2^-8 of the last one's unit
+    if (tid < NT * 32) most[tid] = 0u;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < QL; ++i) {
@@ -367,36 +373,45 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
     for (int i = 0; i < QL; ++i) {
       int row, s, l;
       if (!q_at(i, row, s, l)) continue;
-      const float inv = 127.0f / bitcast<float>(max(most[row], LEAST));
+      // to whole numbers of at most 2^22
+      const float to = bitcast<float>((275u - max(most[row] >> 23, LEAST)) << 23);
       uint32_t w[DIGITS][2] = {};
+      float rest = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float r = T::get((uint16_t)(qr[i][e / 2] >> (16 * (e % 2)))) * inv;
+        const float x = fminf(fmaxf(T::get((uint16_t)(qr[i][e / 2] >> (16 * (e % 2)))) * to, -0x1p22f), 0x1p22f);
+        const float whole = rintf(x);
+        rest += fabsf(x - whole);
+        // bytes of the number with 128 added to the lower two, and taken off again
+        const uint32_t d = ((uint32_t)(int)whole + 0x8080u) ^ 0x8080u;
 #pragma unroll
-        for (int n = 0; n < DIGITS; ++n) {
-          const float d = fminf(fmaxf(rintf(r), -127.0f), 127.0f);
-          r = (r - d) * 254.0f;
-          w[n][e / 4] |= ((uint32_t)(int)d & 0xFFu) << (8 * (e % 4));
-        }
+        for (int n = 0; n < DIGITS; ++n) w[n][e / 4] |= (d >> (8 * (DIGITS - 1 - n)) & 0xFFu) << (8 * (e % 4));
       }
+      if (rest > 0.0f) atomicAdd(lost + row, (uint32_t)ceilf(rest * 256.0f));
       const int t = row / 16;
 #pragma unroll
       for (int n = 0; n < DIGITS; ++n)
         *(u32x2*)((uint32_t*)lds + (((t * DIGITS + n) * KL + s / 2) * 64 + l) * 4 + 2 * (s % 2)) = u32x2{w[n][0], w[n][1]};
     }
+    __syncthreads();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint32_t top = most[16 * t + j];
+      const uint32_t exponent = most[16 * t + j] >> 23;
       // (a query that is not finite makes numbers of no score)
-      qscale[t] = top < 0x7F800000u ? bitcast<float>(max(top, LEAST)) / 127.0f * a.c : __builtin_nanf("");
+      const float unit = bitcast<float>((max(exponent, LEAST) - 5u) << 23) * a.c;
+      qscale[t] = exponent < 255u ? unit : __builtin_nanf("");
+      if (exponent < 255u) left_out = fmaxf(left_out, (float)lost[16 * t + j] * (128.0f * 0x1p-24f) * unit);
     }
+    left_out = wave_max(left_out);
   }
   __syncthreads();
-  float* lsc = lds + QF + NT * 16 + wave * 64;
+  const f32x4* lq = (const f32x4*)(lds + DF) + lane;
+  float* lsc = lds + QF + NT * 32 + wave * 64;
   for (; blk < blk1; blk += kWaves) {
     const bool more = blk + kWaves < blk1;
     f32x4 S[NT][2];
     f32x4 ks[2], vs[2];
+    bool exact = false;
     if constexpr (Q8) {
       // a scale that is not finite makes no number of its key's score (an infinite one of a negative score
       // would leave its key out)
@@ -405,6 +420,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
         odd |= odd >> 32 | odd << 32;
         if (odd >> lane & 1) sc = lane < 32 ? __builtin_nanf("") : 0.0f;
       }
+      exact = __any(lane < 32 && fabsf(sc) * left_out > kLeftOut);
       // (a wave's LDS instructions take effect in order)
       lsc[lane] = sc;
       __builtin_amdgcn_wave_barrier();
@@ -415,7 +431,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
       }
       __builtin_amdgcn_wave_barrier();
     }
-    if constexpr (Q8) {
+    if (Q8 && !exact) {
       // the codes as they are, times each digit of the queries: whole numbers
       const u32x4* lw = (const u32x4*)lds + lane;
 #pragma unroll
@@ -432,7 +448,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            S[t][h][e] = fmaf(fmaf((float)D[2][e], 1.0f / 254.0f, (float)D[1][e]), 1.0f / 254.0f, (float)D[0][e]) * ks[h][e];
+            S[t][h][e] = fmaf(fmaf((float)D[2][e], 0x1p-8f, (float)D[1][e]), 0x1p-8f, (float)D[0][e]) * ks[h][e];
         }
     } else {
 #pragma unroll
@@ -443,9 +459,26 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
 #pragma unroll
         for (int t = 0; t < NT; ++t) qv[t] = bitcast<u32x4>(lq[(t * STEPS + s) * 64]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          u32x4 k;
+          if constexpr (Q8) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) S[t][h] = T::mma16(kr[h][s], qv[t], S[t][h]);
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t w = kr[h][s / 2][2 * (s % 2) + e / 2] >> (16 * (e % 2));
+              k[e] = T::pack_exact((float)(int8_t)w, (float)(int8_t)(w >> 8));
+            }
+          } else {
+            k = kr[h][s];
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) S[t][h] = T::mma16(k, qv[t], S[t][h]);
+        }
+      }
+      if constexpr (Q8) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) S[t][h] *= ks[h];
       }
     }
     if (more) load_k(blk + kWaves, pin);
@@ -465,10 +498,12 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float x[8];
+      float cs = a.c;
+      if constexpr (Q8) cs = exact && qscale[t] == qscale[t] ? a.c : qscale[t];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[4 * h + i] = S[t][h][i] * (Q8 ? qscale[t] : a.c);
+        for (int i = 0; i < 4; ++i) x[4 * h + i] = S[t][h][i] * cs;
       if (last) {
 #pragma unroll
         for (int s = 0; s < 8; ++s)
