@@ -29,8 +29,9 @@ extern "C" {
  * gives zeros; sequences of no group (behind cu_seq[G]) are left as they were.  What qlin_attn.h
  * states of strides, limits, lengths, pages and scales holds here too; cu_seq is clamped to the sequences
  * there are, and bounds that fall count as the highest before them.  Over int8 keys a weight of the softmax may
- * be off by 2^-16 of itself more than over 16-bit ones, whatever sizes a query's values have.  A call's query values (B x q_heads x
- * hd) are at most about 2^24, as the workspace holds 32-bit sums of each twice. */
+ * be off by 2^-16 of itself more than over 16-bit ones, whatever sizes a query's values have.
+ * A call's query values (B x q_heads x hd) are at most about 2^24, whatever groups the sequences are in, as the
+ * workspace holds 32-bit sums of each twice, and those of a cut (a tile of up to 128 rows of each key head). */
 int qlin_attn_decode_shared(const void* q, int64_t q_seq, int64_t q_head, const qlin_paged_kv* cache,
                             const int* prefix_table, int64_t prefix_table_stride, int max_prefix_pages,
                             const int* prefix_len, const int* cu_seq, int G,

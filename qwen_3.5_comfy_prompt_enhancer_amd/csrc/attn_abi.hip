@@ -245,22 +245,23 @@ int plan_shared(const char* fn, SharedArgs& a, int hd, int page, char* part, siz
   if (const char* e = getenv("QLIN_SHARED_UNITS")) {  // for tuning runs
     if (atoi(e) > 0) few = total = atoi(e);
   }
-  const long long tiles = a.B / a.spt + a.G;  // units of a prefix that is not cut
+  const long long tiles = a.B / a.spt + std::min(a.B, a.G);  // units of prefixes that are not cut
   const long long bound = tiles * ((keys + 4 * kSharedBlock - 1) / (4 * kSharedBlock)) +
                           a.B * ((own + 4 * kSharedBlock - 1) / (4 * kSharedBlock));
   long long target = std::min(std::max(1LL, total / a.HKV), bound);
-  // every unit leaves its rows' sums: at most target + tiles of prefixes, target + B own ones (and two more
-  // for what the device's estimate rounds); fewer where that is more than the workspace holds
-  const long long row = (long long)hd * 4 + 8, unit = (long long)(a.spt + 1) * a.R;
-  const long long fixed = ((tiles + 2) * a.spt + a.B + 2) * a.R;
-  target = std::min(target, ((long long)avail / row / a.HKV - fixed) / unit);
+  // Every unit leaves its rows' sums: a tile's and a sequence's uncut work, and at most `target` cuts.  (A group's
+  // parts lie next to each other without room between them; a cut of a prefix leaves those of a tile's sequences.  Cuts are
+  // whole numbers below total / chunk, in which total's rounding in 32 bits is less than a tenth.)  Fewer cuts where that is
+  // more than the workspace holds.
+  const long long row = (long long)hd * 4 + 8, cut = std::min(a.spt, a.B);
+  target = std::min(target, ((long long)avail / row / a.HKV / a.R - 2LL * a.B) / (cut + 1));
   if (target < 1)
     return fail(QLIN_ERR_UNSUPPORTED, "%s: %d sequences of %d query heads are more than the workspace holds sums of", fn,
                 a.B, a.HKV * a.R);
   a.target = (int)target;
   a.few = (int)std::min(std::max(1LL, few / a.HKV), target);
-  a.own_rows = (target + tiles + 2) * a.spt * a.R;
-  a.rows = a.own_rows + (target + a.B + 2) * a.R;
+  a.own_rows = (target * cut + a.B) * a.R;
+  a.rows = a.own_rows + (target + a.B) * a.R;
   const long long units = target + tiles + a.B + 2;
   QA_TRY(check_grid(fn, units * a.HKV));
   QA_TRY(check_grid(fn, (long long)a.B * a.HKV * a.R));

@@ -101,7 +101,7 @@ struct SharedArgs {
   int tiles;              // 16-row tiles of a prefix's unit: 1, 2, or 8 in the wide form
   int spt;                // sequences of a prefix's unit
   float c;                // scale * log2(e)
-  int target, few;        // units of a key head that long and short work is cut into
+  int target, few;        // cuts of a key head's long and short work
   int brief;              // blocks of a unit up to which work is short
   int units;              // units per key head: the grid's bound
   long long own_rows;     // rows of parts of a key head in front of the own ones

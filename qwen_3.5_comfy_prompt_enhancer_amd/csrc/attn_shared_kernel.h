@@ -124,7 +124,7 @@ struct Unit {
   int src, len;
   int b0, n;
   int blk0, blk1;
-  int slot;     // number of its part among the prefix's, or the own ones
+  int row;      // of its key head's: the first one of its sums
 };
 
 // Tiles of one part (t) lie 8 parts apart, so that they run on one XCD at about the same time: the
@@ -137,27 +137,30 @@ __device__ __forceinline__ void part_tile(int i, int parts, int tiles, int& part
 }
 
 __device__ __forceinline__ bool find_unit(const SharedArgs& a, const Plan& p, int u, Unit& r) {
-  int base = 0, start = 0;
+  int base = 0, start = 0, rows = 0;
   for (int g0 = 0; g0 < a.G; g0 += 64) {
     const Group g = group_of(a, groups_at(a, p, g0), start);
     const int tiles = tiles_of(a, g), parts = parts_of(p, g.len);
     const int end = wave_scan(tiles * parts), sum = lane_value(end, 63);
+    const int sums = wave_scan(parts * g.n);
     if (u < base + sum) {
       const int at = __builtin_ctzll(__ballot(base + end > u));
-      const int nt = lane_value(tiles, at), np = lane_value(parts, at), first = base + lane_value(end, at) - nt * np;
+      const int n = lane_value(g.n, at), nt = lane_value(tiles, at), np = lane_value(parts, at);
+      const int first = base + lane_value(end, at) - nt * np;
       int part, tile;
       part_tile(u - first, np, nt, part, tile);
       r.prefix = 1;
       r.src = g0 + at;
       r.len = lane_value(g.len, at);
       r.b0 = lane_value(g.b0, at) + tile * a.spt;
-      r.n = min(a.spt, lane_value(g.n, at) - tile * a.spt);
+      r.n = min(a.spt, n - tile * a.spt);
       r.blk0 = part * p.chunk;
-      r.slot = first + tile * np + part;
+      r.row = (rows + lane_value(sums, at) + (part - np) * n + tile * a.spt) * a.R;
       r.blk1 = min(blocks_of(r.len), r.blk0 + p.chunk);
       return true;
     }
     base += sum;
+    rows += lane_value(sums, 63);
   }
   int own = 0;
   for (int b0 = 0; b0 < p.hi; b0 += 64) {
@@ -170,7 +173,7 @@ __device__ __forceinline__ bool find_unit(const SharedArgs& a, const Plan& p, in
       r.src = r.b0 = b0 + at;
       r.n = 1;
       r.len = lane_value(len, at);
-      r.slot = u - base;
+      r.row = (int)a.own_rows + (u - base) * a.R;
       r.blk0 = (u - base - own - lane_value(end, at) + lane_value(parts, at)) * p.chunk;
       r.blk1 = min(blocks_of(r.len), r.blk0 + p.chunk);
       return true;
@@ -217,11 +220,6 @@ constexpr float kLeftOut = 0x1p-16f;
 template <typename T>
 __device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
   return T::pack_exact((float)(int8_t)(w0 >> (8 * c)), (float)(int8_t)(w1 >> (8 * c)));
-}
-
-// The first row of a unit's part.
-__device__ __forceinline__ long long part_row(const SharedArgs& a, const Unit& U, int hk) {
-  return (long long)hk * a.rows + (U.prefix ? (long long)U.slot * (a.spt * a.R) : a.own_rows + (long long)U.slot * a.R);
 }
 
 // Dynamic LDS: the queries of NT tiles as operands (int8 keys: digits, and as they are); behind the loop the waves' sums of
@@ -599,7 +597,7 @@ __device__ __forceinline__ void run_unit(const SharedArgs& a, const Unit& U, int
   // (rows HD + 4 apart: the 16 of a tile start in different banks; HD apart the stores took 3 us more)
   constexpr int ST = HD + 4;
   float* mlw = lds + kWaves * 16 * ST;
-  const long long row0 = part_row(a, U, hk);
+  const long long row0 = (long long)hk * a.rows + U.row;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int n = min(16, rows - 16 * t);
@@ -978,7 +976,7 @@ __device__ __forceinline__ void wide_unit(const SharedArgs& a, const Unit& U, in
   float x, y;
   lane_pair<32>(l, x, y);
   l = any_bad ? __builtin_nanf("") : x + y;
-  const long long at = part_row(a, U, hk) + mine;
+  const long long at = (long long)hk * a.rows + U.row + mine;
   float* o = a.part + at * HD + 4 * half;
 #pragma unroll
   for (int d = 0; d < G::ND; ++d)
@@ -1004,7 +1002,7 @@ __global__ __launch_bounds__(kThreads, shared_occupancy(HD, NT)) void shared_ker
   const Plan p = make_plan(a);
   Unit U;
   if (!find_unit(a, p, unit, U)) return;
-  for (int* x : {&U.prefix, &U.src, &U.len, &U.b0, &U.n, &U.blk0, &U.blk1, &U.slot}) *x = (int)rfl32((uint32_t)*x);
+  for (int* x : {&U.prefix, &U.src, &U.len, &U.b0, &U.n, &U.blk0, &U.blk1, &U.row}) *x = (int)rfl32((uint32_t)*x);
   if constexpr (NT == 0) {
     if (U.prefix || a.R > 16) {
       wide_unit<T, HD, Q8>(a, U, hk, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
@@ -1032,22 +1030,20 @@ __global__ __launch_bounds__(THREADS) void shared_join_kernel(const SharedArgs a
   const int head = ((int)blockIdx.x - u * runs) * ROWS + rr;
   const Plan p = make_plan(a);
   if (b < p.lo || b >= p.hi) return;  // a row of no group
-  // parts of the prefix: slots pslot, pslot + 1, ..., row prow of each
-  int base = 0, start = 0, pslot = 0, np = 0, prow = 0;
+  // parts of the prefix: row prow of the first, pn rows to the next
+  int start = 0, prow = 0, pn = 0, np = 0;
   for (int g0 = 0; g0 < a.G; g0 += 64) {
     const Group g = group_of(a, groups_at(a, p, g0), start);
-    const int tiles = tiles_of(a, g), parts = parts_of(p, g.len);
-    const int end = wave_scan(tiles * parts);
+    const int parts = parts_of(p, g.len), sums = wave_scan(parts * g.n);
     const uint64_t mine = __ballot(b >= g.b0 && b < g.b0 + g.n);
     if (mine) {
       const int at = __builtin_ctzll(mine);
-      const int nt = lane_value(tiles, at), in = b - lane_value(g.b0, at);
-      np = nt ? lane_value(parts, at) : 0;
-      pslot = base + lane_value(end, at) - nt * np + in / a.spt * np;
-      prow = in % a.spt * a.R;
+      np = lane_value(parts, at);
+      pn = lane_value(g.n, at);
+      prow += lane_value(sums, at) - np * pn + b - lane_value(g.b0, at);
       break;
     }
-    base += lane_value(end, 63);
+    prow += lane_value(sums, 63);
   }
   int oslot = 0, no = 0;
   for (int b0 = 0; b0 < p.hi; b0 += 64) {
@@ -1062,10 +1058,10 @@ __global__ __launch_bounds__(THREADS) void shared_join_kernel(const SharedArgs a
   }
   const int hrow = min(head, a.R - 1);  // (rows behind the last are the last again, and not stored)
   const long long first = (long long)hk * a.rows;
-  const long long pre0 = first + (long long)pslot * (a.spt * a.R) + prow + hrow;
+  const long long pre0 = first + (long long)prow * a.R + hrow;
   const long long own0 = first + a.own_rows + (long long)oslot * a.R + hrow;
   const int n = np + no;
-  auto row_of = [&](int i) { return i < np ? pre0 + (long long)i * (a.spt * a.R) : own0 + (long long)(i - np) * a.R; };
+  auto row_of = [&](int i) { return i < np ? pre0 + (long long)i * (pn * a.R) : own0 + (long long)(i - np) * a.R; };
   f32x4 o = {0, 0, 0, 0};
   float M = kNegInf, ls = 0.0f;
   for (int i0 = s; i0 < n; i0 += SL * N) {
