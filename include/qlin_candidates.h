@@ -28,8 +28,10 @@ extern "C" {
  * out = softmax(scale q k^T) v over both.  Prefix and own keys lie in one cache.  A sequence without keys
  * gives zeros; sequences of no group (behind cu_seq[G]) are left as they were.  What qlin_attn.h
  * states of strides, limits, lengths, pages and scales holds here too; cu_seq is clamped to the sequences
- * there are, and bounds that fall count as the highest before them.  Over int8 keys a weight of the softmax may
- * be off by 2^-16 of itself more than over 16-bit ones, whatever sizes a query's values have.
+ * there are, and bounds that fall count as the highest before them.  Whatever sizes a query's values have and
+ * however many sequences see a key: over int8 keys a weight of the softmax may be off by 2^-16 of itself more
+ * than over 16-bit ones; with fp16 values one as far as 18 octaves below the heaviest of its 32 keys is rounded
+ * to fp16's 11 bits, a lighter one is off by at most 2^-29 of that heaviest.
  * A call's query values (B x q_heads x hd) are at most about 2^24, whatever groups the sequences are in, as the
  * workspace holds 32-bit sums of each twice, and those of a cut (a tile of up to 128 rows of each key head). */
 int qlin_attn_decode_shared(const void* q, int64_t q_seq, int64_t q_head, const qlin_paged_kv* cache,

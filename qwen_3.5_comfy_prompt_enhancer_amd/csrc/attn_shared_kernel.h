@@ -839,13 +839,15 @@ __device__ __forceinline__ void wide_unit(const SharedArgs& a, const Unit& U, in
     lane_pair<32>(mx, x, y);
     mx = fmaxf(x, y) * a.c;
     // (sums are rescaled only when a row's maximum has grown by more than 2^8, in fp16 when a block's largest P would
-    // leave 2^-8 .. 2^15 on either side)
+    // leave 2^4 .. 2^15 on either side: as for few rows, keys down to 18 octaves below it keep their weight.  From the window's
+    // middle, as one of a wave's 32 rows that leaves it costs them all: 64 sequences behind 16384 tokens of 128 values 46.6 us,
+    // from 2^14 48; a window from 2^-8, which holds 6 octaves, 44.8)
     constexpr bool NARROW = TV::DT == DT_F16;
-    if (NARROW ? __any(off_window(mx - m, -8.0f, 15.0f)) : __any(mx > m + 8.0f)) {
+    if (NARROW ? __any(off_window(mx - m, 4.0f, 15.0f)) : __any(mx > m + 8.0f)) {
       float mn = fmaxf(m, mx);
       if constexpr (NARROW) {
         lane_pair<32>(l, x, y);
-        mn = fp16_reference(m, mx, x + y, -8.0f, 8.0f, 15.0f);
+        mn = fp16_reference(m, mx, x + y, 4.0f, 9.0f, 15.0f);
       }
       const float al = exp2_(m - (mn == kNegInf ? 0.0f : mn));
       m = mn;
