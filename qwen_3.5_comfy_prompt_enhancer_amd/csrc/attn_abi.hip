@@ -511,6 +511,12 @@ int qlin_attn_decode_shared(const void* q, int64_t q_seq, int64_t q_head, const 
   QA_TRY(check_region(fn, to));
   QA_TRY(check_regions(fn, to, region("q", q, 2, hd, B, q_seq, q_heads, q_head)));
   QA_TRY(check_cache_apart(fn, to, cache, kv_heads, hd));
+  // (the second launch reads lengths and bounds again, beside workgroups that write)
+  const Region in[5] = {region("prefix_table", max_prefix_pages ? prefix_table : nullptr, 4, max_prefix_pages, G, prefix_table_stride, 1, 0),
+                        region("table", max_pages ? table : nullptr, 4, max_pages, B, table_stride, 1, 0),
+                        region("prefix_len", prefix_len, 4, G, 1, 0, 1, 0), region("kv_len", kv_len, 4, B, 1, 0, 1, 0),
+                        region("cu_seq", cu_seq, 4, G + 1, 1, 0, 1, 0)};
+  for (const Region& r : in) QA_TRY(check_regions(fn, to, r));
   char* part;
   size_t avail;
   QA_TRY(workspace_parts(fn, workspace, workspace_bytes, &part, &avail));
