@@ -228,9 +228,13 @@ int plan_prompt(const char* fn, PromptArgs& a, int hd, long long max_keys, void*
 int plan_shared(const char* fn, SharedArgs& a, int hd, int page, char* part, size_t avail) {
   const long long rows = (long long)((a.B + a.G - 1) / a.G) * a.R;  // of a prefix, on average
   // 17 to 32 rows take one unit of two tiles, or two of one, which read the keys twice (the second time from the L2) but
-  // come two to a CU (of 256 values) and more even: 8 sequences of 4 query heads to a key head, one / two tiles: of 256
-  // values behind 8000 tokens 17.8 / 20.0 us, 64000 40 / 48, 100003 65 / 55; of 128 behind 2000 10.7 / 11.7, 32000 21.8 /
-  // 21.4, six prompts of up to 6000 35 / 31.  int8 keys are cheaper read than two tiles are kept in registers.
+  // come two to a CU (of 256 values) and more even.  One / two tiles, us: of 256 values prefixes of 62 MB together 24.0 /
+  // 26.3, 125 MB 33.7 / 40.2, 195 MB 52.4 / 44.0; of 128 one of 31 MB 16.4 / 17.1, 46 MB 18.8 / 19.0, 93 MB 30.2 / 26.0, six of
+  // 23 MB 17.5 / 18.2, 70 MB 31.0 / 24.4; of 64 one of 11 MB 11.5 / 12.1, 23 MB 14.5 / 14.2, 48 MB 21.1 / 19.4, six of 17 MB
+  // 14.0 / 13.9, 35 MB 21.6 / 17.8.  int8 keys are cheaper read than two tiles are kept in registers.
+  // The average group's rows choose: one of 57 sequences beside seven of one takes 16-row tiles, and its prefix is loaded
+  // for each of them, from the L2 but for the first (8 + 2 heads of 256 behind 8000 tokens each: 48.8 us, in two calls 28.2
+  // and 26.7; eight of eight 34.7).
   const long long keys = std::max(1, a.pre.max_pages) * (long long)page, own = std::max(1, a.own.max_pages) * (long long)page;
   const bool q8 = a.own.k.s != nullptr;
   const long long bytes = (long long)a.G * keys * a.HKV * hd * 4;
@@ -238,8 +242,12 @@ int plan_shared(const char* fn, SharedArgs& a, int hd, int page, char* part, siz
   a.tiles = a.R > 16 || rows > 32 ? 8 : two ? 2 : 1;
   a.spt = 16 * a.tiles / a.R;
   // One workgroup a CU as long as that makes units of at most `brief` blocks: more of them read no faster and leave more
-  // sums to join (8 sequences behind 32000 tokens of 256 values, 256 / 512 units: 25 / 31 us).  Where vector work bounds
-  // a wide unit (int8 keys, 64 values), three (64 sequences behind 16384 int8 keys of 256 values 54 -> 43 us).
+  // sums to join (8 sequences behind 32000 tokens of 256 values, 256 / 512 units: 23.8 / 29.2 us).  Where vector work bounds
+  // a wide unit (int8 keys, 64 values), three: 64 sequences behind 16384 tokens with 30 and with 1000 keys of their own, 512 and
+  // 768 units: int8 of 256 values 48.2 / 50.6 and 70.0 / 48.1, of 128 64.0 / 57.4 and 66.6 / 65.5, of 64 60.7 / 50.9 and 62.3 /
+  // 60.7, 16 bits of 64 38.2 / 34.1 and 38.2 / 39.9; not so 16 bits of 128 41.9 / 43.0 and 49.7 / 50.1, of 256 34.2 / 44.3 and
+  // 52.1 / 51.2.  (512 instead of 256 for those: 40.5 and 49.5, 33.4 and 46.2; behind 50000 tokens 76.1 / 75.3, 52.8 / 55.8.
+  // Where own keys are most of the work finer cuts would be better: 1000 of each behind 1000 tokens, 256 / 768 units: 45 / 31.)
   long long few = a.tiles == 8 && (q8 || hd == 64) ? 768 : 256, total = two && hd == 256 ? 256 : std::max(512LL, few);
   a.brief = q8 ? 24 : 32;
   if (const char* e = getenv("QLIN_SHARED_UNITS")) {  // for tuning runs

@@ -6,9 +6,9 @@
 //
 // Bound by the bytes of the cache where prefixes are long and a group's rows (sequences x query heads of a key
 // head) few: a prefix's keys are read once for all rows of a tile, further tiles over the same keys meet them in
-// the L2.  8 sequences behind 100003 tokens of two key heads of 256 values: 54 us (4.0 TB/s), int8 45 us, bound by
+// the L2.  8 sequences behind 100003 tokens of two key heads of 256 values: 45 us (4.5 TB/s), int8 42 us, bound by
 // the vector instructions that widen values.  Where little is read, latency bounds it: 4 candidates of a prompt of
-// 180 tokens 12.0 us, of which 2 go to finding a workgroup's unit, 3.6 to its first loads, 5 to the second launch.
+// 180 tokens 12.1 us, of which 2 go to finding a workgroup's unit, 3.6 to its first loads, 5 to the second launch.
 //
 // Work units are runs of 32-key blocks, of a prefix for a tile of whole sequences, or of one sequence's own keys;
 // lengths are on the device alone, so every workgroup makes the same plan from them and finds its unit in it.
@@ -20,10 +20,12 @@
 //     - P^T leaves the score layout as the B operand of O^T = V^T P^T without crossing lanes: lane group g holds
 //       keys 4g .. 4g+3 and 16 + 4g .. 16 + 4g+3 of the block, and V's rows are loaded in that order;
 //     - V: a lane loads 8 keys' next hd/16 values; byte permutes pair the keys of a column, once for all tiles;
-//     - int8 keys stay whole numbers and meet the queries' digits where those hold them (see DIGITS); values become 16-bit whole numbers
-//       (exact), a key's scale multiplies its scores in 32 bits, a value's its probability.
-//   * wide (wide_unit): 128 rows, 32 of each wave, over keys that land in LDS for all four.  64 sequences behind
-//     16384 tokens, 32 query heads of 128 values to 4 key heads: 58 us, in tiles of 32 rows 91.
+//     - int8 keys stay whole numbers and meet the queries' digits where those hold them (see DIGITS); values become
+//       16-bit whole numbers (exact), a key's scale multiplies its scores in 32 bits, a value's its probability.
+//   * wide (wide_unit): 128 rows, 32 of each wave, over keys that land in LDS for all four.  64 sequences of 30 keys of their own
+//     behind 16384 tokens, 32 query heads of 128 values to 4 key heads: 42 us, in tiles of 32 rows 54; of 1000 50 and 66.  int8
+//     keys are written to LDS again as 16-bit numbers (a second barrier a block): 58 and 66 us, of 8 + 2 heads of 256 51 and 48,
+//     where 16-bit ones take 33 and 52.
 // The running maximum (the reference that P is taken against) is a column's, hence a lane's own.  P is
 // rounded to 16 bits for its product (half a step of each term; the sum of P is of the unrounded), in fp16
 // against a reference that follows the scores (fp16_reference); with int8 values P times scale goes as
