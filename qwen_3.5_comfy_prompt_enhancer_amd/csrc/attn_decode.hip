@@ -90,31 +90,9 @@ __device__ __forceinline__ bool find_unit(const DecodeArgs& a, int u, Unit& r) {
   return false;
 }
 
-__device__ __forceinline__ float group_max(float v) {  // over the four lanes of a column
-  float x, y;
-  lane_pair<16>(v, x, y);
-  v = fmaxf(x, y);
-  lane_pair<32>(v, x, y);
-  return fmaxf(x, y);
-}
-
-__device__ __forceinline__ float group_sum(float v) {
-  float x, y;
-  lane_pair<16>(v, x, y);
-  v = x + y;
-  lane_pair<32>(v, x, y);
-  return x + y;
-}
-
 // Dwords of codes that the compiler must not take apart before they are used (it would carry
 // single bytes, a register each, around the loop).
 __device__ __forceinline__ void opaque(uint32_t& a, uint32_t& b) { asm volatile("" : "+v"(a), "+v"(b)); }
-
-// Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
-template <typename T>
-__device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
-  return T::pack_exact((float)(int8_t)(w0 >> (8 * c)), (float)(int8_t)(w1 >> (8 * c)));
-}
 
 // n values of a part, four at a time (float4 f of `rows * HD / 4`), and a row's maximum and sum
 // behind them: a part's layout in memory.

@@ -106,10 +106,33 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(x, y);
 }
 
+// Over the four lanes of a column of 16x16 scores.
+__device__ __forceinline__ float group_max(float v) {
+  float x, y;
+  lane_pair<16>(v, x, y);
+  v = fmaxf(x, y);
+  lane_pair<32>(v, x, y);
+  return fmaxf(x, y);
+}
+
+__device__ __forceinline__ float group_sum(float v) {
+  float x, y;
+  lane_pair<16>(v, x, y);
+  v = x + y;
+  lane_pair<32>(v, x, y);
+  return x + y;
+}
+
 // The value of one lane (a uniform number), the same on all.
 template <typename N>
 __device__ __forceinline__ N lane_value(N v, int at) {
   return bitcast<N>(__builtin_amdgcn_readlane(bitcast<int>(v), at));
+}
+
+// Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
+  return T::pack_exact((float)(int8_t)(w0 >> (8 * c)), (float)(int8_t)(w1 >> (8 * c)));
 }
 
 // 2^x; of -inf (nothing seen yet, or scores of -inf alone) zero.

@@ -185,22 +185,6 @@ __device__ __forceinline__ bool find_unit(const SharedArgs& a, const Plan& p, in
   return false;
 }
 
-__device__ __forceinline__ float group_max(float v) {  // over the four lanes of a column
-  float x, y;
-  lane_pair<16>(v, x, y);
-  v = fmaxf(x, y);
-  lane_pair<32>(v, x, y);
-  return fmaxf(x, y);
-}
-
-__device__ __forceinline__ float group_sum(float v) {
-  float x, y;
-  lane_pair<16>(v, x, y);
-  v = x + y;
-  lane_pair<32>(v, x, y);
-  return x + y;
-}
-
 // Dwords of codes that the compiler must not take apart before they are used (it would carry
 // single bytes, a register each, around the loop).
 __device__ __forceinline__ void opaque(uint32_t& a) { asm volatile("" : "+v"(a)); }
@@ -217,12 +201,6 @@ __device__ __forceinline__ void opaque(u32x4& a) { asm volatile("" : "+v"(a)); }
 // the queries as they are: rows of very different values, whose large ones may meet codes of zero.
 constexpr int DIGITS = 3;
 constexpr float kLeftOut = 0x1p-16f;
-
-// Codes of byte column c (0-3 of dword w) of two keys as a pair of 16-bit numbers.
-template <typename T>
-__device__ __forceinline__ uint32_t codes2(uint32_t w0, uint32_t w1, int c) {
-  return T::pack_exact((float)(int8_t)(w0 >> (8 * c)), (float)(int8_t)(w1 >> (8 * c)));
-}
 
 // Dynamic LDS: the queries of NT tiles as operands (int8 keys: digits, and as they are); behind the loop the waves' sums of
 // a tile.
