@@ -22,7 +22,8 @@ extern "C" {
 
 /* One query per sequence, q and out [B][q_heads][hd].  Sequences come in G groups: group g's are
  * cu_seq[g] .. cu_seq[g+1] - 1, and all of them see the first prefix_len[g] tokens of pages
- * prefix_table[g][0 .. max_prefix_pages - 1], which are read once for the group, and then their own first
+ * prefix_table[g][0 .. max_prefix_pages - 1], which are read from memory once for the group (by tiles of 16 to
+ * 128 query rows, chosen by the average group, that meet in the L2 caches), and then their own first
  * kv_len[b] tokens of pages table[b][0 .. max_pages - 1] (the new one among them; a table of no pages may
  * be NULL):
  * out = softmax(scale q k^T) v over both.  Prefix and own keys lie in one cache.  A sequence without keys
